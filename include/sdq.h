@@ -173,6 +173,84 @@ int sdq_quantized_matmul_epilogue(const void* x, sdq_dtype x_dtype, int64_t m, i
                                   void* stream);
 
 /*
+ * ---- Block-scaled 8-bit floating point (e4m3 values, e8m0 scales) ----
+ *
+ * A second quantised form beside the affine one: each value is one e4m3 byte (largest 448, no
+ * infinities, 0x7F NaN) and every 128 values along k share a scale 2^(byte - 127), one e8m0 byte
+ * (255: NaN).  Scales are powers of two, so x / scale is exact and a value is rounded once; the
+ * tensor cores multiply the scales in.  Of `a` = max |x| over the block the scale is 2^e with the
+ * least integer e >= -126 for which a <= 448 * 2^e.  A block that holds an infinity or a NaN has
+ * scale 255 and all its codes 0x7F: it stands for NaN.
+ *
+ *   xq [m, k], x_scales [ceil(k/128), m]             activations: 128 values of a row share a scale
+ *   wq [n, k], w_scales [ceil(n/128), ceil(k/128)]   weights: 128 x 128 values share one
+ *
+ * k is a multiple of 16 (rows start on 16 bytes); the last block of a row or column may be shorter.
+ * No counterpart in the reference, whose quantised weights are affine integers.
+ */
+
+/* Activations x [m,k] (bf16 or f32, 16-byte aligned, as xq) -> xq, x_scales.  m may be 0. */
+int sdq_fp8_quantize(const void* x, sdq_dtype x_dtype, int64_t m, int64_t k, uint8_t* xq, uint8_t* x_scales,
+                     void* stream);
+
+/* A weight w [n,k] (bf16 or f32, 16-byte aligned, as wq) -> wq, w_scales.  Load time. */
+int sdq_fp8_quantize_weight(const void* w, sdq_dtype w_dtype, int64_t n, int64_t k, uint8_t* wq,
+                            uint8_t* w_scales, void* stream);
+
+/*
+ * The values that codes and scales stand for, rounded once to out_dtype (bf16 or f32): out [rows,k].
+ * weight non-zero: scales are a weight's 128 x 128 ones, otherwise an activation's.
+ */
+int sdq_fp8_dequantize(const uint8_t* q, const uint8_t* scales, int64_t rows, int64_t k, int weight, void* out,
+                       sdq_dtype out_dtype, void* stream);
+
+/*
+ * y[t,f] = residual[t,f] + gate[f] * act( sum_k X[t,k] W[f,k] + bias[f] ), X and W the values that
+ * xq / x_scales and wq / w_scales stand for; products and sums in f32, one rounding to y_dtype.
+ * bias, gate, residual may be NULL (0, 1, 0); act is one of SDQ_ACT_*.  With y bf16, bias and gate
+ * are [n] bf16 and residual [m,n] bf16 (residual may be y itself, but not otherwise overlap it).
+ * With y f32 only a bias ([n] f32) may be given.  m may be 0.  xq and wq are 16-byte aligned.
+ */
+int sdq_fp8_matmul(const uint8_t* xq, const uint8_t* x_scales, int64_t m, int64_t k, const uint8_t* wq,
+                   const uint8_t* w_scales, int64_t n, const void* bias, int act, const void* gate,
+                   const void* residual, void* y, sdq_dtype y_dtype, void* stream);
+
+/* ---- Queries, keys and values made ready for attention ---- */
+
+/* A tensor of head vectors [batch, tokens, heads, head_dim] anywhere in device memory: strides in
+ * elements, the last axis contiguous. */
+typedef struct sdq_heads {
+    void* data;
+    int64_t heads;
+    int64_t batch_stride, token_stride, head_stride;
+} sdq_heads;
+
+/*
+ * In one pass over q, k and v: RMS norm of every query and key head (q_weight, k_weight [head_dim],
+ * NULL: no norm), rotation of its first rope_dim values by the cosines and sines of the token's
+ * position, and the copy of all three to wherever q_out, k_out and v_out lie -- a contiguous
+ * [batch, heads, tokens, head_dim], or a part of a longer sequence.  Computed in f32, rounded once.
+ *
+ * cos and sin are [table_rows, rope_dim/2] f32; a token's row is its index, or positions[b, t]
+ * (int32 or int64, rows pos_batch_stride elements apart).  A position outside the tables makes that
+ * token's queries and keys NaN.  interleaved non-zero: pairs (x[2i], x[2i+1]), otherwise
+ * (x[i], x[i + rope_dim/2]).  v may be NULL, and q or k have 0 heads, to leave them out.
+ *
+ * dtype (bf16 or f32) is that of the vectors and of the norm's weights.  head_dim is a multiple of 8
+ * up to 256; rope_dim (0: no rotation) a multiple of 16, at most head_dim.  Bases and strides keep
+ * every vector, and the tables their rows, 16-byte aligned.  An output may be its own input (same
+ * address, same strides); otherwise outputs overlap neither inputs nor each other.
+ *
+ * Replaces the reference's split_qkv, qk_norm, concatenation and rotate between the qkv linear and
+ * attention (crates/sd-models/src/mlx/flux.rs:302-329, 165-212).
+ */
+int sdq_qk_norm_rope(const sdq_heads* q, const sdq_heads* k, const sdq_heads* v, const sdq_heads* q_out,
+                     const sdq_heads* k_out, const sdq_heads* v_out, sdq_dtype dtype, int64_t batch,
+                     int64_t tokens, int head_dim, const void* q_weight, const void* k_weight, float eps,
+                     const float* cos, const float* sin, int64_t table_rows, int rope_dim, int interleaved,
+                     const void* positions, int positions_are_64_bit, int64_t pos_batch_stride, void* stream);
+
+/*
  * Bytes a quantised [n,k] weight occupies, packed words plus scales and
  * biases, with sb_bytes per scale/bias element (the reference counts 4,
  * mlx.rs:1981-1985; this library stores bf16, 2).  Returns 0 on invalid

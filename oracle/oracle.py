@@ -342,3 +342,78 @@ def synthetic_linear(seed: int, m: int, k: int, n: int, sigma_w: float, sigma_x:
     x = (vals[: m * k] * np.float32(sigma_x)).astype(np.float32).reshape(m, k)
     w = (vals[m * k:] * np.float32(sigma_w)).astype(np.float32).reshape(n, k)
     return f32_to_bf16_bits(x), w
+
+
+# ---------------------------------------------------------------- block-scaled e4m3 (NumPy only)
+FP8_BLOCK = 128
+
+
+def e4m3_values() -> np.ndarray:
+    """The 127 finite non-negative e4m3 numbers by code 0x00 .. 0x7E, in f64."""
+    c = np.arange(127)
+    e, m = c >> 3, (c & 7).astype(np.float64)
+    return np.where(e == 0, np.ldexp(m / 8, -6), np.ldexp(1 + m / 8, e - 7))
+
+
+def e4m3_encode(x: np.ndarray) -> np.ndarray:
+    """Nearest e4m3 code of f64 values with |x| <= 448 (ties to the even code), NaN -> 0x7F."""
+    v = e4m3_values()
+    a = np.abs(np.nan_to_num(x, nan=0.0))
+    hi = np.clip(np.searchsorted(v, a), 1, 126)
+    lo = hi - 1
+    dl, dh = a - v[lo], v[hi] - a
+    code = np.where((dl < dh) | ((dl == dh) & (lo % 2 == 0)), lo, hi).astype(np.uint8)
+    code |= (np.signbit(x).astype(np.uint8) << 7)
+    return np.where(np.isnan(x), np.uint8(0x7F), code)
+
+
+def e4m3_decode(code: np.ndarray) -> np.ndarray:
+    v = np.append(e4m3_values(), np.nan)
+    return np.where(code & 0x80, -1.0, 1.0) * v[code & 0x7F]
+
+
+def e8m0_decode(byte: np.ndarray) -> np.ndarray:
+    return np.where(byte == 255, np.nan, np.ldexp(1.0, byte.astype(np.int64) - 127))
+
+
+def _e8m0_of(amax: np.ndarray) -> np.ndarray:
+    """The byte of 2^e, e the least integer >= -126 with amax <= 448 * 2^e; 255 for inf and NaN."""
+    out = np.full(amax.shape, 255, np.uint8)
+    for i, a in np.ndenumerate(amax):
+        if np.isfinite(a):
+            e = -126
+            while a > np.ldexp(448.0, e):
+                e += 1
+            out[i] = e + 127
+    return out
+
+
+def _fp8_blocks(x: np.ndarray, rows: int):
+    """Codes of x [R, K] and one byte for each `rows` x 128 block, [blocks of rows, blocks of K]."""
+    r, k = x.shape
+    rb, kb = -(-r // rows), -(-k // FP8_BLOCK)
+    p = np.zeros((rb * rows, kb * FP8_BLOCK))
+    p[:r, :k] = x
+    p = p.reshape(rb, rows, kb, FP8_BLOCK)
+    with np.errstate(invalid="ignore"):
+        byte = _e8m0_of(np.max(np.abs(p), axis=(1, 3)))
+        q = e4m3_encode(np.where((byte == 255)[:, None, :, None], np.nan, p / e8m0_decode(byte)[:, None, :, None]))
+    return q.reshape(rb * rows, kb * FP8_BLOCK)[:r, :k], byte
+
+
+def fp8_quantize(x: np.ndarray):
+    """x [M, K] f64 -> codes u8 [M, K], scale bytes [ceil(K/128), M]."""
+    q, byte = _fp8_blocks(x, 1)
+    return q, np.ascontiguousarray(byte.T)
+
+
+def fp8_quantize_weight(w: np.ndarray):
+    """w [N, K] f64 -> codes u8 [N, K], scale bytes [ceil(N/128), ceil(K/128)]."""
+    return _fp8_blocks(w, FP8_BLOCK)
+
+
+def fp8_dequantize(q: np.ndarray, byte: np.ndarray, weight: bool) -> np.ndarray:
+    """f64 values of codes [R, K]."""
+    s = e8m0_decode(byte) if weight else e8m0_decode(byte).T
+    rows = FP8_BLOCK if weight else 1
+    return e4m3_decode(q) * s.repeat(rows, 0).repeat(FP8_BLOCK, 1)[: q.shape[0], : q.shape[1]]

@@ -97,6 +97,21 @@ int check_nk(int64_t n, int64_t k, const char* fn) {
     return SDQ_OK;
 }
 
+// Shapes of block-scaled e4m3 operands: rows >= least, k >= 1 and a multiple of 16.
+int check_fp8_shape(int64_t rows, int64_t k, const char* what, int64_t least, const char* fn) {
+    if (rows < least || rows > INT32_MAX)
+        return fail(SDQ_ERR_INVALID, "%s: %s must be >= %lld and < 2^31; got %lld", fn, what, (long long)least,
+                    (long long)rows);
+    if (k <= 0 || k > INT32_MAX) return fail(SDQ_ERR_INVALID, "%s: k must be >= 1 and < 2^31; got %lld", fn, (long long)k);
+    if (k % 16 != 0)
+        return fail(SDQ_ERR_INVALID, "%s: k = %lld is not a multiple of 16 (such weights stay dense)", fn, (long long)k);
+    return SDQ_OK;
+}
+int check_fp8_source(sdq_dtype d, const char* fn) {
+    if (d == SDQ_BF16 || d == SDQ_F32) return SDQ_OK;
+    return fail(SDQ_ERR_UNSUPPORTED, "%s: the unquantised side must be bf16 or f32 (dtype %d)", fn, (int)d);
+}
+
 }  // namespace
 
 int set_error_message(int code, const char* msg) {
@@ -455,6 +470,163 @@ int sdq_quantized_matmul_epilogue(const void* x, sdq_dtype x_dtype, int64_t m, i
     return run_qmm(x, m, k, wq, scales, biases, n, bits, epi, y, stream, fn);
 }
 
+int sdq_fp8_quantize(const void* x, sdq_dtype x_dtype, int64_t m, int64_t k, uint8_t* xq, uint8_t* x_scales,
+                     void* stream) {
+    const char* fn = "sdq_fp8_quantize";
+    int rc;
+    if ((rc = check_fp8_shape(m, k, "m (rows)", 0, fn)) || (rc = check_fp8_source(x_dtype, fn))) return rc;
+    if (m == 0) return ok();
+    if (!x || !xq || !x_scales) return fail(SDQ_ERR_INVALID, "%s: x, xq and x_scales must be non-null", fn);
+    if (!aligned(x, 16) || !aligned(xq, 16)) return fail(SDQ_ERR_INVALID, "%s: misaligned pointer (x and xq need 16 bytes)", fn);
+    if ((rc = check_device())) return rc;
+    cudaError_t e = launch_fp8_quantize(x, x_dtype == SDQ_BF16, m, k, xq, x_scales, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail("sdq_fp8_quantize: kernel launch", e);
+    return ok();
+}
+
+int sdq_fp8_quantize_weight(const void* w, sdq_dtype w_dtype, int64_t n, int64_t k, uint8_t* wq, uint8_t* w_scales,
+                            void* stream) {
+    const char* fn = "sdq_fp8_quantize_weight";
+    int rc;
+    if ((rc = check_fp8_shape(n, k, "n (rows, out features)", 1, fn)) || (rc = check_fp8_source(w_dtype, fn))) return rc;
+    if (!w || !wq || !w_scales) return fail(SDQ_ERR_INVALID, "%s: w, wq and w_scales must be non-null", fn);
+    if (!aligned(w, 16) || !aligned(wq, 16)) return fail(SDQ_ERR_INVALID, "%s: misaligned pointer (w and wq need 16 bytes)", fn);
+    if ((rc = check_device())) return rc;
+    cudaError_t e = launch_fp8_quantize_weight(w, w_dtype == SDQ_BF16, n, k, wq, w_scales, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail("sdq_fp8_quantize_weight: kernel launch", e);
+    return ok();
+}
+
+int sdq_fp8_dequantize(const uint8_t* q, const uint8_t* scales, int64_t rows, int64_t k, int weight, void* out,
+                       sdq_dtype out_dtype, void* stream) {
+    const char* fn = "sdq_fp8_dequantize";
+    int rc;
+    if ((rc = check_fp8_shape(rows, k, "rows", 0, fn)) || (rc = check_fp8_source(out_dtype, fn))) return rc;
+    if (rows == 0) return ok();
+    if (!q || !scales || !out) return fail(SDQ_ERR_INVALID, "%s: q, scales and out must be non-null", fn);
+    if (!aligned(q, 16) || !aligned(out, 16)) return fail(SDQ_ERR_INVALID, "%s: misaligned pointer (q and out need 16 bytes)", fn);
+    if ((rc = check_device())) return rc;
+    cudaError_t e = launch_fp8_dequantize(q, scales, rows, k, weight != 0, out, out_dtype == SDQ_F32,
+                                          static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail("sdq_fp8_dequantize: kernel launch", e);
+    return ok();
+}
+
+int sdq_fp8_matmul(const uint8_t* xq, const uint8_t* x_scales, int64_t m, int64_t k, const uint8_t* wq,
+                   const uint8_t* w_scales, int64_t n, const void* bias, int act, const void* gate,
+                   const void* residual, void* y, sdq_dtype y_dtype, void* stream) {
+    const char* fn = "sdq_fp8_matmul";
+    int rc;
+    if ((rc = check_fp8_shape(m, k, "m (rows of x)", 0, fn)) || (rc = check_fp8_shape(n, k, "n (rows, out features)", 1, fn)))
+        return rc;
+    if (act != SDQ_ACT_NONE && act != SDQ_ACT_GELU_TANH && act != SDQ_ACT_SILU)
+        return fail(SDQ_ERR_INVALID, "%s: act must be SDQ_ACT_NONE, _GELU_TANH or _SILU; got %d", fn, act);
+    if (y_dtype != SDQ_BF16 && y_dtype != SDQ_F32)
+        return fail(SDQ_ERR_UNSUPPORTED, "%s: y must be bf16 or f32 (dtype %d)", fn, (int)y_dtype);
+    if (y_dtype == SDQ_F32 && (act != SDQ_ACT_NONE || gate || residual))
+        return fail(SDQ_ERR_UNSUPPORTED, "%s: an f32 y takes a bias only; act, gate and residual need a bf16 y", fn);
+    if (m == 0) return ok();
+    if (!xq || !x_scales || !wq || !w_scales || !y)
+        return fail(SDQ_ERR_INVALID, "%s: xq, x_scales, wq, w_scales and y must be non-null", fn);
+    const size_t ye = y_dtype == SDQ_F32 ? 4 : 2;
+    if (!aligned(xq, 16) || !aligned(wq, 16) || !aligned(y, ye) || (bias && !aligned(bias, ye)) ||
+        (gate && !aligned(gate, 2)) || (residual && !aligned(residual, 2)))
+        return fail(SDQ_ERR_INVALID, "%s: misaligned pointer (xq and wq need 16 bytes, the others their element's)", fn);
+    if (residual && residual != y) {
+        const uintptr_t r0 = reinterpret_cast<uintptr_t>(residual), y0 = reinterpret_cast<uintptr_t>(y);
+        const uintptr_t bytes = static_cast<uintptr_t>(m) * static_cast<uintptr_t>(n) * 2;
+        if (r0 < y0 + bytes && y0 < r0 + bytes)
+            return fail(SDQ_ERR_INVALID, "%s: residual overlaps y without being y", fn);
+    }
+    if ((rc = check_device())) return rc;
+    EpiArgs epi = bias_only(bias);
+    epi.act = act;
+    epi.gate = static_cast<const uint16_t*>(gate);
+    epi.resid = static_cast<const uint16_t*>(residual);
+    epi.f32 = y_dtype == SDQ_F32;
+    const char* msg = nullptr;
+    cudaError_t e = launch_fp8_mm(xq, x_scales, m, k, wq, w_scales, n, epi, y, static_cast<cudaStream_t>(stream), &msg);
+    if (e != cudaSuccess) {
+        if (msg) return fail(SDQ_ERR_CUDA, "%s: %s", fn, msg);
+        return cuda_fail("sdq_fp8_matmul: kernel launch", e);
+    }
+    return ok();
+}
+
+int sdq_qk_norm_rope(const sdq_heads* q, const sdq_heads* k, const sdq_heads* v, const sdq_heads* q_out,
+                     const sdq_heads* k_out, const sdq_heads* v_out, sdq_dtype dtype, int64_t batch, int64_t tokens,
+                     int head_dim, const void* q_weight, const void* k_weight, float eps, const float* cos,
+                     const float* sin, int64_t table_rows, int rope_dim, int interleaved, const void* positions,
+                     int positions_are_64_bit, int64_t pos_batch_stride, void* stream) {
+    const char* fn = "sdq_qk_norm_rope";
+    if (dtype != SDQ_BF16 && dtype != SDQ_F32)
+        return fail(SDQ_ERR_UNSUPPORTED, "%s: q, k and v must be bf16 or f32 (dtype %d)", fn, (int)dtype);
+    if (head_dim < 8 || head_dim > 256 || head_dim % 8 != 0)
+        return fail(SDQ_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 from 8 to 256; got %d", fn, head_dim);
+    if (rope_dim < 0 || rope_dim > head_dim || rope_dim % 16 != 0)
+        return fail(SDQ_ERR_UNSUPPORTED, "%s: rope_dim must be a multiple of 16 from 0 to head_dim; got %d", fn, rope_dim);
+    if (batch < 0 || tokens < 0 || batch > INT32_MAX || tokens > INT32_MAX || batch * tokens > INT32_MAX)
+        return fail(SDQ_ERR_INVALID, "%s: batch and tokens must be >= 0 and their product < 2^31", fn);
+    if (!(eps >= 0.f)) return fail(SDQ_ERR_INVALID, "%s: eps must be >= 0", fn);
+    if (!q || !k || !q_out || !k_out || (v && !v_out))
+        return fail(SDQ_ERR_INVALID, "%s: q, k and their outputs must be non-null, and v_out where v is", fn);
+    QkArgs a{};
+    const size_t es = dtype == SDQ_F32 ? 4 : 2;
+    const sdq_heads* in[3] = {q, k, v};
+    const sdq_heads* out[3] = {q_out, k_out, v_out};
+    int64_t all = 0;
+    for (int i = 0; i < 3; ++i) {
+        const char* name = i == 0 ? "q" : (i == 1 ? "k" : "v");
+        if (!in[i]) continue;
+        if (in[i]->heads < 0 || in[i]->heads > 65536 || in[i]->heads != out[i]->heads)
+            return fail(SDQ_ERR_INVALID, "%s: %s has %lld heads and its output %lld; they must be equal, 0 to 65536", fn, name,
+                        (long long)in[i]->heads, (long long)out[i]->heads);
+        all += a.heads[i] = (int)in[i]->heads;
+        if (a.heads[i] == 0 || batch == 0 || tokens == 0) continue;
+        for (const sdq_heads* h : {in[i], out[i]}) {
+            if (!h->data) return fail(SDQ_ERR_INVALID, "%s: %s and its output must have data", fn, name);
+            // A stride along an axis of one element is never used.
+            const int64_t used = (batch > 1 ? h->batch_stride : 0) | (tokens > 1 ? h->token_stride : 0) |
+                                 (a.heads[i] > 1 ? h->head_stride : 0);
+            if (!aligned(h->data, 16) || (used * (int64_t)es) % 16 != 0)
+                return fail(SDQ_ERR_INVALID, "%s: %s and its output need 16-byte aligned bases and strides", fn, name);
+        }
+        a.in[i] = {in[i]->data, in[i]->batch_stride, in[i]->token_stride, in[i]->head_stride};
+        a.out[i] = {out[i]->data, out[i]->batch_stride, out[i]->token_stride, out[i]->head_stride};
+    }
+    if ((q_weight && !aligned(q_weight, 16)) || (k_weight && !aligned(k_weight, 16)))
+        return fail(SDQ_ERR_INVALID, "%s: misaligned norm weight (16 bytes)", fn);
+    if (rope_dim > 0) {
+        if (!cos || !sin) return fail(SDQ_ERR_INVALID, "%s: a rotation needs cos and sin", fn);
+        if (!aligned(cos, 16) || !aligned(sin, 16)) return fail(SDQ_ERR_INVALID, "%s: misaligned cos or sin (16 bytes)", fn);
+        if (positions && !aligned(positions, positions_are_64_bit ? 8 : 4))
+            return fail(SDQ_ERR_INVALID, "%s: misaligned positions", fn);
+        if (table_rows < 0 || (!positions && table_rows < tokens))
+            return fail(SDQ_ERR_INVALID, "%s: the tables have %lld rows for %lld tokens", fn, (long long)table_rows,
+                        (long long)tokens);
+    }
+    if (all == 0 || batch == 0 || tokens == 0) return ok();
+    int rc;
+    if ((rc = check_device())) return rc;
+    a.weight[0] = q_weight;
+    a.weight[1] = k_weight;
+    a.cos = cos;
+    a.sin = sin;
+    a.positions = positions;
+    a.pos64 = positions_are_64_bit;
+    a.pos_batch_stride = pos_batch_stride;
+    a.table_rows = table_rows;
+    a.batch = batch;
+    a.tokens = tokens;
+    a.d = head_dim;
+    a.rope = rope_dim;
+    a.eps = eps;
+    a.inv_d = 1.f / (float)head_dim;
+    cudaError_t e = launch_qk_norm_rope(a, dtype == SDQ_BF16, interleaved != 0, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail("sdq_qk_norm_rope: kernel launch", e);
+    return ok();
+}
+
 size_t sdq_gguf_bytes(int ggml_type, int64_t elems) {
     int values = 0, bytes = 0;
     if (!sdq::gguf_block(ggml_type, values, bytes) || elems <= 0 || elems % values != 0) return 0;
@@ -534,6 +706,7 @@ int sdq_debug_wait_hook(uint64_t wait_limit_ns, int withhold_first_copy, void* s
     const int wh = withhold_first_copy != 0;
     cudaError_t e = set_wait_hook_tc(lim, wh, static_cast<cudaStream_t>(stream));
     if (e == cudaSuccess) e = set_wait_hook_qmv(lim, wh, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) e = set_wait_hook_fp8(lim, wh, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail("sdq_debug_wait_hook", e);
     return ok();
 }
@@ -541,18 +714,20 @@ int sdq_debug_wait_hook(uint64_t wait_limit_ns, int withhold_first_copy, void* s
 int sdq_device_status(void* stream) {
     int rc;
     if ((rc = check_device())) return rc;
-    unsigned int st = 0, sv = 0, ss = 0;
+    unsigned int st = 0, sv = 0, ss = 0, sf = 0;
     cudaError_t e = read_and_clear_status(&st, static_cast<cudaStream_t>(stream));
     if (e == cudaSuccess) e = read_and_clear_qmv_status(&sv, static_cast<cudaStream_t>(stream));
     if (e == cudaSuccess) e = read_and_clear_shard_status(&ss, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) e = read_and_clear_fp8_status(&sf, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail("sdq_device_status", e);
-    if (st != 0 || sv != 0 || ss != 0) {
+    if (st != 0 || sv != 0 || ss != 0 || sf != 0) {
         return fail(SDQ_ERR_TIMEOUT,
                     "a device-side wait gave up (tensor-core kernel bits 0x%x: 1 producer, 2 MMA, "
                     "4 dequant, 8 epilogue; small-M kernel bits 0x%x: 1 producer, 2 activations, "
-                    "4 weights; sharded exchange bits 0x%x: 1 a peer's pushes never landed); the "
+                    "4 weights; sharded exchange bits 0x%x: 1 a peer's pushes never landed; fp8 "
+                    "kernel bits 0x%x: 1 producer, 2 MMA, 4 scales, 8 epilogue); the "
                     "kernel returned early and its output is incomplete",
-                    st, sv, ss);
+                    st, sv, ss, sf);
     }
     return ok();
 }

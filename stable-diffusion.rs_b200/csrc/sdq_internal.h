@@ -89,6 +89,39 @@ cudaError_t launch_qmv(const void* x, bool x_f32, int64_t m, int64_t k, const ui
                        const EpiArgs& epi, void* y, bool y_f32, cudaStream_t st, const char** msg,
                        bool* taken);
 
+// Block-scaled e4m3 (sdq_fp8.cuh): activations in row groups of 128 (scales [ceil(k/128), m]),
+// weights in 128 x 128 blocks (scales [ceil(n/128), ceil(k/128)]), and back (sdq_fp8_quant.cu).
+cudaError_t launch_fp8_quantize(const void* x, bool bf16, int64_t m, int64_t k, uint8_t* q, uint8_t* scales,
+                                cudaStream_t st);
+cudaError_t launch_fp8_quantize_weight(const void* w, bool bf16, int64_t n, int64_t k, uint8_t* q,
+                                       uint8_t* scales, cudaStream_t st);
+cudaError_t launch_fp8_dequantize(const uint8_t* q, const uint8_t* scales, int64_t rows, int64_t k, bool weight,
+                                  void* out, bool out_f32, cudaStream_t st);
+// Their product on the tensor cores, every m >= 1 (sdq_fp8_mm.cu).
+cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t k, const uint8_t* wq,
+                          const uint8_t* ws, int64_t n, const EpiArgs& epi, void* y, cudaStream_t st,
+                          const char** msg);
+
+// Queries, keys and values made ready for attention (sdq_qk.cu).  Strides in elements; the last
+// axis is contiguous.  heads[i] == 0 leaves tensor i out; weight == nullptr skips the norm,
+// rope == 0 the rotation.
+struct QkTensor {
+    void* data;
+    int64_t batch_stride, token_stride, head_stride;
+};
+struct QkArgs {
+    QkTensor in[3], out[3];               // queries, keys, values
+    int heads[3];
+    const void* weight[2];                // [d], the tensors' type
+    const float* cos;                     // [table_rows, rope / 2]
+    const float* sin;
+    const void* positions;                // [batch, tokens] int32 or int64, or nullptr: the token's index
+    int64_t pos_batch_stride, table_rows, batch, tokens;
+    int d, rope, pos64;
+    float eps, inv_d;
+};
+cudaError_t launch_qk_norm_rope(const QkArgs& a, bool bf16, bool interleaved, cudaStream_t st);
+
 // GGUF block types (sdq_gguf.cu): values and bytes per block (0 for an unknown type), and
 // the fused dequantise-quantise / the dense dequantise kernels.
 int gguf_block(int type, int& values, int& bytes);
@@ -100,13 +133,15 @@ cudaError_t launch_gguf_dequantize(const void* raw, int type, int64_t count, voi
 // SeededRng::normals (sdq_rng.cu).
 cudaError_t launch_seeded_normals(uint64_t seed, int64_t count, float* out, cudaStream_t st);
 
-// Device status words of the two matmul kernels (see sdq_ptx.cuh): read, then cleared.
+// Device status words of the three matmul kernels (see sdq_ptx.cuh): read, then cleared.
 cudaError_t read_and_clear_status(unsigned int* out, cudaStream_t st);
 cudaError_t read_and_clear_qmv_status(unsigned int* out, cudaStream_t st);
+cudaError_t read_and_clear_fp8_status(unsigned int* out, cudaStream_t st);
 // Status word of the sharded linear's landed-flag wait (sdq_shard.cu): read, then cleared.
 cudaError_t read_and_clear_shard_status(unsigned int* out, cudaStream_t st);
-// Testing hooks of the two matmul files (wait limit, withheld first copy); synchronise `st`.
+// Testing hooks of the three matmul files (wait limit, withheld first copy); synchronise `st`.
 cudaError_t set_wait_hook_tc(unsigned long long limit_ns, int withhold, cudaStream_t st);
 cudaError_t set_wait_hook_qmv(unsigned long long limit_ns, int withhold, cudaStream_t st);
+cudaError_t set_wait_hook_fp8(unsigned long long limit_ns, int withhold, cudaStream_t st);
 
 }  // namespace sdq

@@ -293,6 +293,19 @@ __device__ __forceinline__ void tc_mma_ss_elect(uint32_t d_tmem, uint64_t a_desc
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// Block-scaled form, kind::mxf8f6f4: A and B (8-bit floats, K = 32 per instruction) from shared
+// memory, one e8m0 scale per 32 values of K from tensor memory; one elected lane issues.
+__device__ __forceinline__ void tc_mma_mx_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+        : "memory");
+}
 __device__ __forceinline__ void tc_commit_elect(uint64_t* bar) {
     asm volatile(
         "{\n\t.reg .pred e;\n\t"
@@ -389,6 +402,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// ... four columns.
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c),
+                 "r"(d)
+                 : "memory");
+}
 // Warp-collective: lane i reads 16 consecutive 32-bit columns of TMEM lane (taddr.lane + i).
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -443,6 +462,14 @@ __host__ __device__ constexpr uint32_t idesc_bf16_f32(int M, int N) {
            | (1u << 10)                               // B format BF16
            | (static_cast<uint32_t>(N >> 3) << 17)    // N / 8
            | (static_cast<uint32_t>(M >> 4) << 24);   // M / 16
+}
+
+// Instruction descriptor for kind::mxf8f6f4 with e8m0 scales: e4m3 A and B (format 0), both
+// K-major, scale byte 0 of each 32-bit cell for both, shape M (128 or 256) x N.
+__host__ __device__ constexpr uint32_t idesc_mx_e4m3(int M, int N) {
+    return (static_cast<uint32_t>(N >> 3) << 17)      // N / 8
+           | (1u << 23)                               // scale type e8m0
+           | (static_cast<uint32_t>(M >> 7) << 27);   // M / 128
 }
 
 }  // namespace sdq

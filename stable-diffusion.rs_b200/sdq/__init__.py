@@ -23,7 +23,8 @@ __all__ = [
     "gguf_quantize", "gguf_dequantize", "seeded_normals", "resident_bytes", "ACT_NONE", "ACT_GELU_TANH", "ACT_SILU",
     "device_status", "Comm", "quantized_matmul_sharded", "shard_rows", "unshard", "GROUP_SIZE", "MODE",
     "SDQ_OK", "SDQ_ERR_INVALID", "SDQ_ERR_UNSUPPORTED", "SDQ_ERR_CUDA", "SDQ_ERR_TIMEOUT",
-    "SDQ_ERR_NCCL",
+    "SDQ_ERR_NCCL", "Fp8Array", "fp8_quantize", "fp8_quantize_weight", "fp8_dequantize", "fp8_matmul",
+    "qk_norm_rope",
 ]
 
 #: MLX's default group size (crates/sd-models/src/mlx/quantized.rs:45-46).
@@ -388,3 +389,7 @@ def quantized_matmul_sharded(x, wq, scales, biases, comm: Comm, group_size: int 
         _ptr(bias), _ptr(y_shards), _ptr(out) if permute else None, SDQ_BF16, comm.handle,
         _stream(stream)))
     return (out if permute else None), y_shards
+
+
+from .fp8 import Fp8Array, fp8_dequantize, fp8_matmul, fp8_quantize, fp8_quantize_weight  # noqa: E402
+from .heads import qk_norm_rope  # noqa: E402

@@ -24,6 +24,13 @@ SDQ_F32 = 0
 SDQ_BF16 = 1
 SDQ_F16 = 2
 
+
+class SdqHeads(ctypes.Structure):
+    """``sdq_heads``: head vectors [batch, tokens, heads, head_dim], strides in elements."""
+    _fields_ = [("data", ctypes.c_void_p), ("heads", ctypes.c_int64), ("batch_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
 #: Every symbol include/sdq.h declares, with (restype, argtypes).
 _p, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
 SIGNATURES = {
@@ -37,6 +44,12 @@ SIGNATURES = {
                                          _i32, _p, _p, _i64, _p]),
     "sdq_quantized_matmul_epilogue": (_i32, [_p, _i32, _i64, _i64, _p, _p, _p, _i32, _i64, _i32, _i32,
                                              _p, _i32, _p, _p, _p, _i32, _p]),
+    "sdq_fp8_quantize": (_i32, [_p, _i32, _i64, _i64, _p, _p, _p]),
+    "sdq_fp8_quantize_weight": (_i32, [_p, _i32, _i64, _i64, _p, _p, _p]),
+    "sdq_fp8_dequantize": (_i32, [_p, _p, _i64, _i64, _i32, _p, _i32, _p]),
+    "sdq_fp8_matmul": (_i32, [_p, _p, _i64, _i64, _p, _p, _i64, _p, _i32, _p, _p, _p, _i32, _p]),
+    "sdq_qk_norm_rope": (_i32, [_p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i32, _p, _p, ctypes.c_float, _p, _p,
+                                _i64, _i32, _i32, _p, _i32, _i64, _p]),
     "sdq_resident_bytes": (_sz, [_i64, _i64, _i32, _i32, _i32]),
     "sdq_gguf_bytes": (_sz, [_i32, _i64]),
     "sdq_seeded_normals": (_i32, [ctypes.c_uint64, _i64, _p, _p]),

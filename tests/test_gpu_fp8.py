@@ -1,0 +1,327 @@
+"""GPU: block-scaled e4m3 against the oracle and 64-bit sums.
+
+Codes and scales are compared for equality: dividing by a power of two is exact, so each value has
+one right code.  A product's tolerance counts its roundings.  Products of two 4-bit significands and
+of two powers of two are exact in f32; the sum of K of them is taken 32 at a time and each addition
+into the f32 accumulator, rounded or truncated, is off by at most 2^-23 of the partial sum, the sum
+inside one step by at most as much for each of its 32 terms' alignment.  With S = sum |x w| bounding
+every partial sum:  |error| <= (K/32 + 32) 2^-23 S, and 2^-8 of the value for the bf16 rounding.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import oracle as O
+import sdq
+from conftest import gpu_available
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs an sm_100 device")]
+
+DT = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def u8(t):
+    return t.view(torch.uint8).cpu().numpy()
+
+
+def normals(seed, *shape):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return torch.randn(*shape, device="cuda", generator=g)
+
+
+def spread(seed, m, k):
+    """Normals whose rows and columns differ by powers of two over a wide range."""
+    g = torch.Generator("cuda").manual_seed(seed + 1000)
+    x = normals(seed, m, k)
+    x *= torch.exp2(torch.randint(-20, 20, (m, 1), device="cuda", generator=g).float())
+    return x * torch.exp2(torch.randint(-3, 3, (1, k), device="cuda", generator=g).float())
+
+
+SHAPES = [(1, 16), (1, 128), (3, 144), (4, 256), (5, 112), (33, 272), (129, 128), (130, 400), (257, 2576)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_quantize_matches_the_oracle(m, k, dtype):
+    x = spread(m + k, m, k).to(DT[dtype])
+    q, s = sdq.fp8_quantize(x)
+    assert q.shape == (m, k) and s.shape == (-(-k // 128), m)
+    wq, ws = O.fp8_quantize(x.double().cpu().numpy())
+    assert np.array_equal(u8(s), ws)
+    assert np.array_equal(u8(q), wq)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,k", SHAPES)
+def test_quantize_weight_matches_the_oracle(n, k, dtype):
+    w = spread(n + k, n, k).to(DT[dtype])
+    q, s = sdq.fp8_quantize_weight(w)
+    wq, ws = O.fp8_quantize_weight(w.double().cpu().numpy())
+    assert np.array_equal(u8(s), ws)
+    assert np.array_equal(u8(q), wq)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantize_edges(dtype):
+    """Groups of zeros, of the smallest and the largest numbers, at the border of two scales, with
+    exact ties, and with an infinity or a NaN (which make their own group NaN and no other)."""
+    fi = torch.finfo(DT[dtype])
+    x = torch.zeros(12, 256)
+    x[1] = fi.smallest_normal
+    x[2, 5] = fi.max
+    x[3, :8] = torch.tensor([448.0, 432.0, 17.0, 19.0, -21.0, 2.0 ** -10, 3 * 2.0 ** -10, -(2.0 ** -10)])
+    x[4, 0], x[4, 1] = 450.0, 1.0
+    x[5, 128] = float("inf")
+    x[6, 3] = float("nan")
+    x[7, :] = -float("inf")
+    x[8, 0], x[8, 200] = -0.0, 2.0 ** -130
+    x[9] = torch.linspace(-448, 448, 256)
+    x[10] = fi.tiny * 0.5 if dtype == "f32" else 2.0 ** -133
+    x = x.to(DT[dtype]).cuda()
+    q, s = sdq.fp8_quantize(x)
+    wq, ws = O.fp8_quantize(x.double().cpu().numpy())
+    assert np.array_equal(u8(s), ws) and np.array_equal(u8(q) & 0x7F, wq & 0x7F)
+    live = wq != 0x7F
+    assert np.array_equal(u8(q)[live], wq[live])
+    q, s = sdq.fp8_quantize_weight(x)
+    wq, ws = O.fp8_quantize_weight(x.double().cpu().numpy())
+    assert np.array_equal(u8(s), ws) and (u8(q) & 0x7F == wq & 0x7F).all()
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("weight", [False, True])
+def test_dequantize_matches_the_oracle(weight, out):
+    m, k = 131, 272
+    q = torch.randint(0, 256, (m, k), device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)
+    kb, nb = 3, 2
+    # every byte of e8m0 that keeps the value in range, 0 (2^-127), and 255 (NaN)
+    s = torch.randint(0, 240, (nb, kb) if weight else (kb, m), device="cuda", dtype=torch.uint8)
+    s.view(-1)[:3] = torch.tensor([0, 255, 1], dtype=torch.uint8)
+    got = sdq.fp8_dequantize(q, s.view(torch.float8_e8m0fnu), weight, out)
+    want = torch.from_numpy(O.fp8_dequantize(u8(q), u8(s), weight)).to(out)
+    assert torch.equal(got.cpu().nan_to_num(nan=12345.0), want.nan_to_num(nan=12345.0))
+
+
+def product(xq, xs, wq, ws):
+    """(sum of x w, sum of |x w|) in f64 on the device."""
+    x = xq.double() * xs.double().t().repeat_interleave(128, 1)[:, : xq.shape[1]]
+    w = wq.double() * ws.double().repeat_interleave(128, 0).repeat_interleave(128, 1)[: wq.shape[0], : wq.shape[1]]
+    return x @ w.t(), x.abs() @ w.abs().t()
+
+
+def operands(seed, m, k, n):
+    return (*sdq.fp8_quantize(spread(seed, m, k)), *sdq.fp8_quantize_weight(spread(seed + 7, n, k)))
+
+
+def sums_tol(s, k):
+    return (k / 32 + 32) * 2.0 ** -23 * s
+
+
+def check(got, want, tol):
+    bad = (got.double() - want).abs() > tol
+    assert not bad.any(), (int(bad.sum()), got[bad][:4], want[bad][:4], tol[bad][:4])
+
+
+# m: one row, the small-M kernel's edges, the token tiles' edges; n and k ragged and whole.
+MM = [(1, 16, 1), (1, 128, 128), (2, 256, 130), (3, 144, 8), (5, 2576, 333), (8, 512, 640), (9, 400, 257), (16, 1024, 256),
+      (17, 128, 100), (33, 272, 515), (64, 640, 128), (65, 1040, 384), (128, 512, 129), (129, 4096, 256), (224, 256, 512),
+      (225, 768, 1000), (333, 2576, 499), (512, 1024, 2048), (1000, 208, 3001)]
+
+
+@pytest.mark.parametrize("m,k,n", MM)
+def test_matmul_matches_64_bits(m, k, n):
+    ops = operands(m + k + n, m, k, n)
+    want, s = product(*ops)
+    y = sdq.fp8_matmul(*ops)
+    sdq.device_status()
+    check(y, want, want.abs() * 2.0 ** -8 + sums_tol(s, k))
+    y = sdq.fp8_matmul(*ops, out_dtype=torch.float32)
+    sdq.device_status()
+    check(y, want, want.abs() * 2.0 ** -24 + sums_tol(s, k))
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 512, 256), (7, 400, 130), (40, 272, 300), (300, 640, 1024), (226, 144, 77)])
+@pytest.mark.parametrize("act", [None, "silu", "gelu_approx"])
+def test_output_stage(m, k, n, act):
+    """bias, activation, gate and residual, all of them and in place, against the chain in f64.  The
+    activations' slopes are at most 1.13, their own error at most 2^-10 (1 + |v|) (hardware tanh 2^-11
+    relative, __expf and the fast division 2^-20), times the gate."""
+    ops = operands(m * n + k, m, k, n)
+    want, s = product(*ops)
+    scale = want.abs().mean()
+    ops = (ops[0], ops[1], ops[2], ops[3])
+    bias = (normals(1, n) * scale).to(torch.bfloat16)
+    gate, res = (normals(2, n) / scale).to(torch.bfloat16), normals(3, m, n).to(torch.bfloat16)
+    v = want + bias.double()
+    tol_v = sums_tol(s, k) + v.abs() * 2.0 ** -23
+    if act == "silu":
+        a = v * torch.sigmoid(v)
+    elif act:
+        a = v * torch.sigmoid(2 * (2 / np.pi) ** 0.5 * (v + 0.044715 * v ** 3))
+    else:
+        a = v
+    tol_a = 1.13 * tol_v + (2.0 ** -10 * (1 + v.abs()) if act else 0)
+    y = sdq.fp8_matmul(*ops, bias=bias, act=act)
+    check(y, a, tol_a + a.abs() * 2.0 ** -8)
+    z = res.double() + gate.double() * a
+    tol = tol_a * gate.double().abs() + (z.abs() + (gate.double() * a).abs() * 2.0 ** -14) * 2.0 ** -8
+    check(sdq.fp8_matmul(*ops, bias=bias, act=act, gate=gate, residual=res), z, tol)
+    r = res.clone()
+    assert sdq.fp8_matmul(*ops, bias=bias, act=act, gate=gate, residual=r, out=r) is r
+    check(r, z, tol)
+    sdq.device_status()
+
+
+@pytest.mark.parametrize("m", [1, 6, 40, 300])
+def test_f32_result_with_an_f32_bias(m):
+    k, n = 272, 130
+    ops = operands(m, m, k, n)
+    bias = normals(4, n)
+    want, s = product(*ops)
+    y = sdq.fp8_matmul(*ops, bias=bias, out_dtype=torch.float32)
+    check(y, want + bias.double(), sums_tol(s, k) + (want + bias.double()).abs() * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("m", [2, 20, 300])
+def test_nan_stays_in_its_row_and_its_features(m):
+    """A NaN group of an activation makes that token's row NaN and nothing else; a NaN block of a
+    weight its 128 features."""
+    k, n = 512, 300
+    x, w = normals(5, m, k), normals(6, n, k)
+    x[1, 130] = float("inf")
+    xq, xs = sdq.fp8_quantize(x)
+    wq, ws = sdq.fp8_quantize_weight(w)
+    y = sdq.fp8_matmul(xq, xs, wq, ws)
+    nan = torch.isnan(y)
+    assert nan[1].all() and nan.sum() == n
+    w[140, 3] = float("nan")
+    x[1, 130] = 0
+    y = sdq.fp8_matmul(*sdq.fp8_quantize(x), *sdq.fp8_quantize_weight(w))
+    nan = torch.isnan(y)
+    assert nan[:, 128:256].all() and nan.sum() == m * 128
+
+
+@pytest.mark.parametrize("m", [1, 5, 20, 300])
+def test_nothing_beside_the_result_is_written(m):
+    """Sentinels around y, odd n (an unaligned pitch) and a y that starts off 16 bytes."""
+    k, n = 144, 131
+    ops = operands(m, m, k, n)
+    room = torch.full((m * n + 64,), -7.0, device="cuda", dtype=torch.bfloat16)
+    y = room[33: 33 + m * n].view(m, n)
+    sdq.fp8_matmul(*ops, out=y)
+    torch.cuda.synchronize()
+    assert (room[:33] == -7).all() and (room[33 + m * n:] == -7).all()
+    want, s = product(*ops)
+    check(y, want, want.abs() * 2.0 ** -8 + sums_tol(s, k))
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_same_call_same_bits(m):
+    ops = operands(9, m, 1040, 700)
+    a = sdq.fp8_matmul(*ops)
+    for _ in range(5):
+        assert torch.equal(sdq.fp8_matmul(*ops), a)
+
+
+def test_empty_batch():
+    wq, ws = sdq.fp8_quantize_weight(normals(1, 64, 128))
+    x = torch.empty(0, 128, device="cuda", dtype=torch.bfloat16)
+    xq, xs = sdq.fp8_quantize(x)
+    assert xq.shape == (0, 128) and xs.shape == (1, 0)
+    assert sdq.fp8_matmul(xq, xs, wq, ws).shape == (0, 64)
+    assert sdq.fp8_dequantize(xq, xs, False).shape == (0, 128)
+
+
+def test_leading_axes_and_the_array_class():
+    x = normals(2, 2, 7, 256).to(torch.bfloat16)
+    w = normals(3, 300, 256) / 16
+    a = sdq.Fp8Array.quantize(w)
+    assert a.shape == (300, 256) and a.resident_bytes() == 300 * 256 + 3 * 2
+    y = a.matmul(x)
+    assert y.shape == (2, 7, 300) and y.dtype is torch.bfloat16
+    xq, xs = sdq.fp8_quantize(x)
+    want, s = product(xq.view(14, 256), xs, a.weight, a.scales)
+    check(y.view(14, 300), want, want.abs() * 2.0 ** -8 + sums_tol(s, 256))
+    f = a.matmul(x.float())
+    assert f.dtype is torch.float32
+    check(f.view(14, 300), want, want.abs() * 2.0 ** -24 + sums_tol(s, 256))
+    # each value is within half an e4m3 step (2^-4 of it; 2^-10 of the scale below the normals)
+    d = a.dequantize(torch.float32).double()
+    step = w.double().abs() * 2.0 ** -4 + 2.0 ** -10 * a.scales.double().repeat_interleave(128, 0).repeat_interleave(128, 1)[:300]
+    assert ((d - w.double()).abs() <= step).all()
+
+
+def test_another_stream_and_a_captured_graph():
+    ops = operands(11, 50, 512, 384)
+    want = sdq.fp8_matmul(*ops)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    y = sdq.fp8_matmul(*ops, stream=s)
+    s.synchronize()
+    assert torch.equal(y, want)
+    x, w = normals(12, 50, 512), normals(13, 384, 512)
+    a = sdq.Fp8Array.quantize(w)
+    out = torch.empty(50, 384, device="cuda")
+    a.matmul(x, out=out)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):                       # two graphs of the same call, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            a.matmul(x, out=out)
+        graphs.append(g)
+    for i in range(4):
+        x.copy_(normals(20 + i, 50, 512))
+        want = a.matmul(x)
+        graphs[i % 2].replay()
+        assert torch.equal(out, want)
+    sdq.device_status()
+
+
+def test_refusals_of_the_package():
+    xq, xs, wq, ws = operands(3, 4, 256, 130)
+    bad = [
+        (lambda: sdq.fp8_matmul(xq, xs.t().contiguous(), wq, ws), "xs must have shape"),
+        (lambda: sdq.fp8_matmul(xq, xs, wq[:, :128].contiguous(), ws), "wq must have shape"),
+        (lambda: sdq.fp8_matmul(xq, xs, wq, ws[:1].contiguous()), "ws must have shape"),
+        (lambda: sdq.fp8_matmul(xq.view(torch.uint8), xs, wq, ws), "xq must be"),
+        (lambda: sdq.fp8_matmul(xq, xs.view(torch.uint8), wq, ws), "xs must be"),
+        (lambda: sdq.fp8_matmul(xq, xs, wq, ws, bias=torch.zeros(129, device="cuda", dtype=torch.bfloat16)), "bias must hold 130"),
+        (lambda: sdq.fp8_matmul(xq, xs, wq, ws, bias=torch.zeros(130, device="cuda")), "bias must hold 130"),
+        (lambda: sdq.fp8_matmul(xq, xs, wq, ws, bias=torch.zeros(130)), "bias is on cpu"),
+        (lambda: sdq.fp8_matmul(xq, xs, wq, ws, act="relu"), "unknown activation"),
+        (lambda: sdq.fp8_matmul(xq, xs, wq, ws, out=torch.empty(4, 131, device="cuda")), "out must have shape"),
+        (lambda: sdq.fp8_matmul(xq, xs, wq, ws, out=torch.empty(4, 130, device="cuda", dtype=torch.float16)), "out must be bf16 or f32"),
+        (lambda: sdq.fp8_matmul(xq, xs, wq, ws, act="silu", out_dtype=torch.float32), "bias only"),
+        (lambda: sdq.fp8_matmul(xq[:, ::2], xs, wq, ws), "contiguous"),
+        (lambda: sdq.fp8_quantize(torch.zeros(4, 120, device="cuda")), "multiple of 16"),
+        (lambda: sdq.fp8_quantize(torch.zeros(4, 128, device="cuda", dtype=torch.float16)), "bf16 or f32"),
+        (lambda: sdq.fp8_quantize(torch.zeros(4, 129, device="cuda")[:, :128]), "contiguous"),
+        (lambda: sdq.fp8_quantize(torch.zeros(4 * 128 + 1, device="cuda")[1:].view(4, 128)), "misaligned"),
+        (lambda: sdq.fp8_quantize_weight(torch.zeros(2, 4, 128, device="cuda")), "2-D"),
+        (lambda: sdq.fp8_dequantize(xq, xs, True), "scales must have shape"),
+        (lambda: sdq.fp8_dequantize(xq, xs, False, torch.float16), "bf16 or f32"),
+    ]
+    for call, needle in bad:
+        with pytest.raises(sdq.SdqError, match=needle):
+            call()
+
+
+@pytest.mark.parametrize("m", [20, 300])
+def test_withheld_copy_times_out_then_the_next_call_is_correct(m):
+    """The bounded waits (see test_gpu_abort.py) of the fp8 kernel."""
+    ops = operands(5, m, 1024, 512)
+    want = sdq.fp8_matmul(*ops)
+    sdq.device_status()
+    sdq.debug_wait_hook(20_000_000, True)
+    try:
+        sdq.fp8_matmul(*ops)
+        torch.cuda.synchronize()
+        with pytest.raises(sdq.SdqError, match="gave up"):
+            sdq.device_status()
+    finally:
+        sdq.debug_wait_hook(0, False)
+    sdq.device_status()
+    assert torch.equal(sdq.fp8_matmul(*ops), want)
