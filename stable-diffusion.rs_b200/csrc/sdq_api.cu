@@ -99,8 +99,8 @@ int check_nk(int64_t n, int64_t k, const char* fn) {
 
 // Shapes of block-scaled e4m3 operands: rows >= least, k >= 1 and a multiple of 16.
 int check_fp8_shape(int64_t rows, int64_t k, const char* what, int64_t least, const char* fn) {
-    if (rows < least || rows > INT32_MAX)
-        return fail(SDQ_ERR_INVALID, "%s: %s must be >= %lld and < 2^31; got %lld", fn, what, (long long)least,
+    if (rows < least || rows > (1ll << 30))
+        return fail(SDQ_ERR_INVALID, "%s: %s must be >= %lld and <= 2^30; got %lld", fn, what, (long long)least,
                     (long long)rows);
     if (k <= 0 || k > INT32_MAX) return fail(SDQ_ERR_INVALID, "%s: k must be >= 1 and < 2^31; got %lld", fn, (long long)k);
     if (k % 16 != 0)

@@ -2,21 +2,25 @@
 //
 //   y[t, f] = resid + gate[f] * act( sum_kb xs[kb, t] ws[f/128, kb] sum_{k in kb} xq[t,k] wq[f,k] + bias[f] )
 //
-// The tile is D[f, t] = W[f, :] . X[t, :]^T: 128 features (MMA M) by BT tokens (MMA N), f32 in
-// tensor memory.  One step is one scale block of K (128 values, 128 bytes): W's 128 rows and X's
-// BT rows arrive by TMA with the 128-byte swizzle, four block-scaled MMAs (K = 32 each) consume
-// them, and the scales are multiplied in by the tensor core, from tensor memory, where a warpgroup
-// has laid them: row r of A has its byte in lane r % 32 of column r / 32 (and so for B), repeated
-// in each of the four 32-lane quarters.  All four MMAs of a step use the same byte.
+// A tile is 128 tokens (MMA M; 256 for a CTA pair, 128 in each) by `bn` features (MMA N, 16 .. 224),
+// f32 in tensor memory, double-buffered.  One step is one scale block of K: 128 values, 128 bytes.
+// X's rows and W's rows (a pair's CTAs load half of W's each) arrive by TMA with the 128-byte
+// swizzle; four block-scaled MMAs (K = 32) consume them.  The tensor core multiplies the scales in
+// from tensor memory: row r of an operand has its scale in lane r % 32 of column r / 32, the same
+// in each of the four 32-lane quarters; the four bytes of a 32-bit cell are the scales of four
+// consecutive steps, chosen by the instruction, so they are laid once for 512 values of K.
 //
-// Warp roles (384 threads, one CTA per SM, persistent over tiles):
-//   warp 0       TMA producer of the operand ring
-//   warp 1       tensor memory allocator and MMA issuer
-//   warps 4-7    scale bytes: global -> registers (four steps ahead) -> tensor memory ring
-//   warps 8-11   output stage: accumulator -> registers -> y, while the next tile accumulates in
-//                the other buffer (BT <= 224)
-// Every mbarrier wait is bounded; on expiry the kernel records a status bit, drains its own copies
-// and MMAs, frees its tensor memory and returns.
+// Tokens lie on the lanes, so that a thread of the output stage holds consecutive features of one
+// token and stores whole 32-byte sectors.  (The other way round each thread held one feature and
+// stored 2 bytes a time, which cost more than the product at K = 4096.)
+//
+// Warp roles (512 threads, one CTA per SM, persistent over tiles):
+//   warp 0       TMA producer of the operand ring (one thread)
+//   warp 1       tensor memory allocator and MMA issuer (one thread; in a pair, rank 0's)
+//   warps 4-7    scale bytes: global -> registers, four groups ahead -> shared memory
+//   warps 8-15   output stage, two groups of four warps taking 16 features in turn
+// Every mbarrier wait is bounded; on expiry the kernel records a status bit, waits for its own
+// copies and MMAs, frees its tensor memory and returns.
 #include <cstdint>
 #include <cstring>
 #include <cuda.h>
@@ -34,51 +38,63 @@ __device__ unsigned int g_fp8_status = 0;
 
 namespace {
 
-constexpr int kMmThreads = 384;
+constexpr int kMmThreads = 512;
+constexpr int kTokens = 128;                       // per CTA
+constexpr int kMaxBn = 224;                        // two accumulators and the scales fill 512 columns
+constexpr int kXStage = kTokens * kFp8Block;       // bytes
+constexpr int kMaxStages = 12;
+constexpr int kSlots = 4;                          // scale groups in tensor memory, one for each scale warp
+constexpr int kCells = 3 * 512;                    // bytes of a group's scales in shared memory
+static_assert(2 * kMaxBn + kSlots * 12 <= 512, "tensor memory");
+constexpr int kPitch = 17;                         // words per token of a warp's transposing buffer
+constexpr int kFixedSmem = 1024 /* alignment */ + 512 /* barriers */ + 2 * 256 * 4 /* bias, gate */ +
+                           kSlots * kCells;
+constexpr int kTransposeSmem = 8 * 32 * kPitch * 4;
 
-template <int BT>
-struct MmCfg {
-    static constexpr int BF = 128;                                 // features per tile
-    static constexpr int W_STAGE = BF * kFp8Block;                 // bytes
-    static constexpr int X_STAGE = BT * kFp8Block;
-    static constexpr int STAGE = W_STAGE + X_STAGE;
-    static constexpr int STAGES = (kQmvMaxSmem - 2048) / STAGE < 8 ? (kQmvMaxSmem - 2048) / STAGE : 8;
-    static constexpr int D_BUFS = BT <= 224 ? 2 : 1;
-    static constexpr int D_COLS = (BT + 31) / 32 * 32;             // columns of one accumulator
-    static constexpr int SB_COLS = (BT + 127) / 128 * 4;           // columns of X's scales (a multiple of 4)
-    static constexpr int SLOT = 4 + SB_COLS;                       // W's four, then X's
-    static constexpr int SF_COL = D_BUFS * D_COLS;
-    static constexpr int SLOTS = (512 - SF_COL) / SLOT < STAGES ? (512 - SF_COL) / SLOT : STAGES;
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 1024;
-    static_assert(BT % 16 == 0 && BT >= 16 && BT <= 256, "MMA N");
-    static_assert(SLOTS >= 3 && STAGES >= 3, "rings too short");
+// What the host has settled for a launch.
+struct MmPlan {
+    int m, n, k;
+    int bn;                // features per tile
+    int stages;            // ring depth
+    int group;             // token tiles that are walked together (see place)
+    int x_rows;            // rows of X a CTA loads (128, or M rounded up to 8)
+    int aligned;           // rows of y (and resid) start on 32 bytes and hold whole 16-feature pieces
 };
 
-template <int BT, bool FUSED, bool YF32>
+template <bool PAIR, bool FUSED, bool YF32>
 __global__ void __launch_bounds__(kMmThreads, 1)
     fp8_mm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
-                  const uint8_t* __restrict__ xs, const uint8_t* __restrict__ ws, const EpiArgs epi, void* y, int M,
-                  int N, int K, int group) {
-    using C = MmCfg<BT>;
+                  const uint8_t* __restrict__ xs, const uint8_t* __restrict__ ws, const EpiArgs epi, void* y,
+                  const __grid_constant__ MmPlan p) {
+    constexpr int CG = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE);
-    // Step s uses stage s % STAGES and scale slot s % SLOTS.
-    uint64_t* full = bars;                       // operands landed            count 1 + tx
-    uint64_t* done = full + C::STAGES;           // the step's MMAs finished   count 1 (commit); frees stage and slot
-    uint64_t* sfull = done + C::STAGES;          // scale slot written         count 128
-    uint64_t* dfull = sfull + C::SLOTS;          // accumulator complete       count 1 (commit)
-    uint64_t* dempty = dfull + 2;                // accumulator drained        count 128
+    const int w_rows = p.bn / CG;                               // rows of W this CTA loads
+    const int stage_bytes = kXStage + w_rows * kFp8Block;       // both parts multiples of 1024
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
+    // Step s uses stage s % stages; a group of up to four steps of a tile uses one scale slot.
+    uint64_t* full = bars;                       // operands of the pair landed   count 1 + tx
+    uint64_t* done = full + kMaxStages;          // the step's MMAs finished      count 1 (commit); frees the stage
+    uint64_t* sfull = done + kMaxStages;         // a group's scales in smem      count CG
+    uint64_t* sempty = sfull + kSlots;        // the group's MMAs finished     count 1 (commit); frees the slot
+    uint64_t* dfull = sempty + kSlots;        // accumulator complete          count 1 (commit)
+    uint64_t* dempty = dfull + 2;                // accumulator drained           count 8 (a warp each) x CG
     uint64_t* drain = dempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* sbias = reinterpret_cast<float*>(bars + 64);         // [256]
+    float* sgate = sbias + 256;                                 // [256]
+    // [slots][3 column quads][32 lanes][4 columns][4 steps], X's quad first
+    uint8_t* sscale = reinterpret_cast<uint8_t*>(sgate + 256);
+    float* stage32 = reinterpret_cast<float*>(sscale + kSlots * kCells);    // the transposing buffers, if any
     unsigned int* status = &g_fp8_status;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(done + i, 1); }
-        for (int i = 0; i < C::SLOTS; ++i) mbar_init(sfull + i, 128);
-        for (int i = 0; i < 2; ++i) { mbar_init(dfull + i, 1); mbar_init(dempty + i, 128); }
+        for (int i = 0; i < p.stages; ++i) { mbar_init(full + i, 1); mbar_init(done + i, 1); }
+        for (int i = 0; i < kSlots; ++i) { mbar_init(sfull + i, CG); mbar_init(sempty + i, 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(dfull + i, 1); mbar_init(dempty + i, 8 * CG); }
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
@@ -86,192 +102,306 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         tma_prefetch_desc(&tmW);
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, 512);
-        tmem_relinquish();
+        if (PAIR) {
+            tmem_alloc_pair(tmem_slot, 512);
+        } else {
+            tmem_alloc(tmem_slot, 512);
+            tmem_relinquish();
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();                    // the peer's barriers are initialised too
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    const int KT = (K + kFp8Block - 1) / kFp8Block;
-    const int nft = (N + C::BF - 1) / C::BF, ntt = (M + BT - 1) / BT, ntiles = nft * ntt;
-    // Tiles go in groups of `group` token tiles: within a group, the tokens of one feature tile
-    // first, so that the CTAs at work share W's tiles and the group's X stays in L2 while W
-    // streams past it once per group.
+    const int KT = (p.k + kFp8Block - 1) / kFp8Block;
+    const int d_cols = (p.bn + 31) / 32 * 32, sf_col = 2 * d_cols;
+    const int sb_cols = (p.bn + 127) / 128 * 4, slot_cols = 4 + sb_cols;   // X's four columns, then W's
+    const int nft = (p.n + p.bn - 1) / p.bn, ntt = (p.m + CG * kTokens - 1) / (CG * kTokens), ntiles = nft * ntt;
+    const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+    // Tiles go in groups of `group` token tiles; within a group, the tokens of one feature tile
+    // first.  So the CTAs at work share W's rows, and the group's X stays in L2 while W streams
+    // past it once per group.
     auto place = [&](int tile, int& ft, int& tt) {
-        const int per = group * nft, g = tile / per, r = tile - g * per;
-        const int h = ntt - g * group < group ? ntt - g * group : group;
+        const int per = p.group * nft, g = tile / per, r = tile - g * per;
+        const int h = ntt - g * p.group < p.group ? ntt - g * p.group : p.group;
         ft = r / h;
-        tt = g * group + (r - ft * h);
+        tt = g * p.group + (r - ft * h);
     };
 
     if (warp == 0) {
         // ------------------------------------------------------------ operand producer
-        if (lane == 0) {
-            int it = 0;
+        if (elect_one()) {
+            const uint32_t my_bytes = (uint32_t)((p.x_rows + w_rows) * kFp8Block);
+            const uint32_t full0 = PAIR ? cluster_addr(full, 0) : 0;
+            int it = 0, s = 0;
+            uint32_t phase = 1;
             bool ok = true;
             const bool withhold = g_withhold_first_copy != 0;      // testing hook, normally false
-            for (int tile = blockIdx.x; ok && tile < ntiles; tile += gridDim.x) {
+            for (int tile = first; ok && tile < ntiles; tile += stride) {
                 int ft, tt;
                 place(tile, ft, tt);
+                const int xr = (tt * CG + (int)rank) * kTokens, wr = ft * p.bn + (int)rank * w_rows;
                 for (int kt = 0; kt < KT; ++kt, ++it) {
-                    const int s = it % C::STAGES;
-                    if (!mbar_wait_sleep(done + s, ((it / C::STAGES) & 1) ^ 1, abort_flag, status, 1u, 20)) { ok = false; break; }
-                    if (withhold && it == 0) continue;
-                    mbar_arrive_expect_tx(full + s, C::STAGE);
-                    tma_load_2d(smem + s * C::STAGE, &tmW, full + s, kt * kFp8Block, ft * C::BF);
-                    tma_load_2d(smem + s * C::STAGE + C::W_STAGE, &tmX, full + s, kt * kFp8Block, tt * BT);
+                    if (!mbar_wait(done + s, phase, abort_flag, status, 1u)) { ok = false; break; }
+                    uint8_t* at = smem + s * stage_bytes;
+                    if (!(withhold && it == 0)) {
+                        if (PAIR) {
+                            if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * my_bytes);
+                            tma_load_2d_pair(at, &tmX, full0 + 8 * s, kt * kFp8Block, xr);
+                            tma_load_2d_pair(at + kXStage, &tmW, full0 + 8 * s, kt * kFp8Block, wr);
+                        } else {
+                            mbar_arrive_expect_tx(full + s, my_bytes);
+                            tma_load_2d(at, &tmX, full + s, kt * kFp8Block, xr);
+                            tma_load_2d(at + kXStage, &tmW, full + s, kt * kFp8Block, wr);
+                        }
+                    }
+                    if (++s == p.stages) { s = 0; phase ^= 1; }
                 }
             }
-            // Whatever stopped the loop, no copy may outlive the CTA's shared memory: the last
-            // STAGES steps that were started are waited for.
-            if (!ok)
-                for (int j = it - 1; j >= 0 && j >= it - C::STAGES; --j)
-                    if (!(withhold && j == 0)) mbar_wait_drain(full + j % C::STAGES, (uint32_t)((j / C::STAGES) & 1));
+            // After an abort no copy may outlive shared memory: the last steps started are waited
+            // for, by rank 0 for both CTAs of a pair (its peer waits at the end of the kernel), and
+            // so is the one that the peer alone may have started.
+            if (!ok && rank == 0) {
+                bool landed = true;
+                for (int j = it < p.stages ? 0 : it - p.stages; j < it; ++j)
+                    landed = !(withhold && j == 0) && mbar_wait_drain(full + j % p.stages, (uint32_t)((j / p.stages) & 1)) && landed;
+                if (PAIR && landed) {
+                    mbar_arrive_expect_tx(full + s, my_bytes);
+                    mbar_wait_drain(full + s, (uint32_t)((it / p.stages) & 1));
+                }
+            }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
-        const uint32_t idesc = idesc_mx_e4m3(C::BF, BT);
-        int it = 0, tc = 0;
-        bool ok = true, any = false;
-        for (int tile = blockIdx.x; ok && tile < ntiles; tile += gridDim.x, ++tc) {
-            const int buf = tc % C::D_BUFS;
-            if (!mbar_wait_warp(dempty + buf, ((tc / C::D_BUFS) & 1) ^ 1, abort_flag, status, 2u)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t d = tmem + buf * C::D_COLS;
-            for (int kt = 0; kt < KT; ++kt, ++it) {
-                const int s = it % C::STAGES, f = it % C::SLOTS;
-                if (!mbar_wait_warp(sfull + f, (it / C::SLOTS) & 1, abort_flag, status, 2u) ||
-                    !mbar_wait_warp(full + s, (it / C::STAGES) & 1, abort_flag, status, 2u)) { ok = false; break; }
-                tc_fence_after();
-                const uint64_t adesc = smem_desc_sw128(smem_u32(smem + s * C::STAGE));
-                const uint64_t bdesc = smem_desc_sw128(smem_u32(smem + s * C::STAGE + C::W_STAGE));
-                const uint32_t sf = tmem + C::SF_COL + f * C::SLOT;
-                // Past the end of K both operands are zeros: whole MMAs of them are left out.
-                const int nj = K - kt * kFp8Block < kFp8Block ? (K - kt * kFp8Block + 31) / 32 : 4;
-                for (int j = 0; j < nj; ++j)
-                    tc_mma_mx_elect(d, adesc + 2ull * j, bdesc + 2ull * j, idesc, sf, sf + 4, (kt | j) != 0);
-                tc_commit_elect(done + s);
-                any = true;
+        // One thread does all of it: one wait, four MMAs and one commit per step.  (The whole warp
+        // waiting and an election per MMA took 820 cycles a step, whatever the tile's width.)
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc0 = idesc_mx_e4m3(CG * kTokens, p.bn);
+            const uint64_t adesc0 = smem_desc_sw128(smem_u32(smem));
+            auto commit = [&](uint64_t* bar) {
+                if (PAIR) tc_commit_pair(bar);
+                else tc_commit(bar);
+            };
+            int s = 0, slot = 0, tc = 0;
+            uint32_t phase = 0, sphase = 0;
+            bool ok = true, any = false;
+            for (int tile = first; ok && tile < ntiles; tile += stride, ++tc) {
+                const int buf = tc & 1;
+                if (!mbar_wait(dempty + buf, ((tc >> 1) & 1) ^ 1, abort_flag, status, 2u)) { ok = false; break; }
+                const uint32_t d = tmem + buf * d_cols;
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int q = kt & 3;
+                    const uint32_t sf = tmem + sf_col + slot * slot_cols;
+                    if (q == 0) {
+                        if (!mbar_wait<PAIR>(sfull + slot, sphase, abort_flag, status, 2u)) { ok = false; break; }
+                        const uint64_t cells = smem_desc_rows16(smem_u32(sscale + slot * kCells));
+                        tc_cp_32x16_x4<PAIR>(sf, cells);
+                        tc_cp_32x16_x4<PAIR>(sf + 4, cells + 32);
+                        if (sb_cols > 4) tc_cp_32x16_x4<PAIR>(sf + 8, cells + 64);
+                    }
+                    if (!mbar_wait(full + s, phase, abort_flag, status, 2u)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t adesc = adesc0 + (uint32_t)((s * stage_bytes) >> 4);
+                    const uint64_t bdesc = adesc + (kXStage >> 4);
+                    const uint32_t idesc = idesc0 | ((uint32_t)q << 29) | ((uint32_t)q << 4);   // scale byte q of A and B
+                    // A 32-value piece is 32 bytes along the swizzled rows: +2 in the
+                    // descriptors' 16-byte units.  Pieces past the end of K are zeros: left out.
+                    const int left = p.k - kt * kFp8Block;
+                    tc_mma_mx<PAIR>(d, adesc, bdesc, idesc, sf, sf + 4, kt != 0);
+                    if (left > 32) tc_mma_mx<PAIR>(d, adesc + 2, bdesc + 2, idesc, sf, sf + 4, 1);
+                    if (left > 64) tc_mma_mx<PAIR>(d, adesc + 4, bdesc + 4, idesc, sf, sf + 4, 1);
+                    if (left > 96) tc_mma_mx<PAIR>(d, adesc + 6, bdesc + 6, idesc, sf, sf + 4, 1);
+                    commit(done + s);
+                    any = true;
+                    if (++s == p.stages) { s = 0; phase ^= 1; }
+                    if (q == 3 || kt == KT - 1) {
+                        commit(sempty + slot);
+                        if (++slot == kSlots) { slot = 0; sphase ^= 1; }
+                    }
+                }
+                if (!ok) break;
+                commit(dfull + buf);
             }
-            if (!ok) break;
-            tc_commit_elect(dfull + buf);
-        }
-        if (!ok && any) {
-            tc_commit_elect(drain);
-            mbar_wait_drain(drain, 0);
+            if (!ok && any) {
+                commit(drain);
+                mbar_wait_drain(drain, 0);
+            }
         }
     } else if (warp >= 4 && warp < 8) {
         // ------------------------------------------------------------ scales
-        // Lane l of each of the four warps holds, per step, W's scale (the same for all 128
-        // features) and those of tokens l, l + 32, ...: the columns of its quarter.
-        constexpr int NX = C::SB_COLS, AHEAD = 4;
-        const uint32_t quarter = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        uint32_t next[AHEAD][NX + 1];
-        auto fetch = [&](int tile, int kt0) {
+        // Warp w lays groups w, w + 4, ... of the CTA's steps, all in scale slot w: lane l fetches
+        // the bytes of rows l, l + 32, ... (X's 128 rows of this CTA, and W's bn, all of them in each
+        // CTA of a pair) for the group's four steps and puts them into the slot's cells in shared
+        // memory; the MMA thread has them copied to tensor memory in order with its MMAs.  A fence or
+        // an arrival waits for the loads before it, so a warp has the time of four groups for one
+        // (when the four worked on every group together, that latency set the pace of the MMAs).
+        const uint32_t sfull0 = PAIR ? cluster_addr(sfull, 0) : 0;
+        const int w = warp & 3, per_tile = (KT + 3) / 4;
+        const int groups = first < ntiles ? ((ntiles - 1 - first) / stride + 1) * per_tile : 0;
+        uint32_t raw[48];
+        auto fetch = [&](int g) {
+            const int i = g / per_tile, kt0 = 4 * (g - i * per_tile);
             int ft, tt;
-            place(tile, ft, tt);
+            place(first + i * stride, ft, tt);
+            const int t = (tt * CG + (int)rank) * kTokens + lane, f = ft * p.bn + lane;
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                const int kt = kt0 + i;
-                if (kt < KT) {
-                    next[i][0] = __ldg(ws + (int64_t)ft * KT + kt);
-                    const uint8_t* row = xs + (int64_t)kt * M;
+            for (int q = 0; q < 4; ++q) {
+                const int kt = kt0 + q;
+                const bool in = kt < KT;
+                const uint8_t* x = xs + (int64_t)kt * p.m + t;
 #pragma unroll
-                    for (int c = 0; c < NX; ++c) {
-                        const int t = 32 * c + lane;
-                        next[i][1 + c] = t < BT && (int64_t)tt * BT + t < M ? __ldg(row + (int64_t)tt * BT + t) : 127u;
+                for (int c = 0; c < 12; ++c) {
+                    uint32_t& b = raw[4 * c + q];
+                    b = 127u;                                      // 1.0 for rows that are not there
+                    if (c < 4) {
+                        if (in && t + 32 * c < p.m) b = __ldg(x + 32 * c);
+                    } else {
+                        const uint32_t fc = (uint32_t)(f + 32 * (c - 4));
+                        if (in && c - 4 < sb_cols && fc < (uint32_t)p.n) b = __ldg(ws + (int64_t)(fc / kFp8Block) * KT + kt);
                     }
                 }
             }
         };
-        int it = 0;
-        bool ok = true;
-        if ((int)blockIdx.x < ntiles) fetch(blockIdx.x, 0);
-        for (int tile = blockIdx.x; ok && tile < ntiles; tile += gridDim.x) {
-            for (int kt0 = 0; ok && kt0 < KT; kt0 += AHEAD) {
-                uint32_t cur[AHEAD][NX + 1];
+        uint32_t phase = 1;
+        if (w < groups) fetch(w);
+        for (int g = w; g < groups; g += kSlots, phase ^= 1) {
+            if (!mbar_wait_warp(sempty + w, phase, abort_flag, status, 4u)) break;
+            uint4* cells = reinterpret_cast<uint4*>(sscale + w * kCells) + lane;
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i)
+            for (int c = 0; c < 3; ++c) {
+                uint32_t o[4];
 #pragma unroll
-                    for (int c = 0; c <= NX; ++c) cur[i][c] = next[i][c] * 0x01010101u;
-                if (kt0 + AHEAD < KT) fetch(tile, kt0 + AHEAD);
-                else if (tile + (int)gridDim.x < ntiles) fetch(tile + gridDim.x, 0);
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    if (ok && kt0 + i < KT) {
-                        const int f = it % C::SLOTS;
-                        if (it >= C::SLOTS) {                        // the step that used the slot last
-                            const int prev = it - C::SLOTS;
-                            ok = mbar_wait_warp(done + prev % C::STAGES, (prev / C::STAGES) & 1, abort_flag, status, 4u);
-                        }
-                        if (ok) {
-                            tc_fence_after();
-                            const uint32_t at = tmem + quarter + C::SF_COL + f * C::SLOT;
-                            tmem_st4(at, cur[i][0], cur[i][0], cur[i][0], cur[i][0]);
-#pragma unroll
-                            for (int c = 0; c < NX; c += 4)
-                                tmem_st4(at + 4 + c, cur[i][1 + c], cur[i][2 + c], cur[i][3 + c], cur[i][4 + c]);
-                            tc_wait_st();
-                            tc_fence_before();
-                            mbar_arrive(sfull + f);
-                            ++it;
-                        }
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t* b = raw + 4 * (4 * c + j);
+                    o[j] = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
                 }
+                cells[32 * c] = make_uint4(o[0], o[1], o[2], o[3]);
             }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) mbar_arrive_at(sfull0 + 8 * w);
+                else mbar_arrive(sfull + w);
+            }
+            if (g + kSlots < groups) fetch(g + kSlots);
         }
     } else if (warp >= 8) {
         // ------------------------------------------------------------ output stage
-        // Thread = feature: 16 tokens of the accumulator at a time.  A warp's 32 features are 64
-        // (f32: 128) consecutive bytes of a token's row.
-        const int fl = 32 * (warp & 3) + lane;
+        // Thread = token (its quarter of the lanes); group e of four warps takes pieces e, e + 2, ...
+        // of 16 features.
+        const int e = (warp - 8) >> 2, tid = threadIdx.x - 256;
         const uint32_t quarter = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+        const uint32_t dempty0 = PAIR ? cluster_addr(dempty, 0) : 0;
+        float* mine = stage32 + (warp - 8) * 32 * kPitch;
         int tc = 0;
-        for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++tc) {
+        for (int tile = first; tile < ntiles; tile += stride, ++tc) {
             int ft, tt;
             place(tile, ft, tt);
-            const int buf = tc % C::D_BUFS;
-            const int f = ft * C::BF + fl;
-            float badd = 0.f, gmul = 1.f;
-            if (epi.bias != nullptr && f < N)
-                badd = YF32 ? reinterpret_cast<const float*>(epi.bias)[f] : bf16_bits_to_f32(epi.bias[f]);
-            if (FUSED && epi.gate != nullptr && f < N) gmul = bf16_bits_to_f32(epi.gate[f]);
-            if (!__all_sync(0xffffffffu, mbar_wait_sleep(dfull + buf, (tc / C::D_BUFS) & 1, abort_flag, status, 8u, 64))) break;
+            const int buf = tc & 1, f0 = ft * p.bn;
+            const int width = p.n - f0 < p.bn ? p.n - f0 : p.bn;
+            const int row0 = (tt * CG + (int)rank) * kTokens + 32 * (warp & 3);      // the warp's first token
+            const int row = row0 + lane;
+            // The tile's bias and gate, as f32, for all eight warps.
+            named_barrier_sync(1, 256);
+            {
+                const int f = f0 + tid;
+                const bool in = tid < width;
+                sbias[tid] = !in || epi.bias == nullptr ? 0.f
+                             : YF32 ? reinterpret_cast<const float*>(epi.bias)[f] : bf16_bits_to_f32(epi.bias[f]);
+                if (FUSED) sgate[tid] = !in || epi.gate == nullptr ? 1.f : bf16_bits_to_f32(epi.gate[f]);
+            }
+            const bool resid = FUSED && epi.resid != nullptr;
+            const bool ok = __all_sync(0xffffffffu, mbar_wait_sleep(dfull + buf, (tc >> 1) & 1, abort_flag, status, 8u, 32));
+            // All eight warps go on or none does: none is left at a barrier.
+            if (!named_barrier_and(1, 256, ok)) break;
             tc_fence_after();
-            const int64_t t0 = (int64_t)tt * BT;
-            for (int c = 0; c < BT / 16; ++c) {
-                uint32_t v[16];
+            for (int c = row0 < p.m ? 16 * e : width; c < width; c += 32) {
+                const int64_t at = (int64_t)row * p.n + f0 + c;
+                uint32_t r[8], v[16];
+                if (resid && p.aligned && row < p.m) ld_global_32(r, epi.resid + at);
                 __syncwarp();
-                tmem_ld16(tmem + quarter + buf * C::D_COLS + 16 * c, v);
+                tmem_ld16(tmem + quarter + buf * d_cols + c, v);
                 tc_wait_ld();
+                float a[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int64_t t = t0 + 16 * c + j;
-                    if (t < M && f < N) {
-                        float a = __uint_as_float(v[j]) + badd;
-                        if (FUSED) {
-                            a = epi_activation(a, epi.act) * gmul;
-                            if (epi.resid != nullptr) a += bf16_bits_to_f32(epi.resid[t * N + f]);
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 b = *reinterpret_cast<const float4*>(sbias + c + j);
+                    a[j] = __uint_as_float(v[j]) + b.x;
+                    a[j + 1] = __uint_as_float(v[j + 1]) + b.y;
+                    a[j + 2] = __uint_as_float(v[j + 2]) + b.z;
+                    a[j + 3] = __uint_as_float(v[j + 3]) + b.w;
+                    if (FUSED) {
+                        const float4 g = *reinterpret_cast<const float4*>(sgate + c + j);
+                        a[j] = epi_activation(a[j], epi.act) * g.x;
+                        a[j + 1] = epi_activation(a[j + 1], epi.act) * g.y;
+                        a[j + 2] = epi_activation(a[j + 2], epi.act) * g.z;
+                        a[j + 3] = epi_activation(a[j + 3], epi.act) * g.w;
+                    }
+                }
+                if (p.aligned) {
+                    if (row < p.m) {
+                        uint32_t o[8];
+                        if (YF32) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(a[8 * h + j]);
+                                st_global_32(static_cast<float*>(y) + at + 8 * h, o);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                if (resid) {
+                                    a[2 * j] += bf16_bits_to_f32(r[j] & 0xFFFFu);
+                                    a[2 * j + 1] += bf16_bits_to_f32(r[j] >> 16);
+                                }
+                                o[j] = pack_bf16x2(a[2 * j], a[2 * j + 1]);
+                            }
+                            st_global_32(static_cast<uint16_t*>(y) + at, o);
                         }
-                        if (YF32) static_cast<float*>(y)[t * N + f] = a;
-                        else static_cast<uint16_t*>(y)[t * N + f] = (uint16_t)(pack_bf16x2(a, 0.f) & 0xFFFFu);
+                    }
+                } else {
+                    // Any other pitch: the warp turns its 32 tokens x 16 features around in shared
+                    // memory, and half-warps store 16 features of a token side by side.
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) mine[lane * kPitch + j] = a[j];
+                    __syncwarp();
+                    const int f = f0 + c + (lane & 15);
+                    if ((lane & 15) < width - c) {
+#pragma unroll 4
+                        for (int i = 0; i < 32; i += 2) {
+                            const int t = row0 + i + (lane >> 4);
+                            if (t < p.m) {
+                                float z = mine[(i + (lane >> 4)) * kPitch + (lane & 15)];
+                                const int64_t to = (int64_t)t * p.n + f;
+                                if (resid) z += bf16_bits_to_f32(epi.resid[to]);
+                                if (YF32) static_cast<float*>(y)[to] = z;
+                                else static_cast<uint16_t*>(y)[to] = (uint16_t)(pack_bf16x2(z, 0.f) & 0xFFFFu);
+                            }
+                        }
                     }
                 }
             }
-            __syncwarp();
             tc_fence_before();
-            mbar_arrive(dempty + buf);
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) mbar_arrive_at(dempty0 + 8 * buf);
+                else mbar_arrive(dempty + buf);
+            }
         }
     }
 
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();                    // no MMA, copy or arrival still needs the peer
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        if (PAIR) tmem_dealloc_pair(tmem, 512);
+        else tmem_dealloc(tmem, 512);
     }
 }
 
@@ -288,39 +418,55 @@ bool byte_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int b
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BT, bool FUSED, bool YF32>
-cudaError_t launch_mm_t(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t k, const uint8_t* wq,
-                        const uint8_t* ws, int64_t n, const EpiArgs& epi, void* y, cudaStream_t st, const char** msg) {
-    using C = MmCfg<BT>;
-    CUtensorMap tmX, tmW;
-    if (!byte_map(&tmX, xq, m, k, BT) || !byte_map(&tmW, wq, n, k, C::BF)) {
-        *msg = "cuTensorMapEncodeTiled rejected an fp8 operand's tensor map";
-        return cudaErrorInvalidValue;
+// The tile: a CTA or a pair, and the width, by the time of the longest SM: whole waves of tiles,
+// each KT steps of the longer of the MMAs (2 cycles a feature), the copies (about 40 bytes a
+// cycle from L2) and a step's fixed cost, and a tile's start and end.
+void choose(int64_t m, int64_t n, int64_t k, bool& pair, int& bn) {
+    const int64_t kt = (k + kFp8Block - 1) / kFp8Block, sms = num_sms();
+    int64_t best = -1;
+    for (int cg = 1; cg <= (m > kTokens ? 2 : 1); ++cg) {
+        const int64_t ntt = (m + kTokens * cg - 1) / (kTokens * cg);
+        const int64_t x_rows = m < kTokens ? m : kTokens;
+        for (int w = 16; w <= kMaxBn; w += 16) {
+            const int64_t tiles = ntt * ((n + w - 1) / w), waves = (tiles + sms / cg - 1) / (sms / cg);
+            const int64_t copy = (x_rows + w / cg) * kFp8Block / 40, mma = 2 * w;
+            int64_t step = mma > copy ? mma : copy;
+            step = step < 240 ? 240 : step;
+            const int64_t cost = waves * (kt * step + 600);
+            if (best < 0 || cost < best) {
+                best = cost;
+                pair = cg == 2;
+                bn = w;
+            }
+        }
     }
+}
+
+template <bool PAIR, bool FUSED, bool YF32>
+cudaError_t launch_mm_t(const CUtensorMap& tmX, const CUtensorMap& tmW, const uint8_t* xs, const uint8_t* ws,
+                        const EpiArgs& epi, void* y, const MmPlan& p, int grid, size_t smem, cudaStream_t st) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     static bool configured[64] = {};
-    if (dev >= 0 && dev < 64 && !configured[dev]) {
-        e = cudaFuncSetAttribute(fp8_mm_kernel<BT, FUSED, YF32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    auto kernel = fp8_mm_kernel<PAIR, FUSED, YF32>;
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQmvMaxSmem);
         if (e != cudaSuccess) return e;
-        configured[dev] = true;
+        if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    const int64_t nft = (n + C::BF - 1) / C::BF, ntt = (m + BT - 1) / BT, tiles = nft * ntt;
-    const int64_t fit = (32ll << 20) / ((int64_t)BT * k);          // token tiles whose X is 32 MB
-    const int64_t group = fit < 1 ? 1 : (fit < ntt ? fit : ntt);
-    const int grid = (int)(tiles < num_sms() ? tiles : num_sms());
-    fp8_mm_kernel<BT, FUSED, YF32><<<grid, kMmThreads, C::SMEM, st>>>(tmX, tmW, xs, ws, epi, y, (int)m, (int)n, (int)k,
-                                                                      (int)group);
-    return cudaGetLastError();
-}
-
-template <int BT>
-cudaError_t launch_mm_f(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t k, const uint8_t* wq,
-                        const uint8_t* ws, int64_t n, const EpiArgs& epi, void* y, cudaStream_t st, const char** msg) {
-    if (epi.fused()) return launch_mm_t<BT, true, false>(xq, xs, m, k, wq, ws, n, epi, y, st, msg);
-    if (epi.f32) return launch_mm_t<BT, false, true>(xq, xs, m, k, wq, ws, n, epi, y, st, msg);
-    return launch_mm_t<BT, false, false>(xq, xs, m, k, wq, ws, n, epi, y, st, msg);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kMmThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, tmX, tmW, xs, ws, epi, y, p);
 }
 
 }  // namespace
@@ -328,10 +474,39 @@ cudaError_t launch_mm_f(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t
 cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t k, const uint8_t* wq,
                           const uint8_t* ws, int64_t n, const EpiArgs& epi, void* y, cudaStream_t st,
                           const char** msg) {
-    if (m <= 16) return launch_mm_f<16>(xq, xs, m, k, wq, ws, n, epi, y, st, msg);
-    if (m <= 64) return launch_mm_f<64>(xq, xs, m, k, wq, ws, n, epi, y, st, msg);
-    if (m <= 128) return launch_mm_f<128>(xq, xs, m, k, wq, ws, n, epi, y, st, msg);
-    return launch_mm_f<224>(xq, xs, m, k, wq, ws, n, epi, y, st, msg);
+    MmPlan p{};
+    bool pair = false;
+    choose(m, n, k, pair, p.bn);
+    const int cg = pair ? 2 : 1;
+    p.m = (int)m;
+    p.n = (int)n;
+    p.k = (int)k;
+    p.x_rows = m < kTokens ? (int)((m + 7) / 8 * 8) : kTokens;
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(y) | (epi.resid ? reinterpret_cast<uintptr_t>(epi.resid) : 0);
+    p.aligned = n % 16 == 0 && bases % 32 == 0;
+    const size_t fixed = kFixedSmem + (p.aligned ? 0 : kTransposeSmem), stage = kXStage + (size_t)(p.bn / cg) * kFp8Block;
+    const int fit = (int)((kQmvMaxSmem - fixed) / stage);
+    p.stages = fit < kMaxStages ? fit : kMaxStages;
+    const int64_t nft = (n + p.bn - 1) / p.bn, ntt = (m + cg * kTokens - 1) / (cg * kTokens), tiles = nft * ntt;
+    const int64_t fit_tt = (32ll << 20) / ((int64_t)cg * kTokens * k);     // token tiles whose X is 32 MB
+    p.group = (int)(fit_tt < 1 ? 1 : (fit_tt < ntt ? fit_tt : ntt));
+    const int64_t places = num_sms() / cg;
+    const int grid = (int)(tiles < places ? tiles : places) * cg;
+    CUtensorMap tmX, tmW;
+    if (!byte_map(&tmX, xq, m, k, p.x_rows) || !byte_map(&tmW, wq, n, k, p.bn / cg)) {
+        *msg = "cuTensorMapEncodeTiled rejected an fp8 operand's tensor map";
+        return cudaErrorInvalidValue;
+    }
+    // More than half of an SM's shared memory, so that no second CTA waits there for tensor memory.
+    size_t smem = fixed + p.stages * stage;
+    if (smem < 120 * 1024) smem = 120 * 1024;
+    auto go = [&](auto pr) {
+        constexpr bool P = decltype(pr)::value;
+        if (epi.fused()) return launch_mm_t<P, true, false>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
+        if (epi.f32) return launch_mm_t<P, false, true>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
+        return launch_mm_t<P, false, false>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
+    };
+    return pair ? go(std::true_type{}) : go(std::false_type{});
 }
 
 cudaError_t read_and_clear_fp8_status(unsigned int* out, cudaStream_t st) {
