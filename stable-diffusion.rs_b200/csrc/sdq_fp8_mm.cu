@@ -18,7 +18,7 @@
 //   warp 0       TMA producer of the operand ring (one thread)
 //   warp 1       tensor memory allocator and MMA issuer (one thread; in a pair, rank 0's)
 //   warps 4-7    scale bytes: global -> registers, four groups ahead -> shared memory
-//   warps 8-15   output stage, two groups of four warps taking 16 features in turn
+//   warps 8-15   output stage, two groups of four warps taking 32 features in turn
 // Every mbarrier wait is bounded; on expiry the kernel records a status bit, waits for its own
 // copies and MMAs, frees its tensor memory and returns.
 #include <cstdint>
@@ -46,7 +46,7 @@ constexpr int kMaxStages = 12;
 constexpr int kSlots = 4;                          // scale groups in tensor memory, one for each scale warp
 constexpr int kCells = 3 * 512;                    // bytes of a group's scales in shared memory
 static_assert(2 * kMaxBn + kSlots * 12 <= 512, "tensor memory");
-constexpr int kPitch = 17;                         // words per token of a warp's transposing buffer
+constexpr int kPitch = 33;                         // words per token of a warp's transposing buffer
 constexpr int kFixedSmem = 1024 /* alignment */ + 512 /* barriers */ + 2 * 256 * 4 /* bias, gate */ +
                            kSlots * kCells;
 constexpr int kTransposeSmem = 8 * 32 * kPitch * 4;
@@ -60,6 +60,40 @@ struct MmPlan {
     int x_rows;            // rows of X a CTA loads (128, or M rounded up to 8)
     int aligned;           // rows of y (and resid) start on 32 bytes and hold whole 16-feature pieces
 };
+
+__device__ __forceinline__ uint64_t pack2(float2 a) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+    return unpack2(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+    return unpack2(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)), "l"(pack2(c)));
+    return unpack2(r);
+}
+// epi_activation's GELU of two values: a (1 + tanh(a (c + 0.044715 c a^2))) / 2, c = sqrt(2/pi),
+// with the same hardware tanh, in packed arithmetic.
+__device__ __forceinline__ float2 gelu2(float2 a) {
+    const float c = 0.7978845608028654f, k = 0.044715f * c;
+    const float2 arg = mul2(a, fma2(mul2(a, a), make_float2(k, k), make_float2(c, c)));
+    const float2 h = mul2(a, make_float2(0.5f, 0.5f));
+    return fma2(h, make_float2(tanh_approx(arg.x), tanh_approx(arg.y)), h);
+}
 
 template <bool PAIR, bool FUSED, bool YF32>
 __global__ void __launch_bounds__(kMmThreads, 1)
@@ -191,35 +225,35 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                 const int buf = tc & 1;
                 if (!mbar_wait(dempty + buf, ((tc >> 1) & 1) ^ 1, abort_flag, status, 2u)) { ok = false; break; }
                 const uint32_t d = tmem + buf * d_cols;
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int q = kt & 3;
+                for (int kt0 = 0; kt0 < KT; kt0 += 4) {
+                    if (!mbar_wait<PAIR>(sfull + slot, sphase, abort_flag, status, 2u)) { ok = false; break; }
                     const uint32_t sf = tmem + sf_col + slot * slot_cols;
-                    if (q == 0) {
-                        if (!mbar_wait<PAIR>(sfull + slot, sphase, abort_flag, status, 2u)) { ok = false; break; }
-                        const uint64_t cells = smem_desc_rows16(smem_u32(sscale + slot * kCells));
-                        tc_cp_32x16_x4<PAIR>(sf, cells);
-                        tc_cp_32x16_x4<PAIR>(sf + 4, cells + 32);
-                        if (sb_cols > 4) tc_cp_32x16_x4<PAIR>(sf + 8, cells + 64);
+                    const uint64_t cells = smem_desc_rows16(smem_u32(sscale + slot * kCells));
+                    tc_cp_32x16_x4<PAIR>(sf, cells);
+                    tc_cp_32x16_x4<PAIR>(sf + 4, cells + 32);
+                    if (sb_cols > 4) tc_cp_32x16_x4<PAIR>(sf + 8, cells + 64);
+                    const int left = p.k - kt0 * kFp8Block;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (left <= q * kFp8Block) break;
+                        if (!mbar_wait(full + s, phase, abort_flag, status, 2u)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint64_t adesc = adesc0 + (uint32_t)(s * (stage_bytes >> 4));
+                        const uint64_t bdesc = adesc + (kXStage >> 4);
+                        const uint32_t idesc = idesc0 | ((uint32_t)q << 29) | ((uint32_t)q << 4);   // scale byte q of A and B
+                        // A 32-value piece is 32 bytes along the swizzled rows: +2 in the
+                        // descriptors' 16-byte units.  Pieces past the end of K are zeros: left out.
+                        tc_mma_mx<PAIR>(d, adesc, bdesc, idesc, sf, sf + 4, q != 0 || kt0 != 0);
+                        if (left > q * kFp8Block + 32) tc_mma_mx<PAIR>(d, adesc + 2, bdesc + 2, idesc, sf, sf + 4, 1);
+                        if (left > q * kFp8Block + 64) tc_mma_mx<PAIR>(d, adesc + 4, bdesc + 4, idesc, sf, sf + 4, 1);
+                        if (left > q * kFp8Block + 96) tc_mma_mx<PAIR>(d, adesc + 6, bdesc + 6, idesc, sf, sf + 4, 1);
+                        commit(done + s);
+                        any = true;
+                        if (++s == p.stages) { s = 0; phase ^= 1; }
                     }
-                    if (!mbar_wait(full + s, phase, abort_flag, status, 2u)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint64_t adesc = adesc0 + (uint32_t)((s * stage_bytes) >> 4);
-                    const uint64_t bdesc = adesc + (kXStage >> 4);
-                    const uint32_t idesc = idesc0 | ((uint32_t)q << 29) | ((uint32_t)q << 4);   // scale byte q of A and B
-                    // A 32-value piece is 32 bytes along the swizzled rows: +2 in the
-                    // descriptors' 16-byte units.  Pieces past the end of K are zeros: left out.
-                    const int left = p.k - kt * kFp8Block;
-                    tc_mma_mx<PAIR>(d, adesc, bdesc, idesc, sf, sf + 4, kt != 0);
-                    if (left > 32) tc_mma_mx<PAIR>(d, adesc + 2, bdesc + 2, idesc, sf, sf + 4, 1);
-                    if (left > 64) tc_mma_mx<PAIR>(d, adesc + 4, bdesc + 4, idesc, sf, sf + 4, 1);
-                    if (left > 96) tc_mma_mx<PAIR>(d, adesc + 6, bdesc + 6, idesc, sf, sf + 4, 1);
-                    commit(done + s);
-                    any = true;
-                    if (++s == p.stages) { s = 0; phase ^= 1; }
-                    if (q == 3 || kt == KT - 1) {
-                        commit(sempty + slot);
-                        if (++slot == kSlots) { slot = 0; sphase ^= 1; }
-                    }
+                    if (!ok) break;
+                    commit(sempty + slot);
+                    if (++slot == kSlots) { slot = 0; sphase ^= 1; }
                 }
                 if (!ok) break;
                 commit(dfull + buf);
@@ -290,7 +324,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     } else if (warp >= 8) {
         // ------------------------------------------------------------ output stage
         // Thread = token (its quarter of the lanes); group e of four warps takes pieces e, e + 2, ...
-        // of 16 features.
+        // of 32 features.
         const int e = (warp - 8) >> 2, tid = threadIdx.x - 256;
         const uint32_t quarter = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t dempty0 = PAIR ? cluster_addr(dempty, 0) : 0;
@@ -313,73 +347,107 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                 if (FUSED) sgate[tid] = !in || epi.gate == nullptr ? 1.f : bf16_bits_to_f32(epi.gate[f]);
             }
             const bool resid = FUSED && epi.resid != nullptr;
+            if (resid) {
+                // The residual tile on its way to L2 while the accumulator fills: group e, sixteen of
+                // the warp's rows, four lanes a row, 64 features (128 bytes) each.
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int t = row0 + 16 * e + 8 * i + (lane >> 2), c = 64 * (lane & 3);
+                    if (c < width && t < p.m) prefetch_l2(epi.resid + (int64_t)t * p.n + f0 + c);
+                }
+            }
             const bool ok = __all_sync(0xffffffffu, mbar_wait_sleep(dfull + buf, (tc >> 1) & 1, abort_flag, status, 8u, 32));
             // All eight warps go on or none does: none is left at a barrier.
             if (!named_barrier_and(1, 256, ok)) break;
             tc_fence_after();
-            for (int c = row0 < p.m ? 16 * e : width; c < width; c += 32) {
-                const int64_t at = (int64_t)row * p.n + f0 + c;
-                uint32_t r[8], v[16];
-                if (resid && p.aligned && row < p.m) ld_global_32(r, epi.resid + at);
-                __syncwarp();
-                tmem_ld16(tmem + quarter + buf * d_cols + c, v);
-                tc_wait_ld();
-                float a[16];
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const float4 b = *reinterpret_cast<const float4*>(sbias + c + j);
-                    a[j] = __uint_as_float(v[j]) + b.x;
-                    a[j + 1] = __uint_as_float(v[j + 1]) + b.y;
-                    a[j + 2] = __uint_as_float(v[j + 2]) + b.z;
-                    a[j + 3] = __uint_as_float(v[j + 3]) + b.w;
-                    if (FUSED) {
-                        const float4 g = *reinterpret_cast<const float4*>(sgate + c + j);
-                        a[j] = epi_activation(a[j], epi.act) * g.x;
-                        a[j + 1] = epi_activation(a[j + 1], epi.act) * g.y;
-                        a[j + 2] = epi_activation(a[j + 2], epi.act) * g.z;
-                        a[j + 3] = epi_activation(a[j + 3], epi.act) * g.w;
+            if (row0 < p.m) {                                       // warps of tokens that are not there rest
+                const uint32_t acc = tmem + quarter + buf * d_cols;
+                for (int c = 32 * e; c < width; c += 64) {
+                    const int64_t at = (int64_t)row * p.n + f0 + c;
+                    const bool wide = width - c > 16;               // 32 features of this piece, or 16
+                    uint32_t r[16], v[32];
+                    if (resid && p.aligned && row < p.m) {
+                        ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[0]), epi.resid + at);
+                        if (wide) ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[8]), epi.resid + at + 16);
                     }
-                }
-                if (p.aligned) {
-                    if (row < p.m) {
-                        uint32_t o[8];
-                        if (YF32) {
+                    __syncwarp();
+                    tmem_ld32(acc + c, v);
+                    tc_wait_ld();
+                    float2 o[16];
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
+                    for (int j = 0; j < 16; ++j)
+                        o[j] = add2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])),
+                                    *reinterpret_cast<const float2*>(sbias + c + 2 * j));
+                    if (FUSED) {                                    // one decision a piece, not one a value
+                        if (epi.act == SDQ_ACT_GELU_TANH) {
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(a[8 * h + j]);
-                                st_global_32(static_cast<float*>(y) + at + 8 * h, o);
-                            }
-                        } else {
+                            for (int j = 0; j < 16; ++j) o[j] = gelu2(o[j]);
+                        } else if (epi.act == SDQ_ACT_SILU) {
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                if (resid) {
-                                    a[2 * j] += bf16_bits_to_f32(r[j] & 0xFFFFu);
-                                    a[2 * j + 1] += bf16_bits_to_f32(r[j] >> 16);
-                                }
-                                o[j] = pack_bf16x2(a[2 * j], a[2 * j + 1]);
-                            }
-                            st_global_32(static_cast<uint16_t*>(y) + at, o);
+                            for (int j = 0; j < 16; ++j)
+                                o[j] = make_float2(epi_activation(o[j].x, SDQ_ACT_SILU), epi_activation(o[j].y, SDQ_ACT_SILU));
+                        }
+                        if (epi.gate != nullptr) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = mul2(o[j], *reinterpret_cast<const float2*>(sgate + c + 2 * j));
                         }
                     }
-                } else {
-                    // Any other pitch: the warp turns its 32 tokens x 16 features around in shared
-                    // memory, and half-warps store 16 features of a token side by side.
-                    __syncwarp();
+                    if (p.aligned) {
+                        if (row < p.m) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) mine[lane * kPitch + j] = a[j];
-                    __syncwarp();
-                    const int f = f0 + c + (lane & 15);
-                    if ((lane & 15) < width - c) {
-#pragma unroll 4
-                        for (int i = 0; i < 32; i += 2) {
-                            const int t = row0 + i + (lane >> 4);
-                            if (t < p.m) {
-                                float z = mine[(i + (lane >> 4)) * kPitch + (lane & 15)];
-                                const int64_t to = (int64_t)t * p.n + f;
-                                if (resid) z += bf16_bits_to_f32(epi.resid[to]);
-                                if (YF32) static_cast<float*>(y)[to] = z;
-                                else static_cast<uint16_t*>(y)[to] = (uint16_t)(pack_bf16x2(z, 0.f) & 0xFFFFu);
+                            for (int h = 0; h < 2; ++h) {
+                                if (h == 1 && !wide) break;
+                                uint32_t w[8];
+                                if (YF32) {
+#pragma unroll
+                                    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                                        for (int j = 0; j < 4; ++j) {
+                                            w[2 * j] = __float_as_uint(o[8 * h + 4 * u + j].x);
+                                            w[2 * j + 1] = __float_as_uint(o[8 * h + 4 * u + j].y);
+                                        }
+                                        st_global_32(static_cast<float*>(y) + at + 16 * h + 8 * u, w);
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) {
+                                        float2 z = o[8 * h + j];
+                                        if (resid)
+                                            z = add2(z, make_float2(bf16_bits_to_f32(r[8 * h + j] & 0xFFFFu),
+                                                                    bf16_bits_to_f32(r[8 * h + j] >> 16)));
+                                        w[j] = pack_bf16x2(z.x, z.y);
+                                    }
+                                    st_global_32(static_cast<uint16_t*>(y) + at + 16 * h, w);
+                                }
+                            }
+                        }
+                    } else {
+                        // Any other pitch: the warp turns its 32 tokens x 32 features around in shared
+                        // memory and stores a token's features side by side.
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            mine[lane * kPitch + 2 * j] = o[j].x;
+                            mine[lane * kPitch + 2 * j + 1] = o[j].y;
+                        }
+                        __syncwarp();
+                        const int rows = p.m - row0 < 32 ? p.m - row0 : 32;
+                        if (lane < width - c) {
+                            const int64_t to = (int64_t)row0 * p.n + f0 + c + lane;
+                            for (int t0 = 0; t0 < rows; t0 += 8) {
+                                float z[8];
+#pragma unroll
+                                for (int t = 0; t < 8; ++t) {
+                                    z[t] = resid && t0 + t < rows ? bf16_bits_to_f32(epi.resid[to + (int64_t)(t0 + t) * p.n]) : 0.f;
+                                    z[t] += mine[(t0 + t) * kPitch + lane];
+                                }
+#pragma unroll
+                                for (int t = 0; t < 8; ++t) {
+                                    if (t0 + t < rows) {
+                                        if (YF32) static_cast<float*>(y)[to + (int64_t)(t0 + t) * p.n] = z[t];
+                                        else static_cast<uint16_t*>(y)[to + (int64_t)(t0 + t) * p.n] = (uint16_t)(pack_bf16x2(z[t], 0.f) & 0xFFFFu);
+                                    }
+                                }
                             }
                         }
                     }
@@ -419,9 +487,9 @@ bool byte_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int b
 }
 
 // The tile: a CTA or a pair, and the width, by the time of the longest SM: whole waves of tiles,
-// each KT steps of the longer of the MMAs (2 cycles a feature), the copies (about 40 bytes a
-// cycle from L2) and a step's fixed cost, and a tile's start and end.
-void choose(int64_t m, int64_t n, int64_t k, bool& pair, int& bn) {
+// each KT steps of the longest of the MMAs (2 cycles a feature, 300 at least), the copies (about 40
+// bytes a cycle from L2), the last wave's output stage on top.
+void choose(int64_t m, int64_t n, int64_t k, bool fused, bool& pair, int& bn) {
     const int64_t kt = (k + kFp8Block - 1) / kFp8Block, sms = num_sms();
     int64_t best = -1;
     for (int cg = 1; cg <= (m > kTokens ? 2 : 1); ++cg) {
@@ -429,10 +497,11 @@ void choose(int64_t m, int64_t n, int64_t k, bool& pair, int& bn) {
         const int64_t x_rows = m < kTokens ? m : kTokens;
         for (int w = 16; w <= kMaxBn; w += 16) {
             const int64_t tiles = ntt * ((n + w - 1) / w), waves = (tiles + sms / cg - 1) / (sms / cg);
-            const int64_t copy = (x_rows + w / cg) * kFp8Block / 40, mma = 2 * w;
-            int64_t step = mma > copy ? mma : copy;
-            step = step < 240 ? 240 : step;
-            const int64_t cost = waves * (kt * step + 600);
+            const int64_t copy = (x_rows + w / cg) * kFp8Block / 40;
+            int64_t step = 2 * w > copy ? 2 * w : copy;
+            step = step < 300 ? 300 : step;
+            const int64_t out = 600 + w * (fused ? 24 : 12), tile = kt * step > out ? kt * step : out;
+            const int64_t cost = waves * tile + out;
             if (best < 0 || cost < best) {
                 best = cost;
                 pair = cg == 2;
@@ -476,7 +545,7 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
                           const char** msg) {
     MmPlan p{};
     bool pair = false;
-    choose(m, n, k, pair, p.bn);
+    choose(m, n, k, epi.fused(), pair, p.bn);
     const int cg = pair ? 2 : 1;
     p.m = (int)m;
     p.n = (int)n;

@@ -385,6 +385,9 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_slot, uint32_t nc
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
 // 32 bytes at once; the address is 32-byte aligned.
 __device__ __forceinline__ void ld_global_32(uint32_t (&r)[8], const void* p) {
     asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
