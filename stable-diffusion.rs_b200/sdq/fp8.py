@@ -17,6 +17,7 @@ from dataclasses import dataclass
 
 import torch
 
+from . import _ACTS
 from ._abi import SDQ_BF16, SDQ_ERR_INVALID, SDQ_ERR_UNSUPPORTED, SDQ_F32, SdqError, check, lib
 
 #: Values that share a scale, along a row (activations) or both ways (weights).
@@ -24,15 +25,18 @@ BLOCK = 128
 
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _SOURCE = {torch.bfloat16: SDQ_BF16, torch.float32: SDQ_F32}
+_NAMES = {torch.bfloat16: "bf16", torch.float32: "f32"}
 _current_device = torch.cuda.current_device
 
 
-def _raw_stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _elsewhere(fn, device, stream, *args, **kw):
     """``fn`` again with ``stream`` current (allocations included), or on another device."""
+    if device.type != "cuda":
+        raise SdqError(SDQ_ERR_INVALID, "libsdq takes device tensors (no CPU fallback)")
     if stream is not None:
         if not isinstance(stream, torch.cuda.Stream):
             stream = torch.cuda.ExternalStream(int(stream), device=device)
@@ -44,28 +48,26 @@ def _elsewhere(fn, device, stream, *args, **kw):
         return fn(*args, **kw)
 
 
-def _device_of(name: str, first: torch.Tensor, **others) -> torch.device:
-    """The device that every tensor given lies on; they must be contiguous device tensors."""
-    device = first.device
-    if device.type != "cuda":
+def _refuse(name: str, first: torch.Tensor, expected) -> None:
+    """Raise for the first of ``expected`` -- (name, tensor, dtypes, shape or count) -- that is not a
+    contiguous tensor like that on ``first``'s device.  The entry points test all of it in one
+    expression, which costs a call of a few microseconds less, and come here when that fails."""
+    if not first.is_cuda:
         raise SdqError(SDQ_ERR_INVALID, "libsdq takes device tensors (no CPU fallback)")
-    if not first.is_contiguous():
-        raise SdqError(SDQ_ERR_INVALID, f"libsdq takes contiguous row-major tensors; {name} is not")
-    for n, t in others.items():
+    for n, t, dtypes, shape in expected:
         if t is None:
             continue
-        if t.device != device:
-            raise SdqError(SDQ_ERR_INVALID, f"{n} is on {t.device}, {name} on {device}")
+        if t.device != first.device:
+            raise SdqError(SDQ_ERR_INVALID, f"{n} is on {t.device}, {name} on {first.device}")
         if not t.is_contiguous():
             raise SdqError(SDQ_ERR_INVALID, f"libsdq takes contiguous row-major tensors; {n} is not")
-    return device
-
-
-def _want(name: str, t: torch.Tensor, dtype, shape) -> None:
-    if t.dtype is not dtype:
-        raise SdqError(SDQ_ERR_UNSUPPORTED, f"{name} must be {dtype}, not {t.dtype}")
-    if tuple(t.shape) != shape:
-        raise SdqError(SDQ_ERR_INVALID, f"{name} must have shape {list(shape)}, not {list(t.shape)}")
+        if isinstance(shape, int) and (t.numel() != shape or t.dtype not in dtypes):
+            raise SdqError(SDQ_ERR_INVALID, f"{n} must hold {shape} values of {dtypes[0]}, not {t.numel()} of {t.dtype}")
+        if t.dtype not in dtypes:
+            raise SdqError(SDQ_ERR_UNSUPPORTED, f"{n} must be {' or '.join(_NAMES.get(d, str(d)) for d in dtypes)}, not {t.dtype}")
+        if isinstance(shape, tuple) and tuple(t.shape) != shape:
+            raise SdqError(SDQ_ERR_INVALID, f"{n} must have shape {list(shape)}, not {list(t.shape)}")
+    raise SdqError(SDQ_ERR_INVALID, f"invalid arguments beside {name}")
 
 
 def _rows(x: torch.Tensor, name: str):
@@ -76,23 +78,18 @@ def _rows(x: torch.Tensor, name: str):
     return x.numel() // k, k
 
 
-def _source(t: torch.Tensor, name: str) -> int:
-    code = _SOURCE.get(t.dtype)
-    if code is None:
-        raise SdqError(SDQ_ERR_UNSUPPORTED, f"{name} must be bf16 or f32, not {t.dtype}")
-    return code
-
-
 def fp8_quantize(x: torch.Tensor, stream=None):
     """Activations x [..., k] (bf16 or f32) -> (xq [..., k] e4m3, xs [ceil(k / 128), rows] e8m0),
     rows the product of the leading axes (``sdq_fp8_quantize``).  k is a multiple of 16."""
-    dev = _device_of("x", x)
-    if stream is not None or dev.index != _current_device():
-        return _elsewhere(fp8_quantize, dev, stream, x)
-    dt = _source(x, "x")
+    dev = x.get_device()
+    if stream is not None or dev < 0 or dev != _current_device():
+        return _elsewhere(fp8_quantize, x.device, stream, x)
+    dt = _SOURCE.get(x.dtype)
+    if dt is None or not x.is_contiguous():
+        _refuse("x", x, [("x", x, tuple(_SOURCE), None)])
     m, k = _rows(x, "x")
     xq = torch.empty_like(x, dtype=E4M3)
-    xs = torch.empty((-(-k // BLOCK), m), dtype=E8M0, device=dev)
+    xs = x.new_empty((-(-k // BLOCK), m), dtype=E8M0)
     check(lib().sdq_fp8_quantize(x.data_ptr(), dt, m, k, xq.data_ptr(), xs.data_ptr(), _raw_stream(dev)))
     return xq, xs
 
@@ -100,15 +97,17 @@ def fp8_quantize(x: torch.Tensor, stream=None):
 def fp8_quantize_weight(w: torch.Tensor, stream=None):
     """A weight w [n, k] (bf16 or f32) -> (wq [n, k] e4m3, ws [ceil(n / 128), ceil(k / 128)] e8m0)
     (``sdq_fp8_quantize_weight``).  k is a multiple of 16."""
-    dev = _device_of("w", w)
-    if stream is not None or dev.index != _current_device():
-        return _elsewhere(fp8_quantize_weight, dev, stream, w)
-    dt = _source(w, "w")
+    dev = w.get_device()
+    if stream is not None or dev < 0 or dev != _current_device():
+        return _elsewhere(fp8_quantize_weight, w.device, stream, w)
+    dt = _SOURCE.get(w.dtype)
+    if dt is None or not w.is_contiguous():
+        _refuse("w", w, [("w", w, tuple(_SOURCE), None)])
     if w.dim() != 2:
         raise SdqError(SDQ_ERR_INVALID, f"fp8_quantize_weight wants a 2-D weight, got shape {list(w.shape)}")
     n, k = w.shape
-    wq = torch.empty((n, k), dtype=E4M3, device=dev)
-    ws = torch.empty((-(-n // BLOCK), -(-k // BLOCK)), dtype=E8M0, device=dev)
+    wq = torch.empty_like(w, dtype=E4M3)
+    ws = w.new_empty((-(-n // BLOCK), -(-k // BLOCK)), dtype=E8M0)
     check(lib().sdq_fp8_quantize_weight(w.data_ptr(), dt, n, k, wq.data_ptr(), ws.data_ptr(), _raw_stream(dev)))
     return wq, ws
 
@@ -116,19 +115,25 @@ def fp8_quantize_weight(w: torch.Tensor, stream=None):
 def fp8_dequantize(q: torch.Tensor, scales: torch.Tensor, weight: bool, out_dtype=torch.bfloat16, stream=None):
     """The values that e4m3 codes and their scales stand for, rounded once (``sdq_fp8_dequantize``).
     ``weight`` says which scales they are: a weight's 128 x 128 blocks or an activation's groups."""
-    dev = _device_of("q", q, scales=scales)
-    if stream is not None or dev.index != _current_device():
-        return _elsewhere(fp8_dequantize, dev, stream, q, scales, weight, out_dtype)
+    dev = q.get_device()
+    if stream is not None or dev < 0 or dev != _current_device():
+        return _elsewhere(fp8_dequantize, q.device, stream, q, scales, weight, out_dtype)
     rows, k = _rows(q, "q")
     kb = -(-k // BLOCK)
-    _want("q", q, E4M3, tuple(q.shape))
-    _want("scales", scales, E8M0, (-(-rows // BLOCK), kb) if weight else (kb, rows))
+    shape = (-(-rows // BLOCK), kb) if weight else (kb, rows)
+    if not (q.dtype is E4M3 and scales.dtype is E8M0 and scales.shape == shape and scales.get_device() == dev
+            and q.is_contiguous() and scales.is_contiguous()):
+        _refuse("q", q, [("q", q, (E4M3,), None), ("scales", scales, (E8M0,), shape)])
     if out_dtype not in _SOURCE:
         raise SdqError(SDQ_ERR_UNSUPPORTED, f"out must be bf16 or f32, not {out_dtype}")
     out = torch.empty_like(q, dtype=out_dtype)
     check(lib().sdq_fp8_dequantize(q.data_ptr(), scales.data_ptr(), rows, k, int(bool(weight)), out.data_ptr(),
                                    _SOURCE[out_dtype], _raw_stream(dev)))
     return out
+
+
+def _like(t, dev: int, dtype, count: int) -> bool:
+    return t.dtype is dtype and t.numel() == count and t.get_device() == dev and t.is_contiguous()
 
 
 def fp8_matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias=None, act=None,
@@ -138,31 +143,40 @@ def fp8_matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.T
 
     ``act`` is None, ``"gelu_approx"`` or ``"silu"``; ``bias`` and ``gate`` hold n values, ``residual``
     has the result's shape and may be ``out`` itself."""
-    dev = _device_of("xq", xq, xs=xs, wq=wq, ws=ws, bias=bias, gate=gate, residual=residual, out=out)
-    if stream is not None or dev.index != _current_device():
-        return _elsewhere(fp8_matmul, dev, stream, xq, xs, wq, ws, bias, act, gate, residual, out, out_dtype)
-    from . import _ACTS
-
-    if act not in _ACTS:
+    dev = xq.get_device()
+    if stream is not None or dev < 0 or dev != _current_device():
+        return _elsewhere(fp8_matmul, xq.device, stream, xq, xs, wq, ws, bias, act, gate, residual, out, out_dtype)
+    code = _ACTS.get(act)
+    if code is None:
         raise SdqError(SDQ_ERR_INVALID, f"unknown activation {act!r}")
     m, k = _rows(xq, "xq")
     if wq.dim() != 2:
         raise SdqError(SDQ_ERR_INVALID, f"wq must be 2-D, got shape {list(wq.shape)}")
-    n, kb = wq.shape[0], -(-k // BLOCK)
-    shape = (*xq.shape[:-1], n)
-    _want("xq", xq, E4M3, tuple(xq.shape))
-    _want("xs", xs, E8M0, (kb, m))
-    _want("wq", wq, E4M3, (n, k))
-    _want("ws", ws, E8M0, (-(-n // BLOCK), kb))
+    n, wk = wq.shape
+    kb = -(-k // BLOCK)
+    nb = -(-n // BLOCK)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=dev)
-    dt = _source(out, "out")
-    _want("out", out, out.dtype if out_dtype is None else out_dtype, shape)
-    for name, t, count in (("bias", bias, n), ("gate", gate, n), ("residual", residual, m * n)):
-        if t is not None and (t.numel() != count or t.dtype is not out.dtype):
-            raise SdqError(SDQ_ERR_INVALID, f"{name} must hold {count} values of {out.dtype}, not {t.numel()} of {t.dtype}")
+        dtype = torch.bfloat16 if out_dtype is None else out_dtype
+    else:
+        dtype = out.dtype
+    dt = _SOURCE.get(dtype)
+    if not (dt is not None and xq.dtype is E4M3 and wq.dtype is E4M3 and xs.dtype is E8M0 and ws.dtype is E8M0 and wk == k
+            and xs.shape == (kb, m) and ws.shape == (nb, kb) and wq.get_device() == xs.get_device() == ws.get_device() == dev
+            and xq.is_contiguous() and wq.is_contiguous() and xs.is_contiguous() and ws.is_contiguous()
+            and (bias is None or _like(bias, dev, dtype, n)) and (gate is None or _like(gate, dev, dtype, n))
+            and (residual is None or _like(residual, dev, dtype, m * n))
+            and (out is None or (_like(out, dev, dtype if out_dtype is None else out_dtype, m * n)
+                                 and out.shape == (*xq.shape[:-1], n)))):
+        if dt is None:
+            raise SdqError(SDQ_ERR_UNSUPPORTED, f"out must be bf16 or f32, not {dtype}")
+        _refuse("xq", xq, [
+            ("xq", xq, (E4M3,), None), ("xs", xs, (E8M0,), (kb, m)), ("wq", wq, (E4M3,), (n, k)), ("ws", ws, (E8M0,), (nb, kb)),
+            ("out", out, (dtype if out_dtype is None else out_dtype,), (*xq.shape[:-1], n)), ("bias", bias, (dtype,), n),
+            ("gate", gate, (dtype,), n), ("residual", residual, (dtype,), m * n)])
+    if out is None:
+        out = xq.new_empty((m, n) if xq.dim() == 2 else (*xq.shape[:-1], n), dtype=dtype)
     check(lib().sdq_fp8_matmul(xq.data_ptr(), xs.data_ptr(), m, k, wq.data_ptr(), ws.data_ptr(), n,
-                               None if bias is None else bias.data_ptr(), _ACTS[act],
+                               None if bias is None else bias.data_ptr(), code,
                                None if gate is None else gate.data_ptr(),
                                None if residual is None else residual.data_ptr(), out.data_ptr(), dt, _raw_stream(dev)))
     return out

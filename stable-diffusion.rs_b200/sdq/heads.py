@@ -2,19 +2,44 @@
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import torch
 
 from ._abi import SDQ_ERR_INVALID, SDQ_ERR_UNSUPPORTED, SdqError, SdqHeads, check, lib
-from .fp8 import _SOURCE, _current_device, _elsewhere, _raw_stream
+from .fp8 import _SOURCE, _current_device, _elsewhere, _like, _raw_stream
 
-_byref = ctypes.byref
 _PAIRS = {"interleaved": 1, "halves": 0}
+_WIDE = {torch.int32: 0, torch.int64: 1}
+_HEADS = ctypes.sizeof(SdqHeads)               # five 64-bit fields
 
 
-def _heads(t: torch.Tensor, tokens_axis: int) -> SdqHeads:
-    st = t.stride()
-    return SdqHeads(t.data_ptr(), t.shape[3 - tokens_axis], st[0], st[tokens_axis], st[3 - tokens_axis])
+def _refuse(dev: int, dtype, b: int, n: int, d: int, tensors, weights, cos, sin, positions) -> None:
+    """Raise for the first argument that is not what the call needs (the caller has seen that one is)."""
+    for name, t, o in tensors:
+        if t.dim() != 4 or t.shape[0] != b or t.shape[1] != n or t.shape[3] != d:
+            raise SdqError(SDQ_ERR_INVALID, f"{name} must be [{b}, {n}, heads, {d}], got shape {list(t.shape)}")
+        if tuple(o.shape) != (b, t.shape[2], n, d):
+            raise SdqError(SDQ_ERR_INVALID, f"{name}'s output must be {[b, t.shape[2], n, d]}, got shape {list(o.shape)}")
+        for x in (t, o):
+            if x.dtype is not dtype or x.get_device() != dev:
+                raise SdqError(SDQ_ERR_INVALID, f"{name} and its output must be {dtype} on cuda:{dev}, not {x.dtype} on {x.device}")
+            if x.stride(3) != 1:
+                raise SdqError(SDQ_ERR_INVALID, f"{name} and its output must have a contiguous last axis")
+    for name, w in weights:
+        if w is not None and not _like(w, dev, dtype, d):
+            raise SdqError(SDQ_ERR_INVALID, f"{name} must hold {d} contiguous values of {dtype} on cuda:{dev}")
+    if (cos is None) != (sin is None):
+        raise SdqError(SDQ_ERR_INVALID, "cos and sin come together")
+    if cos is not None:
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dim() != 2 or t.shape != cos.shape or not _like(t, dev, torch.float32, cos.numel()):
+                raise SdqError(SDQ_ERR_INVALID, f"{name} must be a contiguous f32 [positions, rope / 2] on cuda:{dev}")
+    if positions is not None:
+        if cos is None:
+            raise SdqError(SDQ_ERR_INVALID, "positions without cos and sin")
+        raise SdqError(SDQ_ERR_INVALID, f"positions must be int32 or int64 [{b}, {n}] on cuda:{dev}, contiguous along the tokens")
+    raise SdqError(SDQ_ERR_INVALID, "invalid arguments")
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
@@ -31,60 +56,56 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None
     (i, i + rope / 2); values from rope on stay.  ``out`` gives the three results' places, views
     [b, heads, n, d] of any strides with a contiguous last axis, for instance parts of a joint sequence.
     An output may be its input's own memory (with the same strides), and must not overlap otherwise."""
-    dev = q.device
-    if dev.type != "cuda":
-        raise SdqError(SDQ_ERR_INVALID, "libsdq takes device tensors (no CPU fallback)")
-    if stream is not None or dev.index != _current_device():
-        return _elsewhere(qk_norm_rope, dev, stream, q, k, v, q_weight, k_weight, cos, sin, eps, positions, pairs, out)
-    if pairs not in _PAIRS:
+    dev = q.get_device()
+    if stream is not None or dev < 0 or dev != _current_device():
+        return _elsewhere(qk_norm_rope, q.device, stream, q, k, v, q_weight, k_weight, cos, sin, eps, positions, pairs, out)
+    turn = _PAIRS.get(pairs)
+    if turn is None:
         raise SdqError(SDQ_ERR_INVALID, f"pairs must be 'interleaved' or 'halves', not {pairs!r}")
     dtype = q.dtype
-    if dtype not in _SOURCE:
+    dt = _SOURCE.get(dtype)
+    if dt is None:
         raise SdqError(SDQ_ERR_UNSUPPORTED, f"q must be bf16 or f32, not {dtype}")
     if q.dim() != 4:
         raise SdqError(SDQ_ERR_INVALID, f"q must be [batch, tokens, heads, head_dim], got shape {list(q.shape)}")
     b, n, _, d = q.shape
     srcs = (q, k) if v is None else (q, k, v)
     if out is None:
-        outs = [torch.empty((b, t.shape[2], n, d), dtype=dtype, device=dev) if t.dim() == 4 else t for t in srcs]
+        outs = [q.new_empty((b, t.shape[2] if t.dim() == 4 else 0, n, d)) for t in srcs]
     else:
         outs = [t for t in out if t is not None]
         if len(outs) != len(srcs):
             raise SdqError(SDQ_ERR_INVALID, f"out must hold {len(srcs)} tensors, got {len(outs)}")
-    for name, t, o in zip("qkv", srcs, outs):
-        if t.dim() != 4 or t.shape[0] != b or t.shape[1] != n or t.shape[3] != d:
-            raise SdqError(SDQ_ERR_INVALID, f"{name} must be [{b}, {n}, heads, {d}], got shape {list(t.shape)}")
-        if tuple(o.shape) != (b, t.shape[2], n, d):
-            raise SdqError(SDQ_ERR_INVALID, f"{name}'s output must be {[b, t.shape[2], n, d]}, got shape {list(o.shape)}")
-        for x in (t, o):
-            if x.dtype is not dtype or x.device != dev:
-                raise SdqError(SDQ_ERR_INVALID, f"{name} and its output must be {dtype} on {dev}, not {x.dtype} on {x.device}")
-            if x.stride(3) != 1 and d > 1 and x.numel() > 0:
-                raise SdqError(SDQ_ERR_INVALID, f"{name} and its output must have a contiguous last axis")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype is not dtype or w.device != dev or w.numel() != d or not w.is_contiguous()):
-            raise SdqError(SDQ_ERR_INVALID, f"{name} must hold {d} contiguous values of {dtype} on {dev}")
-    rows = rope = wide = stride = 0
-    if (cos is None) != (sin is None):
-        raise SdqError(SDQ_ERR_INVALID, "cos and sin come together")
-    if cos is not None:
-        for name, t in (("cos", cos), ("sin", sin)):
-            if t.dim() != 2 or t.shape != cos.shape or t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous():
-                raise SdqError(SDQ_ERR_INVALID, f"{name} must be a contiguous f32 [positions, rope / 2] on {dev}")
-        rows, rope = cos.shape[0], 2 * cos.shape[1]
+    good, table = True, array("q")
+    for t, o in zip(srcs, outs):
+        ts, os = t.shape, o.shape
+        if not (len(ts) == 4 and len(os) == 4 and ts[0] == b and ts[1] == n and ts[3] == d and os[0] == b and os[1] == ts[2]
+                and os[2] == n and os[3] == d and t.dtype is dtype and o.dtype is dtype and t.get_device() == o.get_device() == dev):
+            good = False
+            break
+        ti, oi = t.stride(), o.stride()
+        good = good and ti[3] == 1 == oi[3]
+        table.extend((t.data_ptr(), ts[2], ti[0], ti[1], ti[2], o.data_ptr(), ts[2], oi[0], oi[2], oi[1]))
+    rows = rope = wide = stride = cp = sp = pp = 0
+    if good and cos is not None and sin is not None and cos.dim() == 2 and sin.shape == cos.shape:
+        rows, rope = cos.shape
+        good = _like(cos, dev, torch.float32, rows * rope) and _like(sin, dev, torch.float32, rows * rope)
+        rope, cp, sp = 2 * rope, cos.data_ptr(), sin.data_ptr()
+    elif cos is not None or sin is not None:
+        good = False
     if positions is not None:
-        if cos is None:
-            raise SdqError(SDQ_ERR_INVALID, "positions without cos and sin")
-        if tuple(positions.shape) != (b, n) or positions.device != dev or positions.dtype not in (torch.int32, torch.int64) \
-                or (n > 1 and positions.stride(1) != 1):
-            raise SdqError(SDQ_ERR_INVALID, f"positions must be int32 or int64 [{b}, {n}] on {dev}, contiguous along the tokens")
-        wide, stride = int(positions.dtype is torch.int64), positions.stride(0)
-    i = [_heads(t, 1) for t in srcs]
-    o = [_heads(t, 2) for t in outs]
+        wide = _WIDE.get(positions.dtype)
+        good = good and cos is not None and wide is not None and positions.shape == (b, n) and positions.get_device() == dev
+        if good:
+            stride, step = positions.stride()
+            good = step == 1 or n == 1
+            pp = positions.data_ptr()
+    if not (good and (q_weight is None or _like(q_weight, dev, dtype, d)) and (k_weight is None or _like(k_weight, dev, dtype, d))):
+        _refuse(dev, dtype, b, n, d, list(zip("qkv", srcs, outs)), (("q_weight", q_weight), ("k_weight", k_weight)), cos, sin,
+                positions)
+    at = table.buffer_info()[0]                    # sdq_heads: input and output of q, of k, of v
     check(lib().sdq_qk_norm_rope(
-        _byref(i[0]), _byref(i[1]), _byref(i[2]) if v is not None else None, _byref(o[0]), _byref(o[1]),
-        _byref(o[2]) if v is not None else None, _SOURCE[dtype], b, n, d,
-        None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
-        None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), rows, rope, _PAIRS[pairs],
-        None if positions is None else positions.data_ptr(), wide, stride, _raw_stream(dev)))
-    return (outs[0], outs[1], outs[2] if v is not None else None)
+        at, at + 2 * _HEADS, None if v is None else at + 4 * _HEADS, at + _HEADS, at + 3 * _HEADS,
+        None if v is None else at + 5 * _HEADS, dt, b, n, d, None if q_weight is None else q_weight.data_ptr(),
+        None if k_weight is None else k_weight.data_ptr(), eps, cp, sp, rows, rope, turn, pp, wide, stride, _raw_stream(dev)))
+    return (*outs, None) if v is None else tuple(outs)
