@@ -578,8 +578,8 @@ int sdq_qk_norm_rope(const sdq_heads* q, const sdq_heads* k, const sdq_heads* v,
     for (int i = 0; i < 3; ++i) {
         const char* name = i == 0 ? "q" : (i == 1 ? "k" : "v");
         if (!in[i]) continue;
-        if (in[i]->heads < 0 || in[i]->heads > 65536 || in[i]->heads != out[i]->heads)
-            return fail(SDQ_ERR_INVALID, "%s: %s has %lld heads and its output %lld; they must be equal, 0 to 65536", fn, name,
+        if (in[i]->heads < 0 || in[i]->heads > 16384 || in[i]->heads != out[i]->heads)
+            return fail(SDQ_ERR_INVALID, "%s: %s has %lld heads and its output %lld; they must be equal, 0 to 16384", fn, name,
                         (long long)in[i]->heads, (long long)out[i]->heads);
         all += a.heads[i] = (int)in[i]->heads;
         if (a.heads[i] == 0 || batch == 0 || tokens == 0) continue;

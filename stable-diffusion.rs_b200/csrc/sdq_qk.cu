@@ -15,9 +15,13 @@
 //
 // Bound by memory: every value is read and written once.  A vector lies in the registers of the
 // fewest lanes (a power of two) that hold it at 8 values each: 16-byte accesses for bf16, sums and
-// the halves' partners by shuffles.  A block takes one token's heads (or several tokens when there
-// are few heads), so the table row is read once and kept in registers for all of them, and each
-// lane has kBatch vectors' loads under way at once.
+// the halves' partners by shuffles.  A warp takes one token and, for each vector's worth of its
+// lanes, BATCH heads of one of the three tensors, all loads issued before the first is worked on;
+// the warps of a block take neighbouring tokens of the same heads, which lie side by side in the
+// output.  The norm's weights are multiplied into the cosines and sines once for all the heads:
+// a c - b s becomes r (x0 (w0 c) - x1 (w1 s)), three operations a value.
+// 4608 tokens, 72 heads of 128: a block a token, looping over its heads, took 63 us (49 KB a SM
+// under way); this layout 40 with the norm and the rotation one after the other.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -27,67 +31,124 @@
 namespace sdq {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kBatch = 4;      // vectors a lane loads before it works on the first
+constexpr int kWarps = 8;      // a block
 
+// Eight values as they are loaded.
 template <bool BF16>
-struct Eight {
-    float f[8];
+struct Raw;
+template <>
+struct Raw<true> {
+    uint32_t w[4];
     __device__ __forceinline__ void load(const void* p, int64_t e) {
-        if (BF16) {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + e));
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f[2 * i] = __uint_as_float(w[i] << 16);
-                f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-            }
-        } else {
-            const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + e);
-            const float4 a = __ldcs(s), b = __ldcs(s + 1);
-            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-            f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-        }
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + e));
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
     }
-    __device__ __forceinline__ void store(void* p, int64_t e) const {
-        if (BF16) {
-            uint32_t o[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-                o[i] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + e) = make_uint4(o[0], o[1], o[2], o[3]);
-        } else {
-            float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + e);
-            d[0] = make_float4(f[0], f[1], f[2], f[3]);
-            d[1] = make_float4(f[4], f[5], f[6], f[7]);
-        }
+    __device__ __forceinline__ float get(int i) const {
+        return i & 1 ? __uint_as_float(w[i >> 1] & 0xFFFF0000u) : __uint_as_float(w[i >> 1] << 16);
     }
+    static __device__ __forceinline__ void store(void* p, int64_t e, const float (&f)[8]) {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            o[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + e) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    __device__ __forceinline__ void put(void* p, int64_t e) const {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + e) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static constexpr int N = 4;
+};
+template <>
+struct Raw<false> {
+    uint32_t w[8];
+    __device__ __forceinline__ void load(const void* p, int64_t e) {
+        const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + e);
+        const uint4 a = __ldcs(s), b = __ldcs(s + 1);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    }
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(w[i]); }
+    static __device__ __forceinline__ void store(void* p, int64_t e, const float (&f)[8]) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + e);
+        d[0] = make_float4(f[0], f[1], f[2], f[3]);
+        d[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+    __device__ __forceinline__ void put(void* p, int64_t e) const {
+        uint4* d = reinterpret_cast<uint4*>(static_cast<float*>(p) + e);
+        d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+    static constexpr int N = 8;
 };
 
-// LPV lanes hold one vector; `per_token` vector slots of the block work on the same token.
-template <bool BF16, bool INTER, int LPV>
-__global__ void __launch_bounds__(kThreads) qk_kernel(const __grid_constant__ QkArgs a, int per_token) {
-    constexpr int kSlots = kThreads / LPV;
-    const int slot = threadIdx.x / LPV, l = threadIdx.x % LPV;
-    const int64_t bt = (int64_t)blockIdx.x * (kSlots / per_token) + slot / per_token;
-    const bool live = bt < a.batch * a.tokens && 8 * l < a.d;
-    const int64_t b = live ? bt / a.tokens : 0, t = live ? bt - b * a.tokens : 0;
-    const int all = a.heads[0] + a.heads[1] + a.heads[2];
-
-    // This lane's cosines and sines, if its values are in the rotated part (whole lanes are: R is
-    // a multiple of 16).  A position outside the tables reads nothing and makes the token's
-    // queries and keys NaN.
-    constexpr int NC = INTER ? 4 : 8;
-    float c[NC], s[NC];
+// LPV lanes hold one vector.  blockIdx.y counts pieces of the queries' heads, then the keys', then
+// the values'.
+template <bool BF16, bool INTER, int LPV, int BATCH>
+__global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__ QkArgs a) {
+    constexpr int kSide = 32 / LPV, kHeads = kSide * BATCH;      // vectors side by side; heads a piece
+    const int lane = threadIdx.x & 31, l = lane % LPV, e = 8 * l;
+    const int64_t bt = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (bt >= a.batch * a.tokens) return;                // whole warps
+    const int64_t b = bt / a.tokens, t = bt - b * a.tokens;
+    int piece = blockIdx.y, kind = 0;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) c[i] = s[i] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+        const int n = (a.heads[i] + kHeads - 1) / kHeads;
+        if (kind == i && piece >= n) { piece -= n; kind = i + 1; }
+    }
+    const QkTensor& x = a.in[kind];
+    const QkTensor& y = a.out[kind];
+    // Vectors this lane takes part in (a head of 80 values fills 10 of 16 lanes).
+    const int h0 = piece * kHeads + lane / LPV;
+    const int count = e < a.d ? a.heads[kind] - h0 : 0;  // vector j is there when j * kSide < count
+    int64_t from = b * x.batch_stride + t * x.token_stride + h0 * x.head_stride + e;
+    int64_t to = b * y.batch_stride + t * y.token_stride + h0 * y.head_stride + e;
+
+    Raw<BF16> v[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+        if (j * kSide < count) {
+            v[j].load(x.data, from + j * kSide * x.head_stride);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Raw<BF16>::N; ++i) v[j].w[i] = 0;
+        }
+    }
+    if (kind == 2) {
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (j * kSide < count) v[j].put(y.data, to + j * kSide * y.head_stride);
+        return;
+    }
+
+    // The norm's weights of this lane's values and, in halves, of their partners' (1 without a norm).
+    const void* weight = a.weight[kind];
     const int half = a.rope / 2;
-    const int e = 8 * l;
+    const bool turns = e < a.rope;                       // whole lanes turn or stay: R is a multiple of 16
     const bool low = e < half;                           // halves: in the first half of the pair
-    const bool turns = e < a.rope;
-    if (live && turns) {
+    const int partner = turns && !INTER ? (low ? e + half : e - half) : e;
+    float w[8], wp[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = wp[i] = 1.f;
+    if (weight != nullptr && e < a.d) {
+        Raw<BF16> g;
+        g.load(weight, e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = g.get(i);
+        if (!INTER) {
+            g.load(weight, partner);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) wp[i] = g.get(i);
+        }
+    }
+    // What each value, and its partner's, is multiplied by.  A position outside the tables reads
+    // nothing and makes the token's queries and keys NaN.
+    float own[8], other[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { own[i] = w[i]; other[i] = 0.f; }
+    if (turns) {
         int64_t row = t;
         if (a.positions != nullptr) {
             const int64_t at = b * a.pos_batch_stride + t;
@@ -95,8 +156,10 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const __grid_constant__ Qk
         }
         if (row < 0 || row >= a.table_rows) {
 #pragma unroll
-            for (int i = 0; i < NC; ++i) c[i] = s[i] = __uint_as_float(0x7FFFFFFFu);
+            for (int i = 0; i < 8; ++i) own[i] = other[i] = __uint_as_float(0x7FFFFFFFu);
         } else {
+            constexpr int NC = INTER ? 4 : 8;
+            float c[NC], s[NC];
             const int64_t at = row * half + (INTER ? e / 2 : (low ? e : e - half));
 #pragma unroll
             for (int i = 0; i < NC / 4; ++i) {
@@ -105,85 +168,68 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const __grid_constant__ Qk
                 c[4 * i] = cc.x; c[4 * i + 1] = cc.y; c[4 * i + 2] = cc.z; c[4 * i + 3] = cc.w;
                 s[4 * i] = ss.x; s[4 * i + 1] = ss.y; s[4 * i + 2] = ss.z; s[4 * i + 3] = ss.w;
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (INTER) {                             // even values: a c - b s; odd ones: b c + a s
+                    own[i] = w[i] * c[i / 2];
+                    other[i] = w[i ^ 1] * (i & 1 ? s[i / 2] : -s[i / 2]);
+                } else {
+                    own[i] = w[i] * c[i];
+                    other[i] = wp[i] * (low ? -s[i] : s[i]);
+                }
+            }
         }
     }
 
-    // Every lane of the block makes the same number of trips: the shuffles below need them all.
-    const int step = per_token * gridDim.y;
-    for (int h0 = blockIdx.y * per_token; h0 < all; h0 += kBatch * step) {
-        Eight<BF16> v[kBatch];
-        int kind[kBatch], head[kBatch];
+    float r[BATCH];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            int h = h0 + j * step + slot % per_token;
-            kind[j] = -1;
-            if (live && h < all) {
-                kind[j] = 0;
-                if (h >= a.heads[0]) { h -= a.heads[0]; kind[j] = 1; }
-                if (kind[j] == 1 && h >= a.heads[1]) { h -= a.heads[1]; kind[j] = 2; }
-                head[j] = h;
-                const QkTensor& x = a.in[kind[j]];
-                v[j].load(x.data, b * x.batch_stride + t * x.token_stride + h * x.head_stride + e);
-            } else {
+    for (int j = 0; j < BATCH; ++j) {
+        r[j] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[j].f[i] = 0.f;
-            }
+        for (int i = 0; i < 8; ++i) r[j] = fmaf(v[j].get(i), v[j].get(i), r[j]);
+    }
+#pragma unroll
+    for (int m = 1; m < LPV; m <<= 1) {
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) r[j] += __shfl_xor_sync(0xFFFFFFFFu, r[j], m);
+    }
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+        Raw<BF16> o;                                     // halves: the partner's values
+        if (!INTER) {
+            const int lp = lane + (partner - e) / 8;
+#pragma unroll
+            for (int i = 0; i < Raw<BF16>::N; ++i) o.w[i] = __shfl_sync(0xFFFFFFFFu, v[j].w[i], lp);
         }
+        if (j * kSide < count) {
+            const float rj = weight != nullptr ? rsqrtf(r[j] * a.inv_d + a.eps) : 1.f;
+            float f[8];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            float* f = v[j].f;
-            const void* w = kind[j] == 0 ? a.weight[0] : (kind[j] == 1 ? a.weight[1] : nullptr);
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
-#pragma unroll
-            for (int m = 1; m < LPV; m <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, m);
-            if (w != nullptr) {
-                const float r = rsqrtf(sum * a.inv_d + a.eps);
-                Eight<BF16> g;
-                g.load(w, e);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g.f[i];
+            for (int i = 0; i < 8; ++i) {
+                f[i] = v[j].get(i) * own[i];
+                if (turns) f[i] = fmaf(INTER ? v[j].get(i ^ 1) : o.get(i), other[i], f[i]);
+                f[i] *= rj;
             }
-            if (INTER) {
-                if (turns && kind[j] != 2) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = f[2 * i], q = f[2 * i + 1];
-                        f[2 * i] = p * c[i] - q * s[i];
-                        f[2 * i + 1] = p * s[i] + q * c[i];
-                    }
-                }
-            } else {
-                // The partner of value i lies R/2 further on: half / 8 lanes up, or down.
-                const int from = (threadIdx.x & 31) + (turns ? (low ? half / 8 : -(half / 8)) : 0);
-                float o[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xFFFFFFFFu, f[i], from);
-                if (turns && kind[j] != 2) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + (low ? -o[i] : o[i]) * s[i];
-                }
-            }
-            if (kind[j] >= 0) {
-                const QkTensor& y = a.out[kind[j]];
-                v[j].store(y.data, b * y.batch_stride + t * y.token_stride + head[j] * y.head_stride + e);
-            }
+            Raw<BF16>::store(y.data, to + j * kSide * y.head_stride, f);
         }
     }
 }
 
 template <bool BF16, bool INTER, int LPV>
 cudaError_t go(const QkArgs& a, cudaStream_t st) {
-    constexpr int kSlots = kThreads / LPV;
-    const int all = a.heads[0] + a.heads[1] + a.heads[2];
-    int per_token = kSlots;
-    while (per_token > 1 && per_token / 2 >= all) per_token /= 2;
-    const int64_t blocks = (a.batch * a.tokens + kSlots / per_token - 1) / (kSlots / per_token);
-    // Few tokens: their heads are spread over blocks, one vector per slot, rather than queued.
-    const int trips = (all + per_token - 1) / per_token;
-    const int spread = blocks * 4 < num_sms() ? trips : 1;
-    qk_kernel<BF16, INTER, LPV><<<dim3((unsigned)blocks, (unsigned)spread), kThreads, 0, st>>>(a, per_token);
+    constexpr int kSide = 32 / LPV;
+    const unsigned blocks = (unsigned)((a.batch * a.tokens + kWarps - 1) / kWarps);
+    auto pieces = [&](int heads) {
+        unsigned n = 0;
+        for (int h : a.heads) n += (unsigned)((h + heads - 1) / heads);
+        return n;
+    };
+    // Few vectors: one a lane group, spread over as many warps as there are; otherwise four, whose
+    // loads overlap.
+    if ((int64_t)blocks * pieces(4 * kSide) < 4 * num_sms())
+        qk_kernel<BF16, INTER, LPV, 1><<<dim3(blocks, pieces(kSide)), 32 * kWarps, 0, st>>>(a);
+    else
+        qk_kernel<BF16, INTER, LPV, 4><<<dim3(blocks, pieces(4 * kSide)), 32 * kWarps, 0, st>>>(a);
     return cudaGetLastError();
 }
 
