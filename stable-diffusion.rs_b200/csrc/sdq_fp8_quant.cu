@@ -31,7 +31,7 @@ struct Sixteen<true> {
     }
     __device__ void load(const void* p, int64_t e) {
         const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + e);
-        const uint4 a = __ldcs(s), b = __ldcs(s + 1);
+        const uint4 a = s[0], b = s[1];
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
         w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
     }
@@ -50,7 +50,7 @@ struct Sixteen<false> {
         const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + e);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint4 a = __ldcs(s + i);
+            const uint4 a = s[i];
             w[4 * i] = a.x; w[4 * i + 1] = a.y; w[4 * i + 2] = a.z; w[4 * i + 3] = a.w;
         }
     }

@@ -16,12 +16,12 @@
 // Bound by memory: every value is read and written once.  A vector lies in the registers of the
 // fewest lanes (a power of two) that hold it at 8 values each: 16-byte accesses for bf16, sums and
 // the halves' partners by shuffles.  A warp takes one token and, for each vector's worth of its
-// lanes, BATCH heads of one of the three tensors, all loads issued before the first is worked on;
+// lanes, kBatch heads of one of the three tensors, all loads issued before the first is worked on;
 // the warps of a block take neighbouring tokens of the same heads, which lie side by side in the
 // output.  The norm's weights are multiplied into the cosines and sines once for all the heads:
 // a c - b s becomes r (x0 (w0 c) - x1 (w1 s)), three operations a value.
 // 4608 tokens, 72 heads of 128: a block a token, looping over its heads, took 63 us (49 KB a SM
-// under way); this layout 40 with the norm and the rotation one after the other.
+// under way); this layout 40 with the norm and the rotation one after the other, now 30.5 (5.6 TB/s).
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -31,7 +31,12 @@
 namespace sdq {
 namespace {
 
-constexpr int kWarps = 8;      // a block
+// A block: 8 warps took 34 us for the case above, 4 32, 2 31.6, 1 31.2 (and 10 % longer at 4096 x 18
+// heads of 80); plain loads 3 % less than streaming ones.
+constexpr int kWarps = 2;
+// Heads a lane group loads before it works on the first: 2 took 10 % longer than 4, 8 20 %; one, for
+// calls of a few tokens, gained 4 % up to 16 tokens and lost 15 % at 128.
+constexpr int kBatch = 4;
 
 // Eight values as they are loaded.
 template <bool BF16>
@@ -40,7 +45,7 @@ template <>
 struct Raw<true> {
     uint32_t w[4];
     __device__ __forceinline__ void load(const void* p, int64_t e) {
-        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + e));
+        const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + e);
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
     }
     __device__ __forceinline__ float get(int i) const {
@@ -65,7 +70,7 @@ struct Raw<false> {
     uint32_t w[8];
     __device__ __forceinline__ void load(const void* p, int64_t e) {
         const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + e);
-        const uint4 a = __ldcs(s), b = __ldcs(s + 1);
+        const uint4 a = s[0], b = s[1];
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
         w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
     }
@@ -85,9 +90,9 @@ struct Raw<false> {
 
 // LPV lanes hold one vector.  blockIdx.y counts pieces of the queries' heads, then the keys', then
 // the values'.
-template <bool BF16, bool INTER, int LPV, int BATCH>
+template <bool BF16, bool INTER, int LPV>
 __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__ QkArgs a) {
-    constexpr int kSide = 32 / LPV, kHeads = kSide * BATCH;      // vectors side by side; heads a piece
+    constexpr int kSide = 32 / LPV, kHeads = kSide * kBatch;      // vectors side by side; heads a piece
     const int lane = threadIdx.x & 31, l = lane % LPV, e = 8 * l;
     const int64_t bt = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (bt >= a.batch * a.tokens) return;                // whole warps
@@ -106,9 +111,9 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
     int64_t from = b * x.batch_stride + t * x.token_stride + h0 * x.head_stride + e;
     int64_t to = b * y.batch_stride + t * y.token_stride + h0 * y.head_stride + e;
 
-    Raw<BF16> v[BATCH];
+    Raw<BF16> v[kBatch];
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
+    for (int j = 0; j < kBatch; ++j) {
         if (j * kSide < count) {
             v[j].load(x.data, from + j * kSide * x.head_stride);
         } else {
@@ -118,7 +123,7 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
     }
     if (kind == 2) {
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j)
+        for (int j = 0; j < kBatch; ++j)
             if (j * kSide < count) v[j].put(y.data, to + j * kSide * y.head_stride);
         return;
     }
@@ -181,9 +186,9 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
         }
     }
 
-    float r[BATCH];
+    float r[kBatch];
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
+    for (int j = 0; j < kBatch; ++j) {
         r[j] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) r[j] = fmaf(v[j].get(i), v[j].get(i), r[j]);
@@ -191,10 +196,10 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
 #pragma unroll
     for (int m = 1; m < LPV; m <<= 1) {
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) r[j] += __shfl_xor_sync(0xFFFFFFFFu, r[j], m);
+        for (int j = 0; j < kBatch; ++j) r[j] += __shfl_xor_sync(0xFFFFFFFFu, r[j], m);
     }
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
+    for (int j = 0; j < kBatch; ++j) {
         Raw<BF16> o;                                     // halves: the partner's values
         if (!INTER) {
             const int lp = lane + (partner - e) / 8;
@@ -219,17 +224,9 @@ template <bool BF16, bool INTER, int LPV>
 cudaError_t go(const QkArgs& a, cudaStream_t st) {
     constexpr int kSide = 32 / LPV;
     const unsigned blocks = (unsigned)((a.batch * a.tokens + kWarps - 1) / kWarps);
-    auto pieces = [&](int heads) {
-        unsigned n = 0;
-        for (int h : a.heads) n += (unsigned)((h + heads - 1) / heads);
-        return n;
-    };
-    // Few vectors: one a lane group, spread over as many warps as there are; otherwise four, whose
-    // loads overlap.
-    if ((int64_t)blocks * pieces(4 * kSide) < 4 * num_sms())
-        qk_kernel<BF16, INTER, LPV, 1><<<dim3(blocks, pieces(kSide)), 32 * kWarps, 0, st>>>(a);
-    else
-        qk_kernel<BF16, INTER, LPV, 4><<<dim3(blocks, pieces(4 * kSide)), 32 * kWarps, 0, st>>>(a);
+    unsigned pieces = 0;
+    for (int h : a.heads) pieces += (unsigned)((h + kBatch * kSide - 1) / (kBatch * kSide));
+    qk_kernel<BF16, INTER, LPV><<<dim3(blocks, pieces), 32 * kWarps, 0, st>>>(a);
     return cudaGetLastError();
 }
 

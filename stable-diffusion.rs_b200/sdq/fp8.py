@@ -29,8 +29,14 @@ _NAMES = {torch.bfloat16: "bf16", torch.float32: "f32"}
 _current_device = torch.cuda.current_device
 
 
-def _raw_stream(index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+try:
+    # torch's allocation without the dispatcher, on the current device: 0.8 us against 1.4 to 2.
+    from torch._C._dynamo.guards import _empty_strided_cuda as _empty_strided
+except ImportError:
+    def _empty_strided(size, stride, dtype):
+        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
 
 
 def _elsewhere(fn, device, stream, *args, **kw):
@@ -88,8 +94,10 @@ def fp8_quantize(x: torch.Tensor, stream=None):
     if dt is None or not x.is_contiguous():
         _refuse("x", x, [("x", x, tuple(_SOURCE), None)])
     m, k = _rows(x, "x")
-    xq = torch.empty_like(x, dtype=E4M3)
-    xs = x.new_empty((-(-k // BLOCK), m), dtype=E8M0)
+    xq = _empty_strided((m, k), (k, 1), E4M3)
+    if x.dim() != 2:
+        xq = xq.view(x.shape)
+    xs = _empty_strided((-(-k // BLOCK), m), (m, 1), E8M0)
     check(lib().sdq_fp8_quantize(x.data_ptr(), dt, m, k, xq.data_ptr(), xs.data_ptr(), _raw_stream(dev)))
     return xq, xs
 
@@ -106,8 +114,9 @@ def fp8_quantize_weight(w: torch.Tensor, stream=None):
     if w.dim() != 2:
         raise SdqError(SDQ_ERR_INVALID, f"fp8_quantize_weight wants a 2-D weight, got shape {list(w.shape)}")
     n, k = w.shape
-    wq = torch.empty_like(w, dtype=E4M3)
-    ws = w.new_empty((-(-n // BLOCK), -(-k // BLOCK)), dtype=E8M0)
+    kb = -(-k // BLOCK)
+    wq = _empty_strided((n, k), (k, 1), E4M3)
+    ws = _empty_strided((-(-n // BLOCK), kb), (kb, 1), E8M0)
     check(lib().sdq_fp8_quantize_weight(w.data_ptr(), dt, n, k, wq.data_ptr(), ws.data_ptr(), _raw_stream(dev)))
     return wq, ws
 
@@ -174,7 +183,9 @@ def fp8_matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.T
             ("out", out, (dtype if out_dtype is None else out_dtype,), (*xq.shape[:-1], n)), ("bias", bias, (dtype,), n),
             ("gate", gate, (dtype,), n), ("residual", residual, (dtype,), m * n)])
     if out is None:
-        out = xq.new_empty((m, n) if xq.dim() == 2 else (*xq.shape[:-1], n), dtype=dtype)
+        out = _empty_strided((m, n), (n, 1), dtype)
+        if xq.dim() != 2:
+            out = out.view((*xq.shape[:-1], n))
     check(lib().sdq_fp8_matmul(xq.data_ptr(), xs.data_ptr(), m, k, wq.data_ptr(), ws.data_ptr(), n,
                                None if bias is None else bias.data_ptr(), code,
                                None if gate is None else gate.data_ptr(),

@@ -7,7 +7,7 @@ from array import array
 import torch
 
 from ._abi import SDQ_ERR_INVALID, SDQ_ERR_UNSUPPORTED, SdqError, SdqHeads, check, lib
-from .fp8 import _SOURCE, _current_device, _elsewhere, _like, _raw_stream
+from .fp8 import _SOURCE, _current_device, _elsewhere, _empty_strided, _like, _raw_stream
 
 _PAIRS = {"interleaved": 1, "halves": 0}
 _WIDE = {torch.int32: 0, torch.int64: 1}
@@ -19,9 +19,9 @@ def _refuse(dev: int, dtype, b: int, n: int, d: int, tensors, weights, cos, sin,
     for name, t, o in tensors:
         if t.dim() != 4 or t.shape[0] != b or t.shape[1] != n or t.shape[3] != d:
             raise SdqError(SDQ_ERR_INVALID, f"{name} must be [{b}, {n}, heads, {d}], got shape {list(t.shape)}")
-        if tuple(o.shape) != (b, t.shape[2], n, d):
+        if o is not None and tuple(o.shape) != (b, t.shape[2], n, d):
             raise SdqError(SDQ_ERR_INVALID, f"{name}'s output must be {[b, t.shape[2], n, d]}, got shape {list(o.shape)}")
-        for x in (t, o):
+        for x in (t, t if o is None else o):
             if x.dtype is not dtype or x.get_device() != dev:
                 raise SdqError(SDQ_ERR_INVALID, f"{name} and its output must be {dtype} on cuda:{dev}, not {x.dtype} on {x.device}")
             if x.stride(3) != 1:
@@ -70,22 +70,34 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None
         raise SdqError(SDQ_ERR_INVALID, f"q must be [batch, tokens, heads, head_dim], got shape {list(q.shape)}")
     b, n, _, d = q.shape
     srcs = (q, k) if v is None else (q, k, v)
-    if out is None:
-        outs = [q.new_empty((b, t.shape[2] if t.dim() == 4 else 0, n, d)) for t in srcs]
-    else:
+    good, table, outs = True, array("q"), out
+    if out is not None:
         outs = [t for t in out if t is not None]
         if len(outs) != len(srcs):
             raise SdqError(SDQ_ERR_INVALID, f"out must hold {len(srcs)} tensors, got {len(outs)}")
-    good, table = True, array("q")
-    for t, o in zip(srcs, outs):
-        ts, os = t.shape, o.shape
-        if not (len(ts) == 4 and len(os) == 4 and ts[0] == b and ts[1] == n and ts[3] == d and os[0] == b and os[1] == ts[2]
-                and os[2] == n and os[3] == d and t.dtype is dtype and o.dtype is dtype and t.get_device() == o.get_device() == dev):
+    else:
+        outs = []
+    for i, t in enumerate(srcs):
+        if t.dim() != 4:
             good = False
             break
-        ti, oi = t.stride(), o.stride()
-        good = good and ti[3] == 1 == oi[3]
-        table.extend((t.data_ptr(), ts[2], ti[0], ti[1], ti[2], o.data_ptr(), ts[2], oi[0], oi[2], oi[1]))
+        tb, tn, h, td = t.shape
+        if not (tb == b and tn == n and td == d and t.dtype is dtype and t.get_device() == dev):
+            good = False
+            break
+        s0, s1, s2, s3 = t.stride()
+        if out is None:
+            o, o0, o1, o2 = _empty_strided((b, h, n, d), (h * n * d, n * d, d, 1), dtype), h * n * d, n * d, d
+            outs.append(o)
+        else:
+            o = outs[i]
+            if not (o.shape == (b, h, n, d) and o.dtype is dtype and o.get_device() == dev):
+                good = False
+                break
+            o0, o1, o2, o3 = o.stride()
+            good = good and o3 == 1
+        good = good and s3 == 1
+        table.extend((t.data_ptr(), h, s0, s1, s2, o.data_ptr(), h, o0, o2, o1))
     rows = rope = wide = stride = cp = sp = pp = 0
     if good and cos is not None and sin is not None and cos.dim() == 2 and sin.shape == cos.shape:
         rows, rope = cos.shape
@@ -101,7 +113,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None
             good = step == 1 or n == 1
             pp = positions.data_ptr()
     if not (good and (q_weight is None or _like(q_weight, dev, dtype, d)) and (k_weight is None or _like(k_weight, dev, dtype, d))):
-        _refuse(dev, dtype, b, n, d, list(zip("qkv", srcs, outs)), (("q_weight", q_weight), ("k_weight", k_weight)), cos, sin,
+        _refuse(dev, dtype, b, n, d, [(*x, outs[i] if out is not None else None) for i, x in enumerate(zip("qkv", srcs))], (("q_weight", q_weight), ("k_weight", k_weight)), cos, sin,
                 positions)
     at = table.buffer_info()[0]                    # sdq_heads: input and output of q, of k, of v
     check(lib().sdq_qk_norm_rope(
