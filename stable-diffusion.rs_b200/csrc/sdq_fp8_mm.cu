@@ -147,6 +147,11 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     __syncthreads();
     if (PAIR) cluster_sync();                    // the peer's barriers are initialised too
     tc_fence_after();
+    // Launched with programmatic stream serialisation: all of the above may run while the kernel
+    // before this one finishes; nothing that it may have written is read, and nothing is written,
+    // before this.
+    griddep_wait();
+    griddep_launch_dependents();
     const uint32_t tmem = *tmem_slot;
 
     const int KT = (p.k + kFp8Block - 1) / kFp8Block;
@@ -366,18 +371,30 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                     const int64_t at = (int64_t)row * p.n + f0 + c;
                     const bool wide = width - c > 16;               // 32 features of this piece, or 16
                     uint32_t r[16], v[32];
+                    // The residual before the accumulator: 32 features of this thread's token or,
+                    // with any other pitch, this lane's feature of the warp's 32 tokens, two a word.
+                    const int64_t to = (int64_t)row0 * p.n + f0 + c + lane;
+                    const int rows = p.m - row0 < 32 ? p.m - row0 : 32;
                     if (resid && p.aligned && row < p.m) {
                         ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[0]), epi.resid + at);
                         if (wide) ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[8]), epi.resid + at + 16);
+                    } else if (resid && lane < width - c) {
+                        uint32_t one[32];                           // no branch between the loads: all under way at once
+#pragma unroll
+                        for (int t = 0; t < 32; ++t) one[t] = epi.resid[to + (int64_t)(t < rows ? t : 0) * p.n];
+#pragma unroll
+                        for (int t = 0; t < 16; ++t) r[t] = one[2 * t] | (one[2 * t + 1] << 16);
                     }
                     __syncwarp();
                     tmem_ld32(acc + c, v);
                     tc_wait_ld();
                     float2 o[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        o[j] = add2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])),
-                                    *reinterpret_cast<const float2*>(sbias + c + 2 * j));
+                    for (int j = 0; j < 16; j += 2) {
+                        const float4 b = *reinterpret_cast<const float4*>(sbias + c + 2 * j);
+                        o[j] = add2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), make_float2(b.x, b.y));
+                        o[j + 1] = add2(make_float2(__uint_as_float(v[2 * j + 2]), __uint_as_float(v[2 * j + 3])), make_float2(b.z, b.w));
+                    }
                     if (FUSED) {                                    // one decision a piece, not one a value
                         if (epi.act == SDQ_ACT_GELU_TANH) {
 #pragma unroll
@@ -431,22 +448,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                             mine[lane * kPitch + 2 * j + 1] = o[j].y;
                         }
                         __syncwarp();
-                        const int rows = p.m - row0 < 32 ? p.m - row0 : 32;
                         if (lane < width - c) {
-                            const int64_t to = (int64_t)row0 * p.n + f0 + c + lane;
-                            for (int t0 = 0; t0 < rows; t0 += 8) {
-                                float z[8];
 #pragma unroll
-                                for (int t = 0; t < 8; ++t) {
-                                    z[t] = resid && t0 + t < rows ? bf16_bits_to_f32(epi.resid[to + (int64_t)(t0 + t) * p.n]) : 0.f;
-                                    z[t] += mine[(t0 + t) * kPitch + lane];
-                                }
-#pragma unroll
-                                for (int t = 0; t < 8; ++t) {
-                                    if (t0 + t < rows) {
-                                        if (YF32) static_cast<float*>(y)[to + (int64_t)(t0 + t) * p.n] = z[t];
-                                        else static_cast<uint16_t*>(y)[to + (int64_t)(t0 + t) * p.n] = (uint16_t)(pack_bf16x2(z[t], 0.f) & 0xFFFFu);
-                                    }
+                            for (int t = 0; t < 32; ++t) {
+                                if (t < rows) {
+                                    float z = mine[t * kPitch + lane];
+                                    if (resid) z += bf16_bits_to_f32(t & 1 ? r[t / 2] >> 16 : r[t / 2] & 0xFFFFu);
+                                    if (YF32) static_cast<float*>(y)[to + (int64_t)t * p.n] = z;
+                                    else static_cast<uint16_t*>(y)[to + (int64_t)t * p.n] = (uint16_t)(pack_bf16x2(z, 0.f) & 0xFFFFu);
                                 }
                             }
                         }
@@ -529,12 +538,14 @@ cudaError_t launch_mm_t(const CUtensorMap& tmX, const CUtensorMap& tmW, const ui
     cfg.blockDim = dim3(kMmThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = PAIR ? 1 : 0;
+    cfg.numAttrs = PAIR ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, tmX, tmW, xs, ws, epi, y, p);
 }
 
