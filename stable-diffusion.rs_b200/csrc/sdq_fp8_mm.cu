@@ -54,7 +54,9 @@ constexpr int kTransposeSmem = 8 * 32 * kPitch * 4;
 // What the host has settled for a launch.
 struct MmPlan {
     int m, n, k;
+    int kt;                // steps: blocks of K
     int bn;                // features per tile
+    int nft, ntt;          // feature tiles, token tiles
     int stages;            // ring depth
     int group;             // token tiles that are walked together (see place)
     int x_rows;            // rows of X a CTA loads (128, or M rounded up to 8)
@@ -154,10 +156,10 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     griddep_launch_dependents();
     const uint32_t tmem = *tmem_slot;
 
-    const int KT = (p.k + kFp8Block - 1) / kFp8Block;
+    const int KT = p.kt;
     const int d_cols = (p.bn + 31) / 32 * 32, sf_col = 2 * d_cols;
     const int sb_cols = (p.bn + 127) / 128 * 4, slot_cols = 4 + sb_cols;   // X's four columns, then W's
-    const int nft = (p.n + p.bn - 1) / p.bn, ntt = (p.m + CG * kTokens - 1) / (CG * kTokens), ntiles = nft * ntt;
+    const int nft = p.nft, ntt = p.ntt, ntiles = nft * ntt;
     const int first = blockIdx.x / CG, stride = gridDim.x / CG;
     // Tiles go in groups of `group` token tiles; within a group, the tokens of one feature tile
     // first.  So the CTAs at work share W's rows, and the group's X stays in L2 while W streams
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                 if (!mbar_wait(dempty + buf, ((tc >> 1) & 1) ^ 1, abort_flag, status, 2u)) { ok = false; break; }
                 const uint32_t d = tmem + buf * d_cols;
                 for (int kt0 = 0; kt0 < KT; kt0 += 4) {
-                    if (!mbar_wait<PAIR>(sfull + slot, sphase, abort_flag, status, 2u)) { ok = false; break; }
+                    if (!mbar_wait(sfull + slot, sphase, abort_flag, status, 2u)) { ok = false; break; }
                     const uint32_t sf = tmem + sf_col + slot * slot_cols;
                     const uint64_t cells = smem_desc_rows16(smem_u32(sscale + slot * kCells));
                     tc_cp_32x16_x4<PAIR>(sf, cells);
@@ -280,29 +282,34 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         const int w = warp & 3, per_tile = (KT + 3) / 4;
         const int groups = first < ntiles ? ((ntiles - 1 - first) / stride + 1) * per_tile : 0;
         uint32_t raw[48];
+        // Rows and steps that are not there read the last one's byte: what it scales is never stored
+        // or never multiplied, and loads without conditions all issue at once (48 guarded ones took
+        // 2600 cycles to).
         auto fetch = [&](int g) {
             const int i = g / per_tile, kt0 = 4 * (g - i * per_tile);
             int ft, tt;
             place(first + i * stride, ft, tt);
             const int t = (tt * CG + (int)rank) * kTokens + lane, f = ft * p.bn + lane;
+            int step[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int kt = kt0 + q;
-                const bool in = kt < KT;
-                const uint8_t* x = xs + (int64_t)kt * p.m + t;
+            for (int q = 0; q < 4; ++q) step[q] = kt0 + q < KT ? q : KT - 1 - kt0;
 #pragma unroll
-                for (int c = 0; c < 12; ++c) {
-                    uint32_t& b = raw[4 * c + q];
-                    b = 127u;                                      // 1.0 for rows that are not there
-                    if (c < 4) {
-                        if (in && t + 32 * c < p.m) b = __ldg(x + 32 * c);
-                    } else {
-                        const uint32_t fc = (uint32_t)(f + 32 * (c - 4));
-                        if (in && c - 4 < sb_cols && fc < (uint32_t)p.n) b = __ldg(ws + (int64_t)(fc / kFp8Block) * KT + kt);
-                    }
-                }
+            for (int c = 0; c < 4; ++c) {
+                const uint8_t* x = xs + (int64_t)kt0 * p.m + (t + 32 * c < p.m ? t + 32 * c : p.m - 1);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) raw[4 * c + q] = __ldg(x + (int64_t)step[q] * p.m);
+            }
+#pragma unroll
+            for (int c = 4; c < 12; ++c) {
+                if (c >= 8 && sb_cols == 4) break;
+                const int fc = f + 32 * (c - 4) < p.n ? f + 32 * (c - 4) : p.n - 1;
+                const uint8_t* row = ws + (int64_t)(fc / kFp8Block) * KT + kt0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) raw[4 * c + q] = __ldg(row + step[q]);
             }
         };
+#pragma unroll
+        for (int c = 0; c < 48; ++c) raw[c] = 0;
         uint32_t phase = 1;
         if (w < groups) fetch(w);
         for (int g = w; g < groups; g += kSlots, phase ^= 1) {
@@ -561,6 +568,7 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
     p.m = (int)m;
     p.n = (int)n;
     p.k = (int)k;
+    p.kt = (int)((k + kFp8Block - 1) / kFp8Block);
     p.x_rows = m < kTokens ? (int)((m + 7) / 8 * 8) : kTokens;
     const uintptr_t bases = reinterpret_cast<uintptr_t>(y) | (epi.resid ? reinterpret_cast<uintptr_t>(epi.resid) : 0);
     p.aligned = n % 16 == 0 && bases % 32 == 0;
@@ -568,6 +576,8 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
     const int fit = (int)((kQmvMaxSmem - fixed) / stage);
     p.stages = fit < kMaxStages ? fit : kMaxStages;
     const int64_t nft = (n + p.bn - 1) / p.bn, ntt = (m + cg * kTokens - 1) / (cg * kTokens), tiles = nft * ntt;
+    p.nft = (int)nft;
+    p.ntt = (int)ntt;
     const int64_t fit_tt = (32ll << 20) / ((int64_t)cg * kTokens * k);     // token tiles whose X is 32 MB
     p.group = (int)(fit_tt < 1 ? 1 : (fit_tt < ntt ? fit_tt : ntt));
     const int64_t places = num_sms() / cg;

@@ -68,19 +68,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
-// try_wait that acquires at cluster scope: what the peer CTA wrote before its arrivals is seen.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 // try_wait with a suspend-time hint: a thread whose phase is not complete may be
 // suspended (issuing nothing) until the phase completes or `hint_ns` passes.
 __device__ __forceinline__ bool mbar_try_wait_hint(uint64_t* bar, uint32_t parity, uint32_t hint_ns) {
@@ -98,14 +85,12 @@ __device__ __forceinline__ bool mbar_try_wait_hint(uint64_t* bar, uint32_t parit
 // Wait for the phase with `parity` to complete, giving up after the wait limit or
 // as soon as another role of this CTA has raised `*abort`.  Returns false when
 // it gave up (and then sets the abort flag and the global status bit).
-template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort,
                                           unsigned int* status, unsigned int status_bit) {
-    auto test = [&]() { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
-    if (test()) return true;
+    if (mbar_try_wait(bar, parity)) return true;
     const unsigned long long t0 = globaltimer(), lim = g_wait_limit_ns;
     for (uint32_t it = 1;; ++it) {
-        if (test()) return true;
+        if (mbar_try_wait(bar, parity)) return true;
         if ((it & 63u) == 0u) {
             if (*abort) return false;
             if (globaltimer() - t0 > lim) {
@@ -355,9 +340,12 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
 }
-// One arrival on a barrier of either CTA of the cluster, by its shared::cluster address.
+// One arrival on a barrier of either CTA of the cluster, by its shared::cluster address.  It
+// releases at CTA scope: what it orders are accesses to this CTA's own shared and tensor memory
+// before the ones that the observer then has made here.  (At cluster scope it waits for the SM's
+// memory operations in flight, and took some 3500 cycles.)
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // 2-D tiled load into this CTA whose bytes are counted on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* tmap, uint32_t bar, int32_t c0,
