@@ -368,6 +368,28 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                     if (c < width && t < p.m) prefetch_l2(epi.resid + (int64_t)t * p.n + f0 + c);
                 }
             }
+            // The residual of a piece: 32 features of this thread's token or, with any other pitch, this
+            // lane's feature of the warp's 32 tokens, two a word.  The first piece's is fetched while
+            // the accumulator fills.
+            const int rows = p.m - row0 < 32 ? p.m - row0 : 32;
+            uint32_t r[16];
+            auto fetch_resid = [&](int c) {
+                if (p.aligned) {
+                    if (row < p.m) {
+                        const uint16_t* from = epi.resid + (int64_t)row * p.n + f0 + c;
+                        ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[0]), from);
+                        if (width - c > 16) ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[8]), from + 16);
+                    }
+                } else if (lane < width - c) {
+                    const uint16_t* from = epi.resid + (int64_t)row0 * p.n + f0 + c + lane;
+                    uint32_t one[32];                               // no branch between the loads: all under way at once
+#pragma unroll
+                    for (int t = 0; t < 32; ++t) one[t] = from[(int64_t)(t < rows ? t : 0) * p.n];
+#pragma unroll
+                    for (int t = 0; t < 16; ++t) r[t] = one[2 * t] | (one[2 * t + 1] << 16);
+                }
+            };
+            if (resid && row0 < p.m && 32 * e < width) fetch_resid(32 * e);
             const bool ok = __all_sync(0xffffffffu, mbar_wait_sleep(dfull + buf, (tc >> 1) & 1, abort_flag, status, 8u, 32));
             // All eight warps go on or none does: none is left at a barrier.
             if (!named_barrier_and(1, 256, ok)) break;
@@ -377,21 +399,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                 for (int c = 32 * e; c < width; c += 64) {
                     const int64_t at = (int64_t)row * p.n + f0 + c;
                     const bool wide = width - c > 16;               // 32 features of this piece, or 16
-                    uint32_t r[16], v[32];
-                    // The residual before the accumulator: 32 features of this thread's token or,
-                    // with any other pitch, this lane's feature of the warp's 32 tokens, two a word.
-                    const int64_t to = (int64_t)row0 * p.n + f0 + c + lane;
-                    const int rows = p.m - row0 < 32 ? p.m - row0 : 32;
-                    if (resid && p.aligned && row < p.m) {
-                        ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[0]), epi.resid + at);
-                        if (wide) ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[8]), epi.resid + at + 16);
-                    } else if (resid && lane < width - c) {
-                        uint32_t one[32];                           // no branch between the loads: all under way at once
-#pragma unroll
-                        for (int t = 0; t < 32; ++t) one[t] = epi.resid[to + (int64_t)(t < rows ? t : 0) * p.n];
-#pragma unroll
-                        for (int t = 0; t < 16; ++t) r[t] = one[2 * t] | (one[2 * t + 1] << 16);
-                    }
+                    if (resid && c != 32 * e) fetch_resid(c);
+                    uint32_t v[32];
                     __syncwarp();
                     tmem_ld32(acc + c, v);
                     tc_wait_ld();
@@ -456,6 +465,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                         }
                         __syncwarp();
                         if (lane < width - c) {
+                            const int64_t to = (int64_t)row0 * p.n + f0 + c + lane;
 #pragma unroll
                             for (int t = 0; t < 32; ++t) {
                                 if (t < rows) {
