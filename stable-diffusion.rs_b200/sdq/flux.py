@@ -14,19 +14,21 @@ interleaved rotation rotate 165-212.  What sits between the linears -- LayerNorm
 query/key norm, the rotary embedding, attention, GELU, SiLU, gates and residuals -- is plain
 torch on the device: the callers' arithmetic around the quantised linear, not the path
 itself.  Every linear goes through a ``WeightSource`` (``sdq.quantized``), so the same forward
-runs on a dense source for comparison.
+runs on a dense source for comparison.  With ``fused_heads`` the split, the query/key norm, the
+concatenation of the streams and the rotation are one ``sdq.qk_norm_rope`` a stream instead, rounded
+once rather than after the norm and after the rotation.
 """
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Callable, Dict, Iterator, List, Optional, Tuple
+from typing import Callable, Dict, Iterator, List, Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
 
-from . import QuantizedArray
-from .quantized import GROUP_SIZE, QuantizedWeights, quantizable
+from . import Fp8Array, QuantizedArray, qk_norm_rope
+from .quantized import Bits, QuantizedWeights, quantize_to
 
 EPS = 1e-6
 TIME_EMBED_DIM = 256
@@ -124,19 +126,20 @@ def dense_tensor_table(cfg: FluxShape) -> List[Tuple[str, Tuple[int, ...]]]:
 
 
 def random_weights(cfg: FluxShape, seed: int = 0, device="cuda",
-                   bits: Callable[[str], int] = bits_for, keep_dense: bool = False):
-    """Random-init weights, each linear drawn on the device, quantised and its dense copy dropped
+                   bits: Callable[[str], Bits] = bits_for, keep_dense: bool = False):
+    """Random-init weights, each linear drawn on the device, quantised (to a bit width or
+    ``quantized.FP8``, as ``bits`` says) and its dense copy dropped
     before the next (the reference's one-tensor-at-a-time load, quantized.rs:273-291).  W ~ N(0,
     1/K) keeps activations O(1) through the stack.  Returns QuantizedWeights, plus (when
     ``keep_dense``) a dict of the dequantised weights and the dense tensors for comparison."""
     g = torch.Generator(device).manual_seed(seed)
-    quantized: Dict[str, QuantizedArray] = {}
+    quantized: Dict[str, Union[QuantizedArray, Fp8Array]] = {}
     dense: Dict[str, torch.Tensor] = {}
     dq: Dict[str, torch.Tensor] = {}
     for name, n, k, _ in linear_table(cfg):
         w = torch.randn(n, k, device=device, generator=g) / math.sqrt(k)
-        assert quantizable(tuple(w.shape))
-        q = QuantizedArray.quantize(w, GROUP_SIZE, bits(name))
+        q = quantize_to(w, bits(name))
+        assert q is not None, name
         quantized[name] = q
         if keep_dense:
             dq[name] = q.dequantize()
@@ -225,26 +228,43 @@ def attention(q, k, v):
     return merge_heads(F.scaled_dot_product_attention(q, k, v, scale=1.0 / math.sqrt(q.shape[-1])))
 
 
-def double_block(w, img, txt, vec, cos, sin, i, cfg: FluxShape):
+def prepare_heads(w, qkv, heads, hd, norm, cos, sin, out=None):
+    """Queries, keys and values [b, heads, n, hd] of a fused projection [b, n, 3 * heads * hd] (a view
+    of a wider one will do), normed with ``norm``'s scales and rotated; into ``out`` if given."""
+    q, k, v = qkv.unflatten(-1, (3, heads, hd)).unbind(2)
+    return qk_norm_rope(q, k, v, w.dense_tensor(f"{norm}.query_norm.scale"), w.dense_tensor(f"{norm}.key_norm.scale"),
+                        cos, sin, EPS, out=out)
+
+
+def double_block(w, img, txt, vec, cos, sin, i, cfg: FluxShape, fused_heads=False):
     p = f"double_blocks.{i}"
     heads, hd = cfg.heads, cfg.head_dim
     im = modulation(w, vec, f"{p}.img_mod", 6)
     tm = modulation(w, vec, f"{p}.txt_mod", 6)
 
+    def projection(x, m, tag):
+        return w.linear(norm_modulate(x, m[0], m[1]), f"{p}.{tag}_attn.qkv.weight",
+                        w.optional(f"{p}.{tag}_attn.qkv.bias"))
+
     def stream_qkv(x, m, tag):
-        qkv = w.linear(norm_modulate(x, m[0], m[1]), f"{p}.{tag}_attn.qkv.weight",
-                       w.optional(f"{p}.{tag}_attn.qkv.bias"))
-        q, k, v = split_qkv(qkv, heads, hd)
+        q, k, v = split_qkv(projection(x, m, tag), heads, hd)
         return (qk_norm(q, w.dense_tensor(f"{p}.{tag}_attn.norm.query_norm.scale")),
                 qk_norm(k, w.dense_tensor(f"{p}.{tag}_attn.norm.key_norm.scale")), v)
 
-    iq, ik, iv = stream_qkv(img, im, "img")
-    tq, tk, tv = stream_qkv(txt, tm, "txt")
-    q = rotate(torch.cat((tq, iq), dim=2), cos, sin)
-    k = rotate(torch.cat((tk, ik), dim=2), cos, sin)
-    v = torch.cat((tv, iv), dim=2)
-    a = attention(q, k, v)
     nt = txt.shape[1]
+    if fused_heads:
+        b, n = txt.shape[0], nt + img.shape[1]
+        q, k, v = (torch.empty((b, heads, n, hd), device=txt.device, dtype=txt.dtype) for _ in range(3))
+        for tag, x, m, at in (("txt", txt, tm, slice(0, nt)), ("img", img, im, slice(nt, n))):
+            prepare_heads(w, projection(x, m, tag), heads, hd, f"{p}.{tag}_attn.norm", cos[at], sin[at],
+                          out=(q[:, :, at], k[:, :, at], v[:, :, at]))
+    else:
+        iq, ik, iv = stream_qkv(img, im, "img")
+        tq, tk, tv = stream_qkv(txt, tm, "txt")
+        q = rotate(torch.cat((tq, iq), dim=2), cos, sin)
+        k = rotate(torch.cat((tk, ik), dim=2), cos, sin)
+        v = torch.cat((tv, iv), dim=2)
+    a = attention(q, k, v)
 
     # x + gate * linear(..) and gelu(linear(..)) run inside the linear's output stage.
     def finish(x, att, m, tag):
@@ -258,32 +278,36 @@ def double_block(w, img, txt, vec, cos, sin, i, cfg: FluxShape):
     return finish(img, a[:, nt:], im, "img"), finish(txt, a[:, :nt], tm, "txt")
 
 
-def single_block(w, x, vec, cos, sin, i, cfg: FluxShape):
+def single_block(w, x, vec, cos, sin, i, cfg: FluxShape, fused_heads=False):
     p = f"single_blocks.{i}"
     h, heads, hd = cfg.hidden, cfg.heads, cfg.head_dim
     m = modulation(w, vec, f"{p}.modulation", 3)
     proj = w.linear(norm_modulate(x, m[0], m[1]), f"{p}.linear1.weight", w.optional(f"{p}.linear1.bias"))
-    q, k, v = split_qkv(proj[..., : 3 * h].contiguous(), heads, hd)
-    q = rotate(qk_norm(q, w.dense_tensor(f"{p}.norm.query_norm.scale")), cos, sin)
-    k = rotate(qk_norm(k, w.dense_tensor(f"{p}.norm.key_norm.scale")), cos, sin)
+    if fused_heads:
+        q, k, v = prepare_heads(w, proj[..., : 3 * h], heads, hd, f"{p}.norm", cos, sin)
+    else:
+        q, k, v = split_qkv(proj[..., : 3 * h].contiguous(), heads, hd)
+        q = rotate(qk_norm(q, w.dense_tensor(f"{p}.norm.query_norm.scale")), cos, sin)
+        k = rotate(qk_norm(k, w.dense_tensor(f"{p}.norm.key_norm.scale")), cos, sin)
     joined = torch.cat((attention(q, k, v), F.gelu(proj[..., 3 * h:], approximate="tanh")), dim=2)
     return w.linear_fused(joined, f"{p}.linear2.weight", w.optional(f"{p}.linear2.bias"),
                           gate=m[2], residual=x)
 
 
-def forward(w, img, txt, timestep, pooled, cfg: FluxShape, rope) -> torch.Tensor:
+def forward(w, img, txt, timestep, pooled, cfg: FluxShape, rope, fused_heads: bool = False) -> torch.Tensor:
     """One transformer forward: img [1, n_img, in_channels], txt [1, n_txt, context_dim],
-    timestep [1], pooled [1, vec_dim] (bf16) -> [1, n_img, in_channels]."""
+    timestep [1], pooled [1, vec_dim] (bf16) -> [1, n_img, in_channels].  ``fused_heads`` prepares
+    the queries, keys and values of each block with one kernel a stream."""
     cos, sin = rope
     img = w.linear(img, "img_in.weight", w.optional("img_in.bias"))
     txt = w.linear(txt, "txt_in.weight", w.optional("txt_in.bias"))
     vec = mlp_embedder(w, timestep_embedding(timestep, TIME_EMBED_DIM, cfg.theta), "time_in")
     vec = vec + mlp_embedder(w, pooled, "vector_in")
     for i in range(cfg.depth):
-        img, txt = double_block(w, img, txt, vec, cos, sin, i, cfg)
+        img, txt = double_block(w, img, txt, vec, cos, sin, i, cfg, fused_heads)
     x = torch.cat((txt, img), dim=1)
     for i in range(cfg.depth_single):
-        x = single_block(w, x, vec, cos, sin, i, cfg)
+        x = single_block(w, x, vec, cos, sin, i, cfg, fused_heads)
     img = x[:, txt.shape[1]:]
     shift, scale = w.linear(F.silu(vec), "final_layer.adaLN_modulation.1.weight",
                             w.optional("final_layer.adaLN_modulation.1.bias")).reshape(1, 1, -1).chunk(2, dim=-1)

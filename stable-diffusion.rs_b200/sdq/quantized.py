@@ -8,28 +8,32 @@ the same errors, with `QuantizedArray` backed by libsdq instead of MLX.  Dense
 """
 from __future__ import annotations
 
-from typing import Callable, Dict, Mapping, Optional, Protocol
+from typing import Callable, Dict, Mapping, Optional, Protocol, Union
 
 import torch
 import torch.nn.functional as F
 
-from . import ACT_GELU_TANH, ACT_NONE, ACT_SILU, QuantizedArray, SdqError
+from . import ACT_GELU_TANH, ACT_NONE, ACT_SILU, Fp8Array, QuantizedArray, SdqError
 from ._abi import SDQ_ERR_INVALID
 
 #: MLX's default group size; must divide the weight's input width (quantized.rs:45-46).
 GROUP_SIZE = 64
 #: Bits per weight by default (quantized.rs:47-49).
 DEFAULT_BITS = 4
+#: In the place of a bit width: hold the weight as block-scaled e4m3 (:class:`sdq.Fp8Array`), whose
+#: linears also quantise their activations.  No counterpart in the reference.
+FP8 = "fp8"
 
+Bits = Union[int, str]
 Weights = Dict[str, torch.Tensor]
 
 
 class QuantizedWeights:
     """Large weights quantised, the rest dense; both consulted by name (quantized.rs:51-86)."""
 
-    def __init__(self, quantized: Optional[Dict[str, QuantizedArray]] = None,
+    def __init__(self, quantized: Optional[Dict[str, Union[QuantizedArray, Fp8Array]]] = None,
                  dense: Optional[Weights] = None):
-        self.quantized: Dict[str, QuantizedArray] = quantized or {}
+        self.quantized: Dict[str, Union[QuantizedArray, Fp8Array]] = quantized or {}
         self.dense: Weights = dense or {}
 
     def resident_bytes(self) -> int:
@@ -82,9 +86,10 @@ def indexed(name: str) -> bool:
             or name == "lm_head.weight")
 
 
-def mixed(bits: int) -> Callable[[str], int]:
-    """Default policy: indexed dense (0), sensitive 8, the rest ``bits`` (quantized.rs:156-166)."""
-    def f(name: str) -> int:
+def mixed(bits: Bits) -> Callable[[str], Bits]:
+    """Default policy: indexed dense (0), sensitive 8, the rest ``bits`` (quantized.rs:156-166),
+    which may be :data:`FP8`."""
+    def f(name: str) -> Bits:
         if indexed(name):
             return 0
         if sensitive(name):
@@ -98,36 +103,52 @@ def quantizable(shape) -> bool:
     return len(shape) == 2 and shape[1] % GROUP_SIZE == 0
 
 
-def from_dense(w: Mapping[str, torch.Tensor], bits: int) -> QuantizedWeights:
+def fp8_quantizable(shape) -> bool:
+    """2-D with rows of whole 16-byte pieces, the block-scaled form's only condition."""
+    return len(shape) == 2 and shape[0] > 0 and shape[1] > 0 and shape[1] % 16 == 0
+
+
+def quantize_to(w: torch.Tensor, bits: Bits, stream=None) -> Union[QuantizedArray, Fp8Array, None]:
+    """``w`` as a policy's ``bits`` say: affine at 4 or 8 bits, :data:`FP8`, or None for a tensor that
+    stays dense (0, or a shape that the form does not take)."""
+    if bits == FP8:
+        return Fp8Array.quantize(w.contiguous(), stream) if fp8_quantizable(tuple(w.shape)) else None
+    if bits >= 2 and quantizable(tuple(w.shape)):
+        return QuantizedArray.quantize(w.contiguous(), GROUP_SIZE, bits, stream)
+    return None
+
+
+def from_dense(w: Mapping[str, torch.Tensor], bits: Bits) -> QuantizedWeights:
     """Quantise an already-loaded dense map with the default policy (quantized.rs:265-267)."""
     return from_dense_with(w, mixed(bits))
 
 
-def from_dense_with(w: Mapping[str, torch.Tensor], bits_for: Callable[[str], int],
+def from_dense_with(w: Mapping[str, torch.Tensor], bits_for: Callable[[str], Bits],
                     stream=None) -> QuantizedWeights:
-    """``from_dense`` with an explicit per-tensor bit width; 0 keeps a tensor dense
+    """``from_dense`` with an explicit per-tensor bit width or :data:`FP8`; 0 keeps a tensor dense
     (quantized.rs:273-291).  Each weight is quantised on the device and the dense
     source may be dropped by the caller right after."""
-    quantized: Dict[str, QuantizedArray] = {}
+    quantized: Dict[str, Union[QuantizedArray, Fp8Array]] = {}
     dense: Weights = {}
     for name, array in w.items():
-        bits = bits_for(name)
-        if bits >= 2 and quantizable(tuple(array.shape)):
-            quantized[name] = QuantizedArray.quantize(array.contiguous(), GROUP_SIZE, bits, stream)
+        q = quantize_to(array, bits_for(name), stream)
+        if q is not None:
+            quantized[name] = q
         else:
             dense[name] = array.contiguous()
     return QuantizedWeights(quantized, dense)
 
 
-def from_gguf(path: str, bits: int, device=None, stream=None) -> QuantizedWeights:
+def from_gguf(path: str, bits: Bits, device=None, stream=None) -> QuantizedWeights:
     """Load a GGUF checkpoint, quantising the large weights as they are read
     (quantized.rs:180-211).  One tensor at a time: its raw block bytes are copied to the
     device and either quantised there straight from the block format (``sdq.gguf_quantize``)
-    or dequantised to a dense f32 tensor; nothing else of the file is held meanwhile."""
+    or dequantised to a dense f32 tensor, which for :data:`FP8` is then quantised; nothing else of
+    the file is held meanwhile."""
     return _load_gguf(path, bits, None, device, stream)
 
 
-def from_gguf_renamed(path: str, bits: int, rename: Callable[[str], Optional[str]], device=None,
+def from_gguf_renamed(path: str, bits: Bits, rename: Callable[[str], Optional[str]], device=None,
                       stream=None) -> QuantizedWeights:
     """``from_gguf`` with file names translated by ``rename`` (None drops a tensor),
     quantized.rs:221-255."""
@@ -140,7 +161,7 @@ def _load_gguf(path, bits, rename, device, stream) -> QuantizedWeights:
 
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     g = G.Gguf(path)
-    quantized: Dict[str, QuantizedArray] = {}
+    quantized: Dict[str, Union[QuantizedArray, Fp8Array]] = {}
     dense: Weights = {}
     policy = mixed(bits)
     for info in g.tensors:
@@ -149,7 +170,15 @@ def _load_gguf(path, bits, rename, device, stream) -> QuantizedWeights:
             continue
         raw = torch.from_numpy(g.raw(info)).to(dev)         # the peak: one tensor's blocks
         want = policy(name)
-        if want >= 2 and quantizable(info.shape):
+        if want == FP8:
+            array = gguf_dequantize(raw, info.kind, info.shape, torch.float32, stream)
+            q = quantize_to(array, FP8, stream)
+            if q is not None:
+                quantized[name] = q
+            else:
+                dense[name] = array
+            del array
+        elif want >= 2 and quantizable(info.shape):
             n, k = info.shape
             wq, s, b = gguf_quantize(raw, info.kind, n, k, want, GROUP_SIZE, stream)
             quantized[name] = QuantizedArray(wq, s, b, GROUP_SIZE, want)
