@@ -57,6 +57,10 @@ struct Sixteen<false> {
     __device__ float get(int i) const { return __uint_as_float(w[i]); }
 };
 
+// Fours of rows that a warp of fp8_quantize_rows takes.
+template <bool BF16>
+__host__ __device__ constexpr int row_quads() { return BF16 ? 2 : 1; }
+
 template <class V>
 __device__ __forceinline__ uint32_t largest(const V& v) {
     uint32_t m = 0;
@@ -75,29 +79,39 @@ __device__ __forceinline__ uint4 encode(const V& v, float inv) {
 }
 
 // Activations: eight lanes take the 128 values of one group, a warp the same group of four
-// consecutive rows, so that the four scale bytes, which lie [group, row], share a sector.
+// consecutive rows, so that the four scale bytes, which lie [group, row], share a sector; of bf16
+// it takes eight rows, for as many bytes under way as of f32.  4608 x 12288 bf16: 27.2 us (6.3 TB/s),
+// four rows 28.6, sixteen 29.5; f32 42.3 us (6.7 TB/s).
 template <bool BF16>
 __global__ void __launch_bounds__(256) fp8_quantize_rows(const void* __restrict__ x, int64_t m, int64_t k,
                                                          uint8_t* __restrict__ q, uint8_t* __restrict__ scales) {
+    constexpr int NQ = row_quads<BF16>();
     const int lane = threadIdx.x & 31;
-    const int64_t kb = (k + kFp8Block - 1) / kFp8Block;
-    const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t quad = u / kb, g = u - quad * kb;
-    const int64_t row = 4 * quad + (lane >> 3);
+    const uint32_t kb = (uint32_t)((k + kFp8Block - 1) / kFp8Block);
+    const uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 5);      // below 2^32: m <= 2^30, and memory's size
+    const uint32_t part = u / kb, g = u - part * kb;
+    const int64_t row0 = (int64_t)4 * NQ * part + (lane >> 3);
     const int64_t c = g * kFp8Block + 16 * (lane & 7);
-    const bool in = row < m && c < k;
-    Sixteen<BF16> v;
-    v.zero();
-    if (in) v.load(x, row * k + c);
-    uint32_t a = largest(v);
+    Sixteen<BF16> v[NQ];
 #pragma unroll
-    for (int d = 1; d < 8; d <<= 1) a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, d));
-    const uint32_t byte = e8m0_of(a);
-    if (in) *reinterpret_cast<uint4*>(q + row * k + c) = encode(v, e8m0_inverse(byte));
-    if ((lane & 7) == 0 && row < m) scales[g * m + row] = (uint8_t)byte;
+    for (int i = 0; i < NQ; ++i) {
+        v[i].zero();
+        if (row0 + 4 * i < m && c < k) v[i].load(x, (row0 + 4 * i) * k + c);
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        const int64_t row = row0 + 4 * i;
+        uint32_t a = largest(v[i]);
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, d));
+        const uint32_t byte = e8m0_of(a);
+        if (row < m && c < k) *reinterpret_cast<uint4*>(q + row * k + c) = encode(v[i], e8m0_inverse(byte));
+        if ((lane & 7) == 0 && row < m) scales[g * m + row] = (uint8_t)byte;
+    }
 }
 
-// Weights: one CTA per 128 x 128 block, four rows of 16 values per thread.
+// Weights: one CTA per 128 x 128 block, four rows of 16 values per thread.  32768 x 5120 bf16: 74 us
+// (6.8 TB/s).
 template <bool BF16>
 __global__ void __launch_bounds__(256) fp8_quantize_blocks(const void* __restrict__ w, int64_t n, int64_t k,
                                                            uint8_t* __restrict__ q, uint8_t* __restrict__ scales) {
@@ -171,7 +185,8 @@ __global__ void __launch_bounds__(256) fp8_dequantize_kernel(const uint8_t* __re
 
 cudaError_t launch_fp8_quantize(const void* x, bool bf16, int64_t m, int64_t k, uint8_t* q, uint8_t* scales,
                                 cudaStream_t st) {
-    const int64_t kb = (k + kFp8Block - 1) / kFp8Block, warps = (m + 3) / 4 * kb;
+    const int64_t kb = (k + kFp8Block - 1) / kFp8Block, rows = 4 * (bf16 ? row_quads<true>() : row_quads<false>());
+    const int64_t warps = (m + rows - 1) / rows * kb;
     const unsigned grid = (unsigned)((warps + 7) / 8);
     if (bf16) fp8_quantize_rows<true><<<grid, 256, 0, st>>>(x, m, k, q, scales);
     else fp8_quantize_rows<false><<<grid, 256, 0, st>>>(x, m, k, q, scales);
