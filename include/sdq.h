@@ -209,7 +209,8 @@ int sdq_fp8_dequantize(const uint8_t* q, const uint8_t* scales, int64_t rows, in
  * xq / x_scales and wq / w_scales stand for; products and sums in f32, one rounding to y_dtype.
  * bias, gate, residual may be NULL (0, 1, 0); act is one of SDQ_ACT_*.  With y bf16, bias and gate
  * are [n] bf16 and residual [m,n] bf16 (residual may be y itself, but not otherwise overlap it).
- * With y f32 only a bias ([n] f32) may be given.  m may be 0.  xq and wq are 16-byte aligned.
+ * With y f32 only a bias ([n] f32) may be given.  y overlaps no other input.  m may be 0.  xq and wq
+ * are 16-byte aligned.  All sizes run one kernel (block-scaled tcgen05 MMAs, alone or in CTA pairs).
  */
 int sdq_fp8_matmul(const uint8_t* xq, const uint8_t* x_scales, int64_t m, int64_t k, const uint8_t* wq,
                    const uint8_t* w_scales, int64_t n, const void* bias, int act, const void* gate,

@@ -15,6 +15,7 @@
 #include "sdq_dequant.cuh"
 #include "sdq_fp8.cuh"
 #include "sdq_internal.h"
+#include "sdq_ptx.cuh"
 
 namespace sdq {
 namespace {
@@ -93,6 +94,8 @@ __global__ void __launch_bounds__(256) fp8_quantize_rows(const void* __restrict_
     const int64_t row0 = (int64_t)4 * NQ * part + (lane >> 3);
     const int64_t c = g * kFp8Block + 16 * (lane & 7);
     Sixteen<BF16> v[NQ];
+    griddep_wait();
+    griddep_launch_dependents();
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
         v[i].zero();
@@ -188,9 +191,8 @@ cudaError_t launch_fp8_quantize(const void* x, bool bf16, int64_t m, int64_t k, 
     const int64_t kb = (k + kFp8Block - 1) / kFp8Block, rows = 4 * (bf16 ? row_quads<true>() : row_quads<false>());
     const int64_t warps = (m + rows - 1) / rows * kb;
     const unsigned grid = (unsigned)((warps + 7) / 8);
-    if (bf16) fp8_quantize_rows<true><<<grid, 256, 0, st>>>(x, m, k, q, scales);
-    else fp8_quantize_rows<false><<<grid, 256, 0, st>>>(x, m, k, q, scales);
-    return cudaGetLastError();
+    return launch_programmatic(bf16 ? fp8_quantize_rows<true> : fp8_quantize_rows<false>, dim3(grid), 256, 0, st, x, m, k, q,
+                               scales);
 }
 
 cudaError_t launch_fp8_quantize_weight(const void* w, bool bf16, int64_t n, int64_t k, uint8_t* q,

@@ -89,6 +89,24 @@ cudaError_t launch_qmv(const void* x, bool x_f32, int64_t m, int64_t k, const ui
                        const EpiArgs& epi, void* y, bool y_f32, cudaStream_t st, const char** msg,
                        bool* taken);
 
+// Launch with programmatic stream serialisation: the kernel may start while the one before it in the
+// stream finishes, and waits for it (griddep_wait) before it touches global memory.
+template <class... Params, class... Args>
+cudaError_t launch_programmatic(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st,
+                                Args&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // Block-scaled e4m3 (sdq_fp8.cuh): activations in row groups of 128 (scales [ceil(k/128), m]),
 // weights in 128 x 128 blocks (scales [ceil(n/128), ceil(k/128)]), and back (sdq_fp8_quant.cu).
 cudaError_t launch_fp8_quantize(const void* x, bool bf16, int64_t m, int64_t k, uint8_t* q, uint8_t* scales,

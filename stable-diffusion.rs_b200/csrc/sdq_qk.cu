@@ -27,6 +27,7 @@
 #include <cuda_runtime.h>
 
 #include "sdq_internal.h"
+#include "sdq_ptx.cuh"
 
 namespace sdq {
 namespace {
@@ -112,6 +113,8 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
     int64_t to = b * y.batch_stride + t * y.token_stride + h0 * y.head_stride + e;
 
     Raw<BF16> v[kBatch];
+    griddep_wait();
+    griddep_launch_dependents();
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
         if (j * kSide < count) {
@@ -226,8 +229,7 @@ cudaError_t go(const QkArgs& a, cudaStream_t st) {
     const unsigned blocks = (unsigned)((a.batch * a.tokens + kWarps - 1) / kWarps);
     unsigned pieces = 0;
     for (int h : a.heads) pieces += (unsigned)((h + kBatch * kSide - 1) / (kBatch * kSide));
-    qk_kernel<BF16, INTER, LPV><<<dim3(blocks, pieces), 32 * kWarps, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch_programmatic(qk_kernel<BF16, INTER, LPV>, dim3(blocks, pieces), 32 * kWarps, 0, st, a);
 }
 
 template <bool BF16, bool INTER>

@@ -225,6 +225,43 @@ def test_same_call_same_bits(m):
         assert torch.equal(sdq.fp8_matmul(*ops), a)
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 values in x and in y: the last rows of each."""
+    m, k = 131136, 16400
+    x = torch.zeros(m, k, device="cuda", dtype=torch.bfloat16)
+    x[-3:] = spread(1, 3, k).to(torch.bfloat16)
+    q, s = sdq.fp8_quantize(x)
+    wq, ws = O.fp8_quantize(x[-3:].double().cpu().numpy())
+    assert np.array_equal(u8(q[-3:]), wq) and np.array_equal(u8(s[:, -3:].contiguous()), ws)
+    assert not q[:1000].view(torch.uint8).any()
+    del x, q, s
+    m, k, n = 65600, 16, 32784
+    ops = operands(2, m, k, n)
+    y = sdq.fp8_matmul(*ops)
+    assert y.numel() > 2 ** 31
+    for rows in (slice(0, 2), slice(m - 3, m)):
+        want, tot = product(ops[0][rows], ops[1][:, rows], *ops[2:])
+        check(y[rows], want, want.abs() * 2.0 ** -8 + sums_tol(tot, k))
+    sdq.device_status()
+
+
+def test_two_streams_at_once():
+    """Products of different shapes, quantisers and heads in flight together; each has its own result."""
+    shapes = [(7, 512, 3000), (300, 1024, 2000), (1000, 512, 999)]
+    ops = [operands(30 + i, *s) for i, s in enumerate(shapes)]
+    want = [sdq.fp8_matmul(*o) for o in ops]
+    streams = [torch.cuda.Stream() for _ in shapes]
+    torch.cuda.synchronize()
+    got = [[] for _ in shapes]
+    for _ in range(10):
+        for g, o, st in zip(got, ops, streams):
+            g.append(sdq.fp8_matmul(*o, stream=st))
+    torch.cuda.synchronize()
+    sdq.device_status()
+    for g, w in zip(got, want):
+        assert all(torch.equal(y, w) for y in g)
+
+
 def test_empty_batch():
     wq, ws = sdq.fp8_quantize_weight(normals(1, 64, 128))
     x = torch.empty(0, 128, device="cuda", dtype=torch.bfloat16)
