@@ -7,6 +7,9 @@ Each ``csrc/*.cu`` is compiled separately (no relocatable device code: every
 ``stable-diffusion.rs_b200/libsdq.so`` next to this script, where the built
 library travels with the source tree.  The CUDA runtime is linked statically,
 so the library's only dynamic dependencies are libc / libstdc++ and NCCL.
+
+``binding/sdq_native.cpp`` becomes ``sdq/_native.so``, the package's C++ shortcut for ordinary calls
+(against the installed torch's headers; it calls libsdq through addresses it is given).
 """
 from __future__ import annotations
 
@@ -21,6 +24,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libsdq.so")
+NATIVE_SRC = os.path.join(HERE, "binding", "sdq_native.cpp")
+NATIVE = os.path.join(HERE, "sdq", "_native.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -67,6 +72,24 @@ def stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def build_native(force: bool = False, verbose: bool = False) -> str:
+    if force or stale(NATIVE, [NATIVE_SRC, os.path.join(ROOT, "include", "sdq.h")]):
+        import sysconfig
+
+        import torch
+
+        base = os.path.join(os.path.dirname(torch.__file__))
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-I", os.path.join(ROOT, "include"),
+               "-I", os.path.join(base, "include"), "-I", os.path.join(base, "include", "torch", "csrc", "api", "include"),
+               "-I", sysconfig.get_paths()["include"], "-I", os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"),
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", NATIVE_SRC, "-o", NATIVE,
+               "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+    return NATIVE
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     cc = nvcc()
@@ -92,6 +115,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+    build_native(force, verbose)
     return LIB
 
 

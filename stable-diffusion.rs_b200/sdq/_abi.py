@@ -10,6 +10,13 @@ from __future__ import annotations
 import ctypes
 import os
 
+import torch  # noqa: F401  (the shortcut below links against its libraries)
+
+try:
+    from . import _native
+except ImportError:
+    _native = None
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SDQ_LIB", os.path.join(os.path.dirname(HERE), "libsdq.so"))
 
@@ -92,7 +99,16 @@ def lib() -> ctypes.CDLL:
             f.restype = res
             f.argtypes = args
         _lib = L
+        if _native is not None:
+            _native.bind(*(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in (
+                "sdq_fp8_quantize", "sdq_fp8_quantize_weight", "sdq_fp8_matmul", "sdq_qk_norm_rope")))
     return _lib
+
+
+def native(name: str):
+    """The C++ shortcut of an entry point (binding/sdq_native.cpp): it returns None, having done
+    nothing, unless the call is an ordinary one.  Where it was not built, ctypes makes every call."""
+    return getattr(_native, name) if _native is not None else lambda *args: None
 
 
 def last_error() -> str:

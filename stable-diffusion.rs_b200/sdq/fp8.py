@@ -18,7 +18,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _ACTS
-from ._abi import SDQ_BF16, SDQ_ERR_INVALID, SDQ_ERR_UNSUPPORTED, SDQ_F32, SdqError, check, lib
+from ._abi import SDQ_BF16, SDQ_ERR_INVALID, SDQ_ERR_UNSUPPORTED, SDQ_F32, SdqError, check, lib, native
 
 #: Values that share a scale, along a row (activations) or both ways (weights).
 BLOCK = 128
@@ -30,13 +30,7 @@ _current_device = torch.cuda.current_device
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
-
-try:
-    # torch's allocation without the dispatcher, on the current device: 0.8 us against 1.4 to 2.
-    from torch._C._dynamo.guards import _empty_strided_cuda as _empty_strided
-except ImportError:
-    def _empty_strided(size, stride, dtype):
-        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+_quantize, _quantize_weight, _matmul = native("fp8_quantize"), native("fp8_quantize_weight"), native("fp8_matmul")
 
 
 def _elsewhere(fn, device, stream, *args, **kw):
@@ -54,10 +48,9 @@ def _elsewhere(fn, device, stream, *args, **kw):
         return fn(*args, **kw)
 
 
-def _refuse(name: str, first: torch.Tensor, expected) -> None:
+def _demand(name: str, first: torch.Tensor, expected) -> None:
     """Raise for the first of ``expected`` -- (name, tensor, dtypes, shape or count) -- that is not a
-    contiguous tensor like that on ``first``'s device.  The entry points test all of it in one
-    expression, which costs a call of a few microseconds less, and come here when that fails."""
+    contiguous tensor like that on ``first``'s device."""
     if not first.is_cuda:
         raise SdqError(SDQ_ERR_INVALID, "libsdq takes device tensors (no CPU fallback)")
     for n, t, dtypes, shape in expected:
@@ -73,7 +66,6 @@ def _refuse(name: str, first: torch.Tensor, expected) -> None:
             raise SdqError(SDQ_ERR_UNSUPPORTED, f"{n} must be {' or '.join(_NAMES.get(d, str(d)) for d in dtypes)}, not {t.dtype}")
         if isinstance(shape, tuple) and tuple(t.shape) != shape:
             raise SdqError(SDQ_ERR_INVALID, f"{n} must have shape {list(shape)}, not {list(t.shape)}")
-    raise SdqError(SDQ_ERR_INVALID, f"invalid arguments beside {name}")
 
 
 def _rows(x: torch.Tensor, name: str):
@@ -87,37 +79,38 @@ def _rows(x: torch.Tensor, name: str):
 def fp8_quantize(x: torch.Tensor, stream=None):
     """Activations x [..., k] (bf16 or f32) -> (xq [..., k] e4m3, xs [ceil(k / 128), rows] e8m0),
     rows the product of the leading axes (``sdq_fp8_quantize``).  k is a multiple of 16."""
+    if stream is None:
+        done = _quantize(x)
+        if done is not None:
+            return done
     dev = x.get_device()
     if stream is not None or dev < 0 or dev != _current_device():
         return _elsewhere(fp8_quantize, x.device, stream, x)
-    dt = _SOURCE.get(x.dtype)
-    if dt is None or not x.is_contiguous():
-        _refuse("x", x, [("x", x, tuple(_SOURCE), None)])
+    _demand("x", x, [("x", x, tuple(_SOURCE), None)])
     m, k = _rows(x, "x")
-    xq = _empty_strided((m, k), (k, 1), E4M3)
-    if x.dim() != 2:
-        xq = xq.view(x.shape)
-    xs = _empty_strided((-(-k // BLOCK), m), (m, 1), E8M0)
-    check(lib().sdq_fp8_quantize(x.data_ptr(), dt, m, k, xq.data_ptr(), xs.data_ptr(), _raw_stream(dev)))
+    xq = torch.empty_like(x, dtype=E4M3)
+    xs = x.new_empty((-(-k // BLOCK), m), dtype=E8M0)
+    check(lib().sdq_fp8_quantize(x.data_ptr(), _SOURCE[x.dtype], m, k, xq.data_ptr(), xs.data_ptr(), _raw_stream(dev)))
     return xq, xs
 
 
 def fp8_quantize_weight(w: torch.Tensor, stream=None):
     """A weight w [n, k] (bf16 or f32) -> (wq [n, k] e4m3, ws [ceil(n / 128), ceil(k / 128)] e8m0)
     (``sdq_fp8_quantize_weight``).  k is a multiple of 16."""
+    if stream is None:
+        done = _quantize_weight(w)
+        if done is not None:
+            return done
     dev = w.get_device()
     if stream is not None or dev < 0 or dev != _current_device():
         return _elsewhere(fp8_quantize_weight, w.device, stream, w)
-    dt = _SOURCE.get(w.dtype)
-    if dt is None or not w.is_contiguous():
-        _refuse("w", w, [("w", w, tuple(_SOURCE), None)])
+    _demand("w", w, [("w", w, tuple(_SOURCE), None)])
     if w.dim() != 2:
         raise SdqError(SDQ_ERR_INVALID, f"fp8_quantize_weight wants a 2-D weight, got shape {list(w.shape)}")
     n, k = w.shape
-    kb = -(-k // BLOCK)
-    wq = _empty_strided((n, k), (k, 1), E4M3)
-    ws = _empty_strided((-(-n // BLOCK), kb), (kb, 1), E8M0)
-    check(lib().sdq_fp8_quantize_weight(w.data_ptr(), dt, n, k, wq.data_ptr(), ws.data_ptr(), _raw_stream(dev)))
+    wq = torch.empty_like(w, dtype=E4M3)
+    ws = w.new_empty((-(-n // BLOCK), -(-k // BLOCK)), dtype=E8M0)
+    check(lib().sdq_fp8_quantize_weight(w.data_ptr(), _SOURCE[w.dtype], n, k, wq.data_ptr(), ws.data_ptr(), _raw_stream(dev)))
     return wq, ws
 
 
@@ -129,20 +122,13 @@ def fp8_dequantize(q: torch.Tensor, scales: torch.Tensor, weight: bool, out_dtyp
         return _elsewhere(fp8_dequantize, q.device, stream, q, scales, weight, out_dtype)
     rows, k = _rows(q, "q")
     kb = -(-k // BLOCK)
-    shape = (-(-rows // BLOCK), kb) if weight else (kb, rows)
-    if not (q.dtype is E4M3 and scales.dtype is E8M0 and scales.shape == shape and scales.get_device() == dev
-            and q.is_contiguous() and scales.is_contiguous()):
-        _refuse("q", q, [("q", q, (E4M3,), None), ("scales", scales, (E8M0,), shape)])
+    _demand("q", q, [("q", q, (E4M3,), None), ("scales", scales, (E8M0,), (-(-rows // BLOCK), kb) if weight else (kb, rows))])
     if out_dtype not in _SOURCE:
         raise SdqError(SDQ_ERR_UNSUPPORTED, f"out must be bf16 or f32, not {out_dtype}")
     out = torch.empty_like(q, dtype=out_dtype)
     check(lib().sdq_fp8_dequantize(q.data_ptr(), scales.data_ptr(), rows, k, int(bool(weight)), out.data_ptr(),
                                    _SOURCE[out_dtype], _raw_stream(dev)))
     return out
-
-
-def _like(t, dev: int, dtype, count: int) -> bool:
-    return t.dtype is dtype and t.numel() == count and t.get_device() == dev and t.is_contiguous()
 
 
 def fp8_matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias=None, act=None,
@@ -152,44 +138,32 @@ def fp8_matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.T
 
     ``act`` is None, ``"gelu_approx"`` or ``"silu"``; ``bias`` and ``gate`` hold n values, ``residual``
     has the result's shape and may be ``out`` itself."""
+    if stream is None:
+        done = _matmul(xq, xs, wq, ws, bias, act, gate, residual, out, out_dtype)
+        if done is not None:
+            return done
     dev = xq.get_device()
     if stream is not None or dev < 0 or dev != _current_device():
         return _elsewhere(fp8_matmul, xq.device, stream, xq, xs, wq, ws, bias, act, gate, residual, out, out_dtype)
-    code = _ACTS.get(act)
-    if code is None:
+    if act not in _ACTS:
         raise SdqError(SDQ_ERR_INVALID, f"unknown activation {act!r}")
     m, k = _rows(xq, "xq")
     if wq.dim() != 2:
         raise SdqError(SDQ_ERR_INVALID, f"wq must be 2-D, got shape {list(wq.shape)}")
-    n, wk = wq.shape
-    kb = -(-k // BLOCK)
-    nb = -(-n // BLOCK)
+    n, kb = wq.shape[0], -(-k // BLOCK)
+    shape = (*xq.shape[:-1], n)
+    dtype = out_dtype if out_dtype is not None else torch.bfloat16 if out is None else out.dtype
+    if dtype not in _SOURCE:
+        raise SdqError(SDQ_ERR_UNSUPPORTED, f"out must be bf16 or f32, not {dtype}")
+    _demand("xq", xq, [
+        ("xq", xq, (E4M3,), None), ("xs", xs, (E8M0,), (kb, m)), ("wq", wq, (E4M3,), (n, k)), ("ws", ws, (E8M0,), (-(-n // BLOCK), kb)),
+        ("out", out, (dtype,), shape), ("bias", bias, (dtype,), n), ("gate", gate, (dtype,), n), ("residual", residual, (dtype,), m * n)])
     if out is None:
-        dtype = torch.bfloat16 if out_dtype is None else out_dtype
-    else:
-        dtype = out.dtype
-    dt = _SOURCE.get(dtype)
-    if not (dt is not None and xq.dtype is E4M3 and wq.dtype is E4M3 and xs.dtype is E8M0 and ws.dtype is E8M0 and wk == k
-            and xs.shape == (kb, m) and ws.shape == (nb, kb) and wq.get_device() == xs.get_device() == ws.get_device() == dev
-            and xq.is_contiguous() and wq.is_contiguous() and xs.is_contiguous() and ws.is_contiguous()
-            and (bias is None or _like(bias, dev, dtype, n)) and (gate is None or _like(gate, dev, dtype, n))
-            and (residual is None or _like(residual, dev, dtype, m * n))
-            and (out is None or (_like(out, dev, dtype if out_dtype is None else out_dtype, m * n)
-                                 and out.shape == (*xq.shape[:-1], n)))):
-        if dt is None:
-            raise SdqError(SDQ_ERR_UNSUPPORTED, f"out must be bf16 or f32, not {dtype}")
-        _refuse("xq", xq, [
-            ("xq", xq, (E4M3,), None), ("xs", xs, (E8M0,), (kb, m)), ("wq", wq, (E4M3,), (n, k)), ("ws", ws, (E8M0,), (nb, kb)),
-            ("out", out, (dtype if out_dtype is None else out_dtype,), (*xq.shape[:-1], n)), ("bias", bias, (dtype,), n),
-            ("gate", gate, (dtype,), n), ("residual", residual, (dtype,), m * n)])
-    if out is None:
-        out = _empty_strided((m, n), (n, 1), dtype)
-        if xq.dim() != 2:
-            out = out.view((*xq.shape[:-1], n))
+        out = xq.new_empty(shape, dtype=dtype)
     check(lib().sdq_fp8_matmul(xq.data_ptr(), xs.data_ptr(), m, k, wq.data_ptr(), ws.data_ptr(), n,
-                               None if bias is None else bias.data_ptr(), code,
+                               None if bias is None else bias.data_ptr(), _ACTS[act],
                                None if gate is None else gate.data_ptr(),
-                               None if residual is None else residual.data_ptr(), out.data_ptr(), dt, _raw_stream(dev)))
+                               None if residual is None else residual.data_ptr(), out.data_ptr(), _SOURCE[dtype], _raw_stream(dev)))
     return out
 
 

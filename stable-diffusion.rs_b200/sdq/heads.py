@@ -2,44 +2,23 @@
 from __future__ import annotations
 
 import ctypes
-from array import array
 
 import torch
 
-from ._abi import SDQ_ERR_INVALID, SDQ_ERR_UNSUPPORTED, SdqError, SdqHeads, check, lib
-from .fp8 import _SOURCE, _current_device, _elsewhere, _empty_strided, _like, _raw_stream
+from ._abi import SDQ_ERR_INVALID, SDQ_ERR_UNSUPPORTED, SdqError, SdqHeads, check, lib, native
+from .fp8 import _SOURCE, _current_device, _elsewhere, _raw_stream
 
 _PAIRS = {"interleaved": 1, "halves": 0}
-_WIDE = {torch.int32: 0, torch.int64: 1}
-_HEADS = ctypes.sizeof(SdqHeads)               # five 64-bit fields
+_heads = native("qk_norm_rope")
 
 
-def _refuse(dev: int, dtype, b: int, n: int, d: int, tensors, weights, cos, sin, positions) -> None:
-    """Raise for the first argument that is not what the call needs (the caller has seen that one is)."""
-    for name, t, o in tensors:
-        if t.dim() != 4 or t.shape[0] != b or t.shape[1] != n or t.shape[3] != d:
-            raise SdqError(SDQ_ERR_INVALID, f"{name} must be [{b}, {n}, heads, {d}], got shape {list(t.shape)}")
-        if o is not None and tuple(o.shape) != (b, t.shape[2], n, d):
-            raise SdqError(SDQ_ERR_INVALID, f"{name}'s output must be {[b, t.shape[2], n, d]}, got shape {list(o.shape)}")
-        for x in (t, t if o is None else o):
-            if x.dtype is not dtype or x.get_device() != dev:
-                raise SdqError(SDQ_ERR_INVALID, f"{name} and its output must be {dtype} on cuda:{dev}, not {x.dtype} on {x.device}")
-            if x.stride(3) != 1:
-                raise SdqError(SDQ_ERR_INVALID, f"{name} and its output must have a contiguous last axis")
-    for name, w in weights:
-        if w is not None and not _like(w, dev, dtype, d):
-            raise SdqError(SDQ_ERR_INVALID, f"{name} must hold {d} contiguous values of {dtype} on cuda:{dev}")
-    if (cos is None) != (sin is None):
-        raise SdqError(SDQ_ERR_INVALID, "cos and sin come together")
-    if cos is not None:
-        for name, t in (("cos", cos), ("sin", sin)):
-            if t.dim() != 2 or t.shape != cos.shape or not _like(t, dev, torch.float32, cos.numel()):
-                raise SdqError(SDQ_ERR_INVALID, f"{name} must be a contiguous f32 [positions, rope / 2] on cuda:{dev}")
-    if positions is not None:
-        if cos is None:
-            raise SdqError(SDQ_ERR_INVALID, "positions without cos and sin")
-        raise SdqError(SDQ_ERR_INVALID, f"positions must be int32 or int64 [{b}, {n}] on cuda:{dev}, contiguous along the tokens")
-    raise SdqError(SDQ_ERR_INVALID, "invalid arguments")
+def _like(t, dev: int, dtype, count: int) -> bool:
+    return t.dtype is dtype and t.numel() == count and t.get_device() == dev and t.is_contiguous()
+
+
+def _struct(t: torch.Tensor, tokens_axis: int):
+    st = t.stride()
+    return ctypes.byref(SdqHeads(t.data_ptr(), t.shape[3 - tokens_axis], st[0], st[tokens_axis], st[3 - tokens_axis]))
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
@@ -56,68 +35,61 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None
     (i, i + rope / 2); values from rope on stay.  ``out`` gives the three results' places, views
     [b, heads, n, d] of any strides with a contiguous last axis, for instance parts of a joint sequence.
     An output may be its input's own memory (with the same strides), and must not overlap otherwise."""
+    if stream is None:
+        done = _heads(q, k, v, q_weight, k_weight, cos, sin, eps, positions, pairs, out)
+        if done is not None:
+            return done
     dev = q.get_device()
     if stream is not None or dev < 0 or dev != _current_device():
         return _elsewhere(qk_norm_rope, q.device, stream, q, k, v, q_weight, k_weight, cos, sin, eps, positions, pairs, out)
-    turn = _PAIRS.get(pairs)
-    if turn is None:
+    if pairs not in _PAIRS:
         raise SdqError(SDQ_ERR_INVALID, f"pairs must be 'interleaved' or 'halves', not {pairs!r}")
     dtype = q.dtype
-    dt = _SOURCE.get(dtype)
-    if dt is None:
+    if dtype not in _SOURCE:
         raise SdqError(SDQ_ERR_UNSUPPORTED, f"q must be bf16 or f32, not {dtype}")
     if q.dim() != 4:
         raise SdqError(SDQ_ERR_INVALID, f"q must be [batch, tokens, heads, head_dim], got shape {list(q.shape)}")
     b, n, _, d = q.shape
     srcs = (q, k) if v is None else (q, k, v)
-    good, table, outs = True, array("q"), out
     if out is not None:
-        outs = [t for t in out if t is not None]
+        outs = tuple(t for t in out if t is not None)
         if len(outs) != len(srcs):
             raise SdqError(SDQ_ERR_INVALID, f"out must hold {len(srcs)} tensors, got {len(outs)}")
     else:
-        outs = []
-    for i, t in enumerate(srcs):
-        if t.dim() != 4:
-            good = False
-            break
-        tb, tn, h, td = t.shape
-        if not (tb == b and tn == n and td == d and t.dtype is dtype and t.get_device() == dev):
-            good = False
-            break
-        s0, s1, s2, s3 = t.stride()
-        if out is None:
-            o, o0, o1, o2 = _empty_strided((b, h, n, d), (h * n * d, n * d, d, 1), dtype), h * n * d, n * d, d
-            outs.append(o)
-        else:
-            o = outs[i]
-            if not (o.shape == (b, h, n, d) and o.dtype is dtype and o.get_device() == dev):
-                good = False
-                break
-            o0, o1, o2, o3 = o.stride()
-            good = good and o3 == 1
-        good = good and s3 == 1
-        table.extend((t.data_ptr(), h, s0, s1, s2, o.data_ptr(), h, o0, o2, o1))
-    rows = rope = wide = stride = cp = sp = pp = 0
-    if good and cos is not None and sin is not None and cos.dim() == 2 and sin.shape == cos.shape:
-        rows, rope = cos.shape
-        good = _like(cos, dev, torch.float32, rows * rope) and _like(sin, dev, torch.float32, rows * rope)
-        rope, cp, sp = 2 * rope, cos.data_ptr(), sin.data_ptr()
-    elif cos is not None or sin is not None:
-        good = False
+        outs = tuple(t.new_empty((b, t.shape[2], n, d)) if t.dim() == 4 else t for t in srcs)
+    for name, t, o in zip("qkv", srcs, outs):
+        if t.dim() != 4 or t.shape[0] != b or t.shape[1] != n or t.shape[3] != d:
+            raise SdqError(SDQ_ERR_INVALID, f"{name} must be [{b}, {n}, heads, {d}], got shape {list(t.shape)}")
+        if tuple(o.shape) != (b, t.shape[2], n, d):
+            raise SdqError(SDQ_ERR_INVALID, f"{name}'s output must be {[b, t.shape[2], n, d]}, got shape {list(o.shape)}")
+        for x in (t, o):
+            if x.dtype is not dtype or x.get_device() != dev:
+                raise SdqError(SDQ_ERR_INVALID, f"{name} and its output must be {dtype} on cuda:{dev}, not {x.dtype} on {x.device}")
+            if x.stride(3) != 1:
+                raise SdqError(SDQ_ERR_INVALID, f"{name} and its output must have a contiguous last axis")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and not _like(w, dev, dtype, d):
+            raise SdqError(SDQ_ERR_INVALID, f"{name} must hold {d} contiguous values of {dtype} on cuda:{dev}")
+    if (cos is None) != (sin is None):
+        raise SdqError(SDQ_ERR_INVALID, "cos and sin come together")
+    rows = rope = wide = stride = 0
+    if cos is not None:
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dim() != 2 or t.shape != cos.shape or not _like(t, dev, torch.float32, cos.numel()):
+                raise SdqError(SDQ_ERR_INVALID, f"{name} must be a contiguous f32 [positions, rope / 2] on cuda:{dev}")
+        rows, rope = cos.shape[0], 2 * cos.shape[1]
     if positions is not None:
-        wide = _WIDE.get(positions.dtype)
-        good = good and cos is not None and wide is not None and positions.shape == (b, n) and positions.get_device() == dev
-        if good:
-            stride, step = positions.stride()
-            good = step == 1 or n == 1
-            pp = positions.data_ptr()
-    if not (good and (q_weight is None or _like(q_weight, dev, dtype, d)) and (k_weight is None or _like(k_weight, dev, dtype, d))):
-        _refuse(dev, dtype, b, n, d, [(*x, outs[i] if out is not None else None) for i, x in enumerate(zip("qkv", srcs))], (("q_weight", q_weight), ("k_weight", k_weight)), cos, sin,
-                positions)
-    at = table.buffer_info()[0]                    # sdq_heads: input and output of q, of k, of v
+        if cos is None:
+            raise SdqError(SDQ_ERR_INVALID, "positions without cos and sin")
+        if tuple(positions.shape) != (b, n) or positions.get_device() != dev or positions.dtype not in (torch.int32, torch.int64) \
+                or (n > 1 and positions.stride(1) != 1):
+            raise SdqError(SDQ_ERR_INVALID, f"positions must be int32 or int64 [{b}, {n}] on cuda:{dev}, contiguous along the tokens")
+        wide, stride = int(positions.dtype is torch.int64), positions.stride(0)
+    i = [_struct(t, 1) for t in srcs] + [None]
+    o = [_struct(t, 2) for t in outs] + [None]
     check(lib().sdq_qk_norm_rope(
-        at, at + 2 * _HEADS, None if v is None else at + 4 * _HEADS, at + _HEADS, at + 3 * _HEADS,
-        None if v is None else at + 5 * _HEADS, dt, b, n, d, None if q_weight is None else q_weight.data_ptr(),
-        None if k_weight is None else k_weight.data_ptr(), eps, cp, sp, rows, rope, turn, pp, wide, stride, _raw_stream(dev)))
-    return (*outs, None) if v is None else tuple(outs)
+        i[0], i[1], i[2], o[0], o[1], o[2], _SOURCE[dtype], b, n, d, None if q_weight is None else q_weight.data_ptr(),
+        None if k_weight is None else k_weight.data_ptr(), eps, None if cos is None else cos.data_ptr(),
+        None if sin is None else sin.data_ptr(), rows, rope, _PAIRS[pairs],
+        None if positions is None else positions.data_ptr(), wide, stride, _raw_stream(dev)))
+    return (*outs, None) if v is None else outs

@@ -317,6 +317,27 @@ def test_another_stream_and_a_captured_graph():
     sdq.device_status()
 
 
+@pytest.mark.parametrize("m", [3, 200])
+def test_the_shortcut_and_ctypes_make_the_same_calls(m, monkeypatch):
+    """An ordinary call goes through the C++ shortcut, any other through ctypes: the same results."""
+    from sdq import _abi, fp8
+
+    assert _abi._native is not None, "binding/sdq_native.cpp was not built"
+    x, w = spread(1, m, 272), spread(2, 130, 272)
+    bias, gate, res = (normals(3 + i, *shape).to(torch.bfloat16) for i, shape in enumerate(((130,), (130,), (m, 130))))
+
+    def run():
+        a, b = sdq.fp8_quantize(x), sdq.fp8_quantize_weight(w)
+        return [*a, *b, sdq.fp8_matmul(*a, *b, bias=bias, act="silu", gate=gate, residual=res), sdq.fp8_matmul(*a, *b, out_dtype=torch.float32),
+                sdq.fp8_quantize(x.view(1, m, 272))[0]]
+
+    quick = run()
+    for name in ("_quantize", "_quantize_weight", "_matmul"):
+        monkeypatch.setattr(fp8, name, lambda *args: None)
+    for a, b in zip(quick, run()):
+        assert a.dtype is b.dtype and a.shape == b.shape and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_refusals_of_the_package():
     xq, xs, wq, ws = operands(3, 4, 256, 130)
     bad = [
@@ -346,7 +367,7 @@ def test_refusals_of_the_package():
             call()
 
 
-@pytest.mark.parametrize("m", [20, 300])
+@pytest.mark.parametrize("m", [100, 300])
 def test_withheld_copy_times_out_then_the_next_call_is_correct(m):
     """The bounded waits (see test_gpu_abort.py) of the fp8 kernel."""
     ops = operands(5, m, 1024, 512)

@@ -192,6 +192,25 @@ def test_empty_and_another_stream_and_a_graph():
     assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+@pytest.mark.parametrize("pairs", ["interleaved", "halves"])
+def test_the_shortcut_and_ctypes_make_the_same_calls(pairs, monkeypatch):
+    from sdq import heads
+
+    q, k, v = normals(1, 2, 9, 4, 64), normals(2, 2, 9, 2, 64), normals(3, 2, 9, 2, 64)
+    cos, sin = tables(50, 32)
+    w = 1 + 0.1 * normals(4, 64)
+    pos = torch.arange(18, device="cuda").view(2, 9)
+    place = [torch.empty(2, h, 9, 64, device="cuda") for h in (4, 2, 2)]
+
+    def run():
+        return [*sdq.qk_norm_rope(q, k, v, w, w, cos, sin, 1e-5, pos, pairs), *sdq.qk_norm_rope(q, k, None, None, w)[:2],
+                *(t.clone() for t in sdq.qk_norm_rope(q, k, v, w, None, cos, sin, positions=pos.int(), pairs=pairs, out=place))]
+
+    quick = run()
+    monkeypatch.setattr(heads, "_heads", lambda *args: None)
+    assert all(torch.equal(a, b) for a, b in zip(quick, run()))
+
+
 def test_refusals_of_the_package():
     q, k = normals(1, 1, 4, 2, 64), normals(2, 1, 4, 2, 64)
     cos, sin = tables(4, 64)
