@@ -545,9 +545,7 @@ int sdq_fp8_matmul(const uint8_t* xq, const uint8_t* x_scales, int64_t m, int64_
     epi.resid = static_cast<const uint16_t*>(residual);
     epi.f32 = y_dtype == SDQ_F32;
     const char* msg = nullptr;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e = m <= fp8_mv_tokens() ? launch_fp8_mv(xq, x_scales, m, k, wq, w_scales, n, epi, y, st)
-                                         : launch_fp8_mm(xq, x_scales, m, k, wq, w_scales, n, epi, y, st, &msg);
+    cudaError_t e = launch_fp8_mm(xq, x_scales, m, k, wq, w_scales, n, epi, y, static_cast<cudaStream_t>(stream), &msg);
     if (e != cudaSuccess) {
         if (msg) return fail(SDQ_ERR_CUDA, "%s: %s", fn, msg);
         return cuda_fail("sdq_fp8_matmul: kernel launch", e);

@@ -14,6 +14,11 @@
 // token and stores whole 32-byte sectors.  (The other way round each thread held one feature and
 // stored 2 bytes a time, which cost more than the product at K = 4096.)
 //
+// One kernel for every number of tokens.  For a few of them a stream of the weight through mma.sync
+// was measured beside it and is not kept: its e4m3 form is emulated on sm_100a (170 cycles each), and
+// with the codes turned into f16 the conversion sets the pace (1 x 2560 x 9728: 14.3 us by the
+// conversion instruction, 18.7 by shifts, 7.5 here, where nothing is unpacked).
+//
 // Warp roles (512 threads, one CTA per SM, persistent over tiles):
 //   warp 0       TMA producer of the operand ring (one thread)
 //   warp 1       tensor memory allocator and MMA issuer (one thread; in a pair, rank 0's)

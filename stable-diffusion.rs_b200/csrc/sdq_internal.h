@@ -119,11 +119,6 @@ cudaError_t launch_fp8_dequantize(const uint8_t* q, const uint8_t* scales, int64
 cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t k, const uint8_t* wq,
                           const uint8_t* ws, int64_t n, const EpiArgs& epi, void* y, cudaStream_t st,
                           const char** msg);
-// The same product for at most fp8_mv_tokens() tokens, steps of K spread over warps (sdq_fp8_mv.cu).
-int fp8_mv_tokens();
-cudaError_t launch_fp8_mv(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t k, const uint8_t* wq,
-                          const uint8_t* ws, int64_t n, const EpiArgs& epi, void* y, cudaStream_t st);
-
 // Queries, keys and values made ready for attention (sdq_qk.cu).  Strides in elements; the last
 // axis is contiguous.  heads[i] == 0 leaves tensor i out; weight == nullptr skips the norm,
 // rope == 0 the rotation.

@@ -124,7 +124,7 @@ def check(got, want, tol):
     assert not bad.any(), (int(bad.sum()), got[bad][:4], want[bad][:4], tol[bad][:4])
 
 
-# m: one row, the small-M kernel's edges, the token tiles' edges; n and k ragged and whole.
+# m: one row, a tile's edges, pairs' edges; n and k ragged and whole.
 MM = [(1, 16, 1), (1, 128, 128), (2, 256, 130), (3, 144, 8), (5, 2576, 333), (8, 512, 640), (9, 400, 257), (16, 1024, 256),
       (17, 128, 100), (33, 272, 515), (64, 640, 128), (65, 1040, 384), (128, 512, 129), (129, 4096, 256), (224, 256, 512),
       (225, 768, 1000), (333, 2576, 499), (512, 1024, 2048), (1000, 208, 3001)]
