@@ -184,6 +184,19 @@ def test_f32_result_with_an_f32_bias(m):
     check(y, want + bias.double(), sums_tol(s, k) + (want + bias.double()).abs() * 2.0 ** -23)
 
 
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_scales_far_apart_and_codes_of_any_value(m):
+    """Scales from 2^-40 to 2^40 in no order, every finite code, operands that no quantiser made."""
+    k, n = 400, 200
+    g = torch.Generator("cuda").manual_seed(m)
+    code = lambda r: (lambda c: torch.where((c & 0x7F) == 0x7F, c - 1, c))(torch.randint(0, 256, (r, k), device="cuda", generator=g)).to(torch.uint8).view(torch.float8_e4m3fn)  # noqa: E731
+    byte = lambda *s: torch.randint(87, 168, s, device="cuda", generator=g).to(torch.uint8).view(torch.float8_e8m0fnu)  # noqa: E731
+    ops = (code(m), byte(4, m), code(n), byte(2, 4))
+    want, s = product(*ops)
+    check(sdq.fp8_matmul(*ops, out_dtype=torch.float32), want, want.abs() * 2.0 ** -24 + sums_tol(s, k))
+    check(sdq.fp8_matmul(*ops), want, want.abs() * 2.0 ** -8 + sums_tol(s, k))
+
+
 @pytest.mark.parametrize("m", [2, 20, 300])
 def test_nan_stays_in_its_row_and_its_features(m):
     """A NaN group of an activation makes that token's row NaN and nothing else; a NaN block of a
