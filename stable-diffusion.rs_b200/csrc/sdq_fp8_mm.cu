@@ -102,6 +102,18 @@ __device__ __forceinline__ float2 gelu2(float2 a) {
     return fma2(h, make_float2(tanh_approx(arg.x), tanh_approx(arg.y)), h);
 }
 
+// Its SiLU of two values, a / (1 + 2^(-a log2 e)), with the hardware exponential and reciprocal (the
+// sum overflows to infinity where the result is 0).
+__device__ __forceinline__ float2 silu2(float2 a) {
+    float2 e = mul2(a, make_float2(-1.4426950408889634f, -1.4426950408889634f)), r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
+    e = add2(e, make_float2(1.f, 1.f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+    return mul2(a, r);
+}
+
 template <bool PAIR, bool FUSED, bool YF32>
 __global__ void __launch_bounds__(kMmThreads, 1)
     fp8_mm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
@@ -422,8 +434,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                             for (int j = 0; j < 16; ++j) o[j] = gelu2(o[j]);
                         } else if (epi.act == SDQ_ACT_SILU) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                o[j] = make_float2(epi_activation(o[j].x, SDQ_ACT_SILU), epi_activation(o[j].y, SDQ_ACT_SILU));
+                            for (int j = 0; j < 16; ++j) o[j] = silu2(o[j]);
                         }
                         if (epi.gate != nullptr) {
 #pragma unroll
