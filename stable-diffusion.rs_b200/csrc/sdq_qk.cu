@@ -21,7 +21,7 @@
 // output.  The norm's weights are multiplied into the cosines and sines once for all the heads:
 // a c - b s becomes r (x0 (w0 c) - x1 (w1 s)), three operations a value.
 // 4608 tokens, 72 heads of 128: a block a token, looping over its heads, took 63 us (49 KB a SM
-// under way); this layout 40 with the norm and the rotation one after the other, now 30.5 (5.6 TB/s).
+// under way); this layout 40 with the norm and the rotation one after the other, now 30.4 (5.6 TB/s).
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -32,9 +32,9 @@
 namespace sdq {
 namespace {
 
-// A block: 8 warps took 34 us for the case above, 4 32, 2 31.6, 1 31.2 (and 10 % longer at 4096 x 18
-// heads of 80); plain loads 3 % less than streaming ones.
-constexpr int kWarps = 2;
+// A block: 8 warps took 34 us for the case above, 4 and 2 30.3 (2 10 % longer at 4096 x 18 heads of
+// 80), 1 43.8; plain loads 3 % less than streaming ones.
+constexpr int kWarps = 4;
 // Heads a lane group loads before it works on the first: 2 took 10 % longer than 4, 8 20 %; one, for
 // calls of a few tokens, gained 4 % up to 16 tokens and lost 15 % at 128.
 constexpr int kBatch = 4;
@@ -95,9 +95,9 @@ template <bool BF16, bool INTER, int LPV>
 __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__ QkArgs a) {
     constexpr int kSide = 32 / LPV, kHeads = kSide * kBatch;      // vectors side by side; heads a piece
     const int lane = threadIdx.x & 31, l = lane % LPV, e = 8 * l;
-    const int64_t bt = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (bt >= a.batch * a.tokens) return;                // whole warps
-    const int64_t b = bt / a.tokens, t = bt - b * a.tokens;
+    const uint32_t bt = blockIdx.x * kWarps + (threadIdx.x >> 5);      // batch * tokens < 2^31
+    if (bt >= (uint32_t)(a.batch * a.tokens)) return;    // whole warps
+    const int64_t b = bt / (uint32_t)a.tokens, t = bt - (uint32_t)b * (uint32_t)a.tokens;
     int piece = blockIdx.y, kind = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
