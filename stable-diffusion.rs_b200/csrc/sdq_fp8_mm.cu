@@ -14,6 +14,10 @@
 // token and stores whole 32-byte sectors.  (The other way round each thread held one feature and
 // stored 2 bytes a time, which cost more than the product at K = 4096.)
 //
+// Where the tiles leave SMs idle and K is long, a cluster of 2, 4 or 8 CTAs shares one tile's K (SPLIT):
+// each accumulates its steps, then they exchange pieces of 16 features through one another's shared
+// memory, each adding up (in the order of K) and storing its own.  1 x 9728 x 2560: 15.3 -> 9.6 us.
+//
 // One kernel for every number of tokens.  For a few of them a stream of the weight through mma.sync
 // was measured beside it and is not kept: its e4m3 form is emulated on sm_100a (170 cycles each), and
 // with the codes turned into f16 the conversion sets the pace (1 x 2560 x 9728: 14.3 us by the
@@ -64,6 +68,7 @@ struct MmPlan {
     int nft, ntt;          // feature tiles, token tiles
     int stages;            // ring depth
     int group;             // token tiles that are walked together (see place)
+    int split;             // CTAs that share a tile's K
     int x_rows;            // rows of X a CTA loads (128, or M rounded up to 8)
     int aligned;           // rows of y (and resid) start on 32 bytes and hold whole 16-feature pieces
 };
@@ -114,7 +119,7 @@ __device__ __forceinline__ float2 silu2(float2 a) {
     return mul2(a, r);
 }
 
-template <bool PAIR, bool FUSED, bool YF32>
+template <bool PAIR, bool SPLIT, bool FUSED, bool YF32>
 __global__ void __launch_bounds__(kMmThreads, 1)
     fp8_mm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                   const uint8_t* __restrict__ xs, const uint8_t* __restrict__ ws, const EpiArgs epi, void* y,
@@ -173,11 +178,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     griddep_launch_dependents();
     const uint32_t tmem = *tmem_slot;
 
-    const int KT = p.kt;
+    // This CTA's steps: all of them, or its share of the cluster's.
+    const int share = SPLIT ? (int)cluster_rank() : 0;
+    const int kbase = SPLIT ? p.kt * share / p.split : 0, KT = SPLIT ? p.kt * (share + 1) / p.split - kbase : p.kt;
     const int d_cols = (p.bn + 31) / 32 * 32, sf_col = 2 * d_cols;
     const int sb_cols = (p.bn + 127) / 128 * 4, slot_cols = 4 + sb_cols;   // X's four columns, then W's
     const int nft = p.nft, ntt = p.ntt, ntiles = nft * ntt;
-    const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+    const int per_tile_ctas = SPLIT ? p.split : CG;
+    const int first = blockIdx.x / per_tile_ctas, stride = gridDim.x / per_tile_ctas;
     // Tiles go in groups of `group` token tiles; within a group, the tokens of one feature tile
     // first.  So the CTAs at work share W's rows, and the group's X stays in L2 while W streams
     // past it once per group.
@@ -188,6 +196,20 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         tt = g * p.group + (r - ft * h);
     };
 
+    auto place_of = [&](int tile) {
+        int ft, tt;
+        place(tile, ft, tt);
+        return ft;
+    };
+    // The bias and gate of the tile of features f0, f0 + 1, ..., as f32, by the output stage's 256 threads.
+    auto load_bias = [&](int f0) {
+        const int i = threadIdx.x - 256, f = f0 + i;
+        const bool in = i < p.bn && f < p.n;
+        sbias[i] = !in || epi.bias == nullptr ? 0.f
+                   : YF32 ? reinterpret_cast<const float*>(epi.bias)[f] : bf16_bits_to_f32(epi.bias[f]);
+        if (FUSED) sgate[i] = !in || epi.gate == nullptr ? 1.f : bf16_bits_to_f32(epi.gate[f]);
+    };
+    bool complete = false;                       // SPLIT: this warp has seen the accumulator complete
     if (warp == 0) {
         // ------------------------------------------------------------ operand producer
         if (elect_one()) {
@@ -211,8 +233,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                             tma_load_2d_pair(at + kXStage, &tmW, full0 + 8 * s, kt * kFp8Block, wr);
                         } else {
                             mbar_arrive_expect_tx(full + s, my_bytes);
-                            tma_load_2d(at, &tmX, full + s, kt * kFp8Block, xr);
-                            tma_load_2d(at + kXStage, &tmW, full + s, kt * kFp8Block, wr);
+                            tma_load_2d(at, &tmX, full + s, (kbase + kt) * kFp8Block, xr);
+                            tma_load_2d(at + kXStage, &tmW, full + s, (kbase + kt) * kFp8Block, wr);
                         }
                     }
                     if (++s == p.stages) { s = 0; phase ^= 1; }
@@ -256,10 +278,10 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                     tc_cp_32x16_x4<PAIR>(sf, cells);
                     tc_cp_32x16_x4<PAIR>(sf + 4, cells + 32);
                     if (sb_cols > 4) tc_cp_32x16_x4<PAIR>(sf + 8, cells + 64);
-                    const int left = p.k - kt0 * kFp8Block;
+                    const int left = p.k - (kbase + kt0) * kFp8Block;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        if (left <= q * kFp8Block) break;
+                        if (kt0 + q >= KT) break;
                         if (!mbar_wait(full + s, phase, abort_flag, status, 2u)) { ok = false; break; }
                         tc_fence_after();
                         const uint64_t adesc = adesc0 + (uint32_t)(s * (stage_bytes >> 4));
@@ -312,7 +334,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             for (int q = 0; q < 4; ++q) step[q] = kt0 + q < KT ? q : KT - 1 - kt0;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const uint8_t* x = xs + (int64_t)kt0 * p.m + (t + 32 * c < p.m ? t + 32 * c : p.m - 1);
+                const uint8_t* x = xs + (int64_t)(kbase + kt0) * p.m + (t + 32 * c < p.m ? t + 32 * c : p.m - 1);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) raw[4 * c + q] = __ldg(x + (int64_t)step[q] * p.m);
             }
@@ -320,7 +342,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             for (int c = 4; c < 12; ++c) {
                 if (c >= 8 && sb_cols == 4) break;
                 const int fc = f + 32 * (c - 4) < p.n ? f + 32 * (c - 4) : p.n - 1;
-                const uint8_t* row = ws + (int64_t)(fc / kFp8Block) * KT + kt0;
+                const uint8_t* row = ws + (int64_t)(fc / kFp8Block) * p.kt + kbase + kt0;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) raw[4 * c + q] = __ldg(row + step[q]);
             }
@@ -350,11 +372,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             }
             if (g + kSlots < groups) fetch(g + kSlots);
         }
+    } else if (SPLIT && warp >= 8) {
+        load_bias(place_of(first) * p.bn);
+        complete = __all_sync(0xffffffffu, mbar_wait_sleep(dfull, 0, abort_flag, status, 8u, 32));
     } else if (warp >= 8) {
         // ------------------------------------------------------------ output stage
         // Thread = token (its quarter of the lanes); group e of four warps takes pieces e, e + 2, ...
         // of 32 features.
-        const int e = (warp - 8) >> 2, tid = threadIdx.x - 256;
+        const int e = (warp - 8) >> 2;
         const uint32_t quarter = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t dempty0 = PAIR ? cluster_addr(dempty, 0) : 0;
         float* mine = stage32 + (warp - 8) * 32 * kPitch;
@@ -366,15 +391,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             const int width = p.n - f0 < p.bn ? p.n - f0 : p.bn;
             const int row0 = (tt * CG + (int)rank) * kTokens + 32 * (warp & 3);      // the warp's first token
             const int row = row0 + lane;
-            // The tile's bias and gate, as f32, for all eight warps.
             named_barrier_sync(1, 256);
-            {
-                const int f = f0 + tid;
-                const bool in = tid < width;
-                sbias[tid] = !in || epi.bias == nullptr ? 0.f
-                             : YF32 ? reinterpret_cast<const float*>(epi.bias)[f] : bf16_bits_to_f32(epi.bias[f]);
-                if (FUSED) sgate[tid] = !in || epi.gate == nullptr ? 1.f : bf16_bits_to_f32(epi.gate[f]);
-            }
+            load_bias(f0);
             const bool resid = FUSED && epi.resid != nullptr;
             if (resid) {
                 // The residual tile on its way to L2 while the accumulator fills: group e, sixteen of
@@ -506,6 +524,97 @@ __global__ void __launch_bounds__(kMmThreads, 1)
 
     tc_fence_before();
     __syncthreads();
+    if constexpr (SPLIT) {
+        // ------------------------------------------------------------ output of a shared tile
+        // Every CTA's copies and MMAs are done: the operand rings are free for the exchange.  Piece
+        // c / 16 belongs to CTA (c / 16) % split; what the others have of it goes into its ring, one
+        // place a sender, four features of 128 tokens at a time (16 bytes a lane, side by side).
+        cluster_sync_relaxed();
+        tc_fence_after();
+        const int e = (warp - 8) >> 2, S = p.split;
+        int ft, tt;
+        place(first, ft, tt);
+        const int f0 = ft * p.bn, width = p.n - f0 < p.bn ? p.n - f0 : p.bn;
+        const int row0 = tt * kTokens + 32 * (warp & 3), row = row0 + lane, token = 32 * (warp & 3) + lane;
+        const uint32_t acc = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+        const int places = (p.bn / 16 + S - 1) / S;                      // pieces a CTA owns at most
+        auto slot_of = [&](int sender, int piece) { return (uint32_t)((sender * places + piece / S) * 4 * kTokens * 16); };
+        if (warp >= 8 && complete && row0 < p.m) {
+            for (int piece = e; 16 * piece < width; piece += 2) {
+                const int owner = piece % S;
+                if (owner == share) continue;
+                uint32_t v[16];
+                __syncwarp();
+                tmem_ld16(acc + 16 * piece, v);
+                tc_wait_ld();
+                const uint32_t to = cluster_addr(smem, owner) + slot_of(share, piece) + 16 * token;
+                if (row < p.m) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        st_cluster_16(to + q * kTokens * 16, make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]),
+                                                                         __uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])));
+                }
+            }
+        }
+        cluster_sync();
+        if (warp >= 8 && complete && row0 < p.m) {
+            for (int piece = e; 16 * piece < width; piece += 2) {
+                if (piece % S != share) continue;
+                uint32_t v[16];
+                __syncwarp();
+                tmem_ld16(acc + 16 * piece, v);
+                tc_wait_ld();
+                if (row >= p.m) continue;
+                float a[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) a[j] = 0.f;
+                for (int from = 0; from < S; ++from) {
+                    const float4* at = reinterpret_cast<const float4*>(smem + slot_of(from, piece)) + token;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 z = from == share ? make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]),
+                                                                     __uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3]))
+                                                       : at[q * kTokens];
+                        a[4 * q] += z.x; a[4 * q + 1] += z.y; a[4 * q + 2] += z.z; a[4 * q + 3] += z.w;
+                    }
+                }
+                const int64_t to = (int64_t)row * p.n + f0 + 16 * piece;
+                uint32_t o[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int i = 16 * piece + j;
+                    float z = a[j] + sbias[i];
+                    if (YF32) {
+                        o[j] = __float_as_uint(z);
+                    } else {
+                        if (FUSED) {
+                            z = epi_activation(z, epi.act) * sgate[i];
+                            if (epi.resid != nullptr && f0 + i < p.n) z += bf16_bits_to_f32(epi.resid[to + j]);
+                        }
+                        if (j & 1) o[j / 2] = pack_bf16x2(__uint_as_float(o[j / 2]), z);
+                        else o[j / 2] = __float_as_uint(z);
+                    }
+                }
+                if (p.aligned) {
+                    if (YF32) {
+                        st_global_32(static_cast<float*>(y) + to, reinterpret_cast<uint32_t(&)[8]>(o[0]));
+                        st_global_32(static_cast<float*>(y) + to + 8, reinterpret_cast<uint32_t(&)[8]>(o[8]));
+                    } else {
+                        st_global_32(static_cast<uint16_t*>(y) + to, reinterpret_cast<uint32_t(&)[8]>(o[0]));
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if (f0 + 16 * piece + j >= p.n) break;
+                        if (YF32) static_cast<uint32_t*>(y)[to + j] = o[j];
+                        else static_cast<uint16_t*>(y)[to + j] = (uint16_t)(j & 1 ? o[j / 2] >> 16 : o[j / 2] & 0xFFFFu);
+                    }
+                }
+            }
+        }
+        tc_fence_before();
+        __syncthreads();
+    }
     if (PAIR) cluster_sync();                    // no MMA, copy or arrival still needs the peer
     if (warp == 1) {
         __syncwarp();
@@ -528,41 +637,14 @@ bool byte_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int b
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The tile: a CTA or a pair, and the width, by the time of the longest SM: whole waves of tiles,
-// each KT steps of the longest of the MMAs (2 cycles a feature, 300 at least) and the copies (64
-// bytes a cycle from L2), the last wave's output stage and a pair's later start on top.  Over 24
-// shapes from 1 to 4608 tokens its choice measured within 8 % of the best of all tiles, 4 % mostly (512 x 4096 x
-// 10240: pairs by 144, 20.7 us, best 20.6; by 224, 23.4; single CTAs by 144, 23.5).
-void choose(int64_t m, int64_t n, int64_t k, bool fused, bool& pair, int& bn) {
-    const int64_t kt = (k + kFp8Block - 1) / kFp8Block, sms = num_sms();
-    int64_t best = -1;
-    for (int cg = 1; cg <= (m > kTokens ? 2 : 1); ++cg) {
-        const int64_t ntt = (m + kTokens * cg - 1) / (kTokens * cg);
-        const int64_t x_rows = m < kTokens ? m : kTokens;
-        for (int w = 16; w <= kMaxBn; w += 16) {
-            const int64_t tiles = ntt * ((n + w - 1) / w), waves = (tiles + sms / cg - 1) / (sms / cg);
-            const int64_t copy = (x_rows + w / cg) * kFp8Block / 64;
-            int64_t step = 2 * w > copy ? 2 * w : copy;
-            step = step < 300 ? 300 : step;
-            const int64_t out = 600 + w * (fused ? 24 : 12), tile = kt * step > out ? kt * step : out;
-            const int64_t cost = waves * tile + out + (cg == 2 ? 700 : 0);
-            if (best < 0 || cost < best) {
-                best = cost;
-                pair = cg == 2;
-                bn = w;
-            }
-        }
-    }
-}
-
-template <bool PAIR, bool FUSED, bool YF32>
+template <bool PAIR, bool SPLIT, bool FUSED, bool YF32>
 cudaError_t launch_mm_t(const CUtensorMap& tmX, const CUtensorMap& tmW, const uint8_t* xs, const uint8_t* ws,
                         const EpiArgs& epi, void* y, const MmPlan& p, int grid, size_t smem, cudaStream_t st) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     static bool configured[64] = {};
-    auto kernel = fp8_mm_kernel<PAIR, FUSED, YF32>;
+    auto kernel = fp8_mm_kernel<PAIR, SPLIT, FUSED, YF32>;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQmvMaxSmem);
         if (e != cudaSuccess) return e;
@@ -577,11 +659,84 @@ cudaError_t launch_mm_t(const CUtensorMap& tmX, const CUtensorMap& tmW, const ui
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.x = PAIR ? 2 : p.split;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = PAIR ? 2 : 1;
+    cfg.numAttrs = PAIR || SPLIT ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, tmX, tmW, xs, ws, epi, y, p);
+}
+
+// Clusters of `ctas` CTAs of the kernel that the device runs at once (those of 4 and 8 do not reach
+// every SM: 132 and 120 of 148).
+int clusters_at_once(int ctas) {
+    static int known[64][9] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int& n = known[dev][ctas];
+    if (n == 0) {
+        auto kernel = fp8_mm_kernel<false, true, false, false>;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(ctas * num_sms()));
+        cfg.blockDim = dim3(kMmThreads);
+        cfg.dynamicSmemBytes = kQmvMaxSmem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)ctas;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int at_once = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQmvMaxSmem) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&at_once, kernel, &cfg) != cudaSuccess || at_once < 1) {
+            cudaGetLastError();                  // then no tile is shared that way
+            at_once = -1;
+        }
+        n = at_once;
+    }
+    return n;
+}
+
+// The tile: a CTA, a pair or a cluster that shares it, and the width, by the cycles of the longest SM:
+// whole waves of tiles, each KT steps of the longest of the MMAs (2 cycles a feature, 300 at least) and
+// the copies (64 bytes a cycle from L2), not less than the weight's way from DRAM (3500 bytes a cycle),
+// the last wave's output stage, and a pair's later start or the exchange on top.  Measured, us: 512 x
+// 4096 x 10240 pairs by 144 20.7 (by 224 23.4, CTAs by 144 23.5); 1 x 9728 x 2560 fours by 80 9.6
+// (CTAs by 48 15.3, twos by 48 11.7, eights by 176 10.7); 16 x 8192 x 128 eights by 16 5.7 (CTAs by 32
+// 12.5).  Over some 30 shapes from 1 to 4608 tokens its choice was within 8 % of the best, mostly 4 %.
+void choose(int64_t m, int64_t n, int64_t k, bool fused, bool& pair, int& bn, int& split) {
+    const int64_t kt = (k + kFp8Block - 1) / kFp8Block, sms = num_sms();
+    const int64_t dram = n * k / 3500;
+    int64_t best = -1;
+    for (int cg = 1; cg <= (m > kTokens ? 2 : 1); ++cg) {
+        const int64_t ntt = (m + kTokens * cg - 1) / (kTokens * cg);
+        const int64_t x_rows = m < kTokens ? m : kTokens;
+        for (int w = 16; w <= kMaxBn; w += 16) {
+            const int64_t tiles = ntt * ((n + w - 1) / w), waves = (tiles + sms / cg - 1) / (sms / cg);
+            const int64_t copy = (x_rows + w / cg) * kFp8Block / 64;
+            int64_t step = 2 * w > copy ? 2 * w : copy;
+            step = step < 300 ? 300 : step;
+            const int64_t out = 600 + w * (fused ? 24 : 12), tile = kt * step > out ? kt * step : out;
+            const int64_t cost = (waves * tile > dram ? waves * tile : dram) + out + (cg == 2 ? 700 : 0);
+            if (best < 0 || cost < best) {
+                best = cost;
+                pair = cg == 2;
+                bn = w;
+                split = 1;
+            }
+            // Shared tiles: all clusters at once, a step at least for every CTA, and the exchange.
+            for (int s = 2; cg == 1 && s <= 8 && s <= kt; s *= 2) {
+                if (tiles > clusters_at_once(s)) break;
+                const int64_t steps = (kt + s - 1) / s * step, exchange = 3000 + 150 * s + w * (15 + x_rows / 12);
+                const int64_t shared = (steps > dram ? steps : dram) + out + exchange;
+                if (shared < best) {
+                    best = shared;
+                    pair = false;
+                    bn = w;
+                    split = s;
+                }
+            }
+        }
+    }
 }
 
 }  // namespace
@@ -591,7 +746,7 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
                           const char** msg) {
     MmPlan p{};
     bool pair = false;
-    choose(m, n, k, epi.fused(), pair, p.bn);
+    choose(m, n, k, epi.fused(), pair, p.bn, p.split);
     const int cg = pair ? 2 : 1;
     p.m = (int)m;
     p.n = (int)n;
@@ -609,7 +764,7 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
     const int64_t fit_tt = (32ll << 20) / ((int64_t)cg * kTokens * k);     // token tiles whose X is 32 MB
     p.group = (int)(fit_tt < 1 ? 1 : (fit_tt < ntt ? fit_tt : ntt));
     const int64_t places = num_sms() / cg;
-    const int grid = (int)(tiles < places ? tiles : places) * cg;
+    const int grid = p.split > 1 ? (int)tiles * p.split : (int)(tiles < places ? tiles : places) * cg;
     CUtensorMap tmX, tmW;
     if (!byte_map(&tmX, xq, m, k, p.x_rows) || !byte_map(&tmW, wq, n, k, p.bn / cg)) {
         *msg = "cuTensorMapEncodeTiled rejected an fp8 operand's tensor map";
@@ -618,13 +773,14 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
     // More than half of an SM's shared memory, so that no second CTA waits there for tensor memory.
     size_t smem = fixed + p.stages * stage;
     if (smem < 120 * 1024) smem = 120 * 1024;
-    auto go = [&](auto pr) {
-        constexpr bool P = decltype(pr)::value;
-        if (epi.fused()) return launch_mm_t<P, true, false>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
-        if (epi.f32) return launch_mm_t<P, false, true>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
-        return launch_mm_t<P, false, false>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
+    auto go = [&](auto pr, auto sp) {
+        constexpr bool P = decltype(pr)::value, S = decltype(sp)::value;
+        if (epi.fused()) return launch_mm_t<P, S, true, false>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
+        if (epi.f32) return launch_mm_t<P, S, false, true>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
+        return launch_mm_t<P, S, false, false>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
     };
-    return pair ? go(std::true_type{}) : go(std::false_type{});
+    if (pair) return go(std::true_type{}, std::false_type{});
+    return p.split > 1 ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
 }
 
 cudaError_t read_and_clear_fp8_status(unsigned int* out, cudaStream_t st) {

@@ -334,11 +334,22 @@ __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same for threads that hand nothing over: the arrival releases nothing (releasing costs the wait
+// for the SM's memory operations in flight).
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // The shared::cluster address of `p`'s place in the pair's CTA `rank`.
 __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
+}
+// Four floats into shared memory of any CTA of the cluster.
+__device__ __forceinline__ void st_cluster_16(uint32_t addr, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                 : "memory");
 }
 // One arrival on a barrier of either CTA of the cluster, by its shared::cluster address.  It
 // releases at CTA scope: what it orders are accesses to this CTA's own shared and tensor memory

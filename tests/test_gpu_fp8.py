@@ -127,7 +127,10 @@ def check(got, want, tol):
 # m: one row, a tile's edges, pairs' edges; n and k ragged and whole.
 MM = [(1, 16, 1), (1, 128, 128), (2, 256, 130), (3, 144, 8), (5, 2576, 333), (8, 512, 640), (9, 400, 257), (16, 1024, 256),
       (17, 128, 100), (33, 272, 515), (64, 640, 128), (65, 1040, 384), (128, 512, 129), (129, 4096, 256), (224, 256, 512),
-      (225, 768, 1000), (333, 2576, 499), (512, 1024, 2048), (1000, 208, 3001)]
+      (225, 768, 1000), (333, 2576, 499), (512, 1024, 2048), (1000, 208, 3001),
+      # few tiles and a long K, shared by 2, 4 or 8 CTAs; steps that do not divide evenly, a ragged last one
+      (1, 9728, 1024), (3, 2064, 24), (16, 8192, 40), (100, 4112, 99), (128, 4096, 512), (200, 8080, 130), (7, 9728, 2560),
+      (300, 6000, 64), (1, 16384, 8)]
 
 
 @pytest.mark.parametrize("m,k,n", MM)
@@ -142,7 +145,8 @@ def test_matmul_matches_64_bits(m, k, n):
     check(y, want, want.abs() * 2.0 ** -24 + sums_tol(s, k))
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 512, 256), (7, 400, 130), (40, 272, 300), (300, 640, 1024), (226, 144, 77)])
+@pytest.mark.parametrize("m,k,n", [(1, 512, 256), (7, 400, 130), (40, 272, 300), (300, 640, 1024), (226, 144, 77), (5, 8192, 96),
+                                   (130, 4096, 51)])
 @pytest.mark.parametrize("act", [None, "silu", "gelu_approx"])
 def test_output_stage(m, k, n, act):
     """bias, activation, gate and residual, all of them and in place, against the chain in f64.  The
@@ -230,9 +234,9 @@ def test_nothing_beside_the_result_is_written(m):
     check(y, want, want.abs() * 2.0 ** -8 + sums_tol(s, k))
 
 
-@pytest.mark.parametrize("m", [1, 40, 300])
-def test_same_call_same_bits(m):
-    ops = operands(9, m, 1040, 700)
+@pytest.mark.parametrize("m,k,n", [(1, 1040, 700), (40, 1040, 700), (300, 1040, 700), (9, 9728, 512), (70, 8192, 72)])
+def test_same_call_same_bits(m, k, n):
+    ops = operands(9, m, k, n)
     a = sdq.fp8_matmul(*ops)
     for _ in range(5):
         assert torch.equal(sdq.fp8_matmul(*ops), a)
@@ -380,10 +384,10 @@ def test_refusals_of_the_package():
             call()
 
 
-@pytest.mark.parametrize("m", [100, 300])
-def test_withheld_copy_times_out_then_the_next_call_is_correct(m):
-    """The bounded waits (see test_gpu_abort.py) of the fp8 kernel."""
-    ops = operands(5, m, 1024, 512)
+@pytest.mark.parametrize("m,k,n", [(100, 1024, 4096), (300, 1024, 4096), (20, 8192, 128)])
+def test_withheld_copy_times_out_then_the_next_call_is_correct(m, k, n):
+    """The bounded waits (see test_gpu_abort.py) of the fp8 kernel: single CTAs, pairs, shared tiles."""
+    ops = operands(5, m, k, n)
     want = sdq.fp8_matmul(*ops)
     sdq.device_status()
     sdq.debug_wait_hook(20_000_000, True)
