@@ -15,13 +15,15 @@
 //
 // Bound by memory: every value is read and written once.  A vector lies in the registers of the
 // fewest lanes (a power of two) that hold it at 8 values each: 16-byte accesses for bf16, sums and
-// the halves' partners by shuffles.  A warp takes one token and, for each vector's worth of its
-// lanes, kBatch heads of one of the three tensors, all loads issued before the first is worked on;
-// the warps of a block take neighbouring tokens of the same heads, which lie side by side in the
-// output.  The norm's weights are multiplied into the cosines and sines once for all the heads:
+// the halves' partners by shuffles.  A warp works on one of the three tensors.  The vectors that fit
+// its lanes side by side are heads of one token, or, of tensors with fewer heads than that, the heads
+// of several tokens; for each of them it takes BATCH heads, all loads issued before the first is
+// worked on.  The warps of a block take neighbouring tokens of the same heads, which lie side by side
+// in the output.  The norm's weights are multiplied into the cosines and sines once for all the heads:
 // a c - b s becomes r (x0 (w0 c) - x1 (w1 s)), three operations a value.
 // 4608 tokens, 72 heads of 128: a block a token, looping over its heads, took 63 us (49 KB a SM
-// under way); this layout 40 with the norm and the rotation one after the other, now 30.4 (5.6 TB/s).
+// under way); this layout 40 with the norm and the rotation one after the other, now 30.8 (5.5 TB/s).
+// 4 x 8192 tokens with one query and one key head of 64: 35 us with a token a warp, 7.9 with four.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -35,9 +37,8 @@ namespace {
 // A block: 8 warps took 34 us for the case above, 4 and 2 30.3 (2 10 % longer at 4096 x 18 heads of
 // 80), 1 43.8; plain loads 3 % less than streaming ones.
 constexpr int kWarps = 4;
-// Heads a lane group loads before it works on the first: 2 took 10 % longer than 4, 8 20 %; one, for
-// calls of a few tokens, gained 4 % up to 16 tokens and lost 15 % at 128.
-constexpr int kBatch = 4;
+// BATCH, the heads a lane group loads before it works on the first: 4 (2 took 10 % longer for the case
+// above, 8 20 %), or 1 where no tensor has a second one for it.
 
 // Eight values as they are loaded.
 template <bool BF16>
@@ -89,36 +90,45 @@ struct Raw<false> {
     static constexpr int N = 8;
 };
 
-// LPV lanes hold one vector.  blockIdx.y counts pieces of the queries' heads, then the keys', then
-// the values'.
-template <bool BF16, bool INTER, int LPV>
-__global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__ QkArgs a) {
-    constexpr int kSide = 32 / LPV, kHeads = kSide * kBatch;      // vectors side by side; heads a piece
+// What go() has settled for a launch: for each tensor the logarithm of how many heads lie side by side
+// in a warp (the other lanes take further tokens) and the pieces that its heads come in.
+struct QkPlan {
+    int log_side[3], pieces[3];
+};
+
+// LPV lanes hold one vector.  blockIdx.y counts the pieces of the queries, then the keys', then the
+// values'; tokens go along x (the pieces of one token next to one another took 6 % longer).
+template <bool BF16, bool INTER, int LPV, int BATCH>
+__global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__ QkArgs a, const __grid_constant__ QkPlan p) {
     const int lane = threadIdx.x & 31, l = lane % LPV, e = 8 * l;
-    const uint32_t bt = blockIdx.x * kWarps + (threadIdx.x >> 5);      // batch * tokens < 2^31
-    if (bt >= (uint32_t)(a.batch * a.tokens)) return;    // whole warps
-    const int64_t b = bt / (uint32_t)a.tokens, t = bt - (uint32_t)b * (uint32_t)a.tokens;
     int piece = blockIdx.y, kind = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int n = (a.heads[i] + kHeads - 1) / kHeads;
-        if (kind == i && piece >= n) { piece -= n; kind = i + 1; }
-    }
+    for (int i = 0; i < 2; ++i)
+        if (kind == i && piece >= p.pieces[i]) { piece -= p.pieces[i]; kind = i + 1; }
+    const int log_side = p.log_side[kind], side = 1 << log_side, apart = (32 / LPV) >> log_side;   // heads, tokens of a warp
+    const int group = lane / LPV, which = group & (side - 1);
+    const uint64_t first = (uint64_t)(blockIdx.x * kWarps + (threadIdx.x >> 5)) * apart;
+    const uint32_t all = (uint32_t)(a.batch * a.tokens);                 // < 2^31
+    if (first >= all) return;                            // whole warps
+    const uint32_t bt = (uint32_t)first + (group >> log_side);
+    const bool there = bt < all;
+    const uint32_t at0 = there ? bt : 0;
+    const int64_t b = at0 / (uint32_t)a.tokens, t = at0 - (uint32_t)b * (uint32_t)a.tokens;
     const QkTensor& x = a.in[kind];
     const QkTensor& y = a.out[kind];
     // Vectors this lane takes part in (a head of 80 values fills 10 of 16 lanes).
-    const int h0 = piece * kHeads + lane / LPV;
-    const int count = e < a.d ? a.heads[kind] - h0 : 0;  // vector j is there when j * kSide < count
+    const int h0 = piece * side * BATCH + which;
+    const int count = there && e < a.d ? a.heads[kind] - h0 : 0;         // vector j is there when j * side < count
     int64_t from = b * x.batch_stride + t * x.token_stride + h0 * x.head_stride + e;
     int64_t to = b * y.batch_stride + t * y.token_stride + h0 * y.head_stride + e;
 
-    Raw<BF16> v[kBatch];
+    Raw<BF16> v[BATCH];
     griddep_wait();
     griddep_launch_dependents();
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-        if (j * kSide < count) {
-            v[j].load(x.data, from + j * kSide * x.head_stride);
+    for (int j = 0; j < BATCH; ++j) {
+        if (j * side < count) {
+            v[j].load(x.data, from + j * side * x.head_stride);
         } else {
 #pragma unroll
             for (int i = 0; i < Raw<BF16>::N; ++i) v[j].w[i] = 0;
@@ -126,8 +136,8 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
     }
     if (kind == 2) {
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-            if (j * kSide < count) v[j].put(y.data, to + j * kSide * y.head_stride);
+        for (int j = 0; j < BATCH; ++j)
+            if (j * side < count) v[j].put(y.data, to + j * side * y.head_stride);
         return;
     }
 
@@ -189,9 +199,9 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
         }
     }
 
-    float r[kBatch];
+    float r[BATCH];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
+    for (int j = 0; j < BATCH; ++j) {
         r[j] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) r[j] = fmaf(v[j].get(i), v[j].get(i), r[j]);
@@ -199,17 +209,17 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
 #pragma unroll
     for (int m = 1; m < LPV; m <<= 1) {
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) r[j] += __shfl_xor_sync(0xFFFFFFFFu, r[j], m);
+        for (int j = 0; j < BATCH; ++j) r[j] += __shfl_xor_sync(0xFFFFFFFFu, r[j], m);
     }
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
+    for (int j = 0; j < BATCH; ++j) {
         Raw<BF16> o;                                     // halves: the partner's values
         if (!INTER) {
             const int lp = lane + (partner - e) / 8;
 #pragma unroll
             for (int i = 0; i < Raw<BF16>::N; ++i) o.w[i] = __shfl_sync(0xFFFFFFFFu, v[j].w[i], lp);
         }
-        if (j * kSide < count) {
+        if (j * side < count) {
             const float rj = weight != nullptr ? rsqrtf(r[j] * a.inv_d + a.eps) : 1.f;
             float f[8];
 #pragma unroll
@@ -218,18 +228,33 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
                 if (turns) f[i] = fmaf(INTER ? v[j].get(i ^ 1) : o.get(i), other[i], f[i]);
                 f[i] *= rj;
             }
-            Raw<BF16>::store(y.data, to + j * kSide * y.head_stride, f);
+            Raw<BF16>::store(y.data, to + j * side * y.head_stride, f);
         }
     }
 }
 
 template <bool BF16, bool INTER, int LPV>
 cudaError_t go(const QkArgs& a, cudaStream_t st) {
-    constexpr int kSide = 32 / LPV;
-    const unsigned blocks = (unsigned)((a.batch * a.tokens + kWarps - 1) / kWarps);
+    constexpr int kGroups = 32 / LPV;
+    const int64_t all = a.batch * a.tokens;
+    QkPlan p{};
+    bool one = true;
+    for (int i = 0; i < 3; ++i) {
+        while ((1 << p.log_side[i]) < kGroups && (1 << p.log_side[i]) < a.heads[i]) ++p.log_side[i];
+        one = one && a.heads[i] <= 1 << p.log_side[i];
+    }
+    // Tensors with fewer heads have further tokens in a warp and leave the last blocks of x idle.
+    int64_t blocks = 0;
     unsigned pieces = 0;
-    for (int h : a.heads) pieces += (unsigned)((h + kBatch * kSide - 1) / (kBatch * kSide));
-    return launch_programmatic(qk_kernel<BF16, INTER, LPV>, dim3(blocks, pieces), 32 * kWarps, 0, st, a);
+    for (int i = 0; i < 3; ++i) {
+        const int heads = (1 << p.log_side[i]) * (one ? 1 : 4), tokens = kWarps * (kGroups >> p.log_side[i]);
+        p.pieces[i] = (a.heads[i] + heads - 1) / heads;
+        pieces += (unsigned)p.pieces[i];
+        if (a.heads[i] > 0 && (all + tokens - 1) / tokens > blocks) blocks = (all + tokens - 1) / tokens;
+    }
+    const dim3 grid((unsigned)blocks, pieces);
+    return one ? launch_programmatic(qk_kernel<BF16, INTER, LPV, 1>, grid, 32 * kWarps, 0, st, a, p)
+               : launch_programmatic(qk_kernel<BF16, INTER, LPV, 4>, grid, 32 * kWarps, 0, st, a, p);
 }
 
 template <bool BF16, bool INTER>

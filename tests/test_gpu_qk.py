@@ -58,6 +58,8 @@ CASES = [  # b, n, heads, kv heads, d, rope
     (1, 1, 1, 1, 8, 0), (1, 1, 2, 1, 16, 16), (2, 3, 4, 4, 32, 32), (1, 7, 5, 1, 48, 16), (3, 1, 28, 4, 128, 128),
     (1, 129, 24, 24, 128, 128), (2, 33, 14, 2, 80, 80), (1, 65, 8, 8, 96, 48), (1, 40, 7, 1, 256, 256), (2, 300, 1, 1, 64, 32),
     (1, 2, 100, 100, 128, 64),
+    # fewer heads than fit a warp: several tokens side by side, the last of them not there
+    (3, 37, 1, 1, 32, 32), (2, 5, 3, 1, 16, 16), (1, 9, 9, 1, 64, 64), (5, 3, 2, 2, 8, 0), (1, 41, 33, 1, 32, 16),
 ]
 
 
