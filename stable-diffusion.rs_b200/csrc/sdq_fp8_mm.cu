@@ -27,7 +27,7 @@
 //   warp 0       TMA producer of the operand ring (one thread)
 //   warp 1       tensor memory allocator and MMA issuer (one thread; in a pair, rank 0's)
 //   warps 4-7    scale bytes: global -> registers, four groups ahead -> shared memory
-//   warps 8-15   output stage, two groups of four warps taking 32 features in turn
+//   warps 8-15   output stage, two groups of four warps, a half of the tile's features each
 // Every mbarrier wait is bounded; on expiry the kernel records a status bit, waits for its own
 // copies and MMAs, frees its tensor memory and returns.
 #include <cstdint>
@@ -55,10 +55,23 @@ constexpr int kMaxStages = 12;
 constexpr int kSlots = 4;                          // scale groups in tensor memory, one for each scale warp
 constexpr int kCells = 3 * 512;                    // bytes of a group's scales in shared memory
 static_assert(2 * kMaxBn + kSlots * 12 <= 512, "tensor memory");
-constexpr int kPitch = 33;                         // words per token of a warp's transposing buffer
-constexpr int kFixedSmem = 1024 /* alignment */ + 512 /* barriers */ + 2 * 256 * 4 /* bias, gate */ +
+constexpr int kMaxPitch = 43;                      // words per token of a warp's transposing buffer
+constexpr int kFixedSmem = 1024 /* alignment */ + 512 /* barriers */ + 4 * 256 * 4 /* two tiles' bias and gate */ +
                            kSlots * kCells;
-constexpr int kTransposeSmem = 8 * 32 * kPitch * 4;
+constexpr int kTransposeSmem = 8 * 32 * kMaxPitch * 4 + 32 /* a cut chunk is read whole */;
+
+// Quotients of numbers below 2^31 by a settled divisor d, 2^(l-1) < d <= 2^l: n / d is the upper half of
+// n * ceil(2^(31+l) / d), l - 1 places down.  (A tile's place took 400 cycles by division.)
+struct Divisor {
+    uint32_t mul, shift;
+    Divisor(uint32_t d = 1) {
+        uint32_t l = 0;
+        while ((1ull << l) < d) ++l;
+        mul = l == 0 ? 0 : (uint32_t)(((1ull << (31 + l)) + d - 1) / d);      // d = 1: n itself
+        shift = l == 0 ? 0 : l - 1;
+    }
+    __device__ __forceinline__ int of(int n) const { return mul == 0 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift); }
+};
 
 // What the host has settled for a launch.
 struct MmPlan {
@@ -68,9 +81,12 @@ struct MmPlan {
     int nft, ntt;          // feature tiles, token tiles
     int stages;            // ring depth
     int group;             // token tiles that are walked together (see place)
+    Divisor by_tiles, by_group, by_rest;   // group * nft; group; the last group's token tiles
     int split;             // CTAs that share a tile's K
     int x_rows;            // rows of X a CTA loads (128, or M rounded up to 8)
     int aligned;           // rows of y (and resid) start on 32 bytes and hold whole 16-feature pieces
+    int resid_like_y;      // resid lies at y's offset within 16 bytes
+    int pitch;             // of the transposing buffer
 };
 
 __device__ __forceinline__ uint64_t pack2(float2 a) {
@@ -119,6 +135,27 @@ __device__ __forceinline__ float2 silu2(float2 a) {
     return mul2(a, r);
 }
 
+// The 2-byte values [a, b) of the 16-byte aligned chunk w, 0 <= a < b <= 8.
+__device__ __forceinline__ void store_chunk(uint8_t* to, const uint32_t (&w)[4], int a, int b) {
+    uint16_t* h = reinterpret_cast<uint16_t*>(to);
+    if (b - a == 8) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if (b == 8) {                         // from a on: 2, 4 and 8 bytes, as far as they are due
+        if (a & 1) h[a] = (uint16_t)((a < 4 ? (a < 2 ? w[0] : w[1]) : (a < 6 ? w[2] : w[3])) >> 16);
+        const int a4 = (a + 1) & 6;
+        if (a < 7 && a4 & 2) *reinterpret_cast<uint32_t*>(h + a4) = a4 < 4 ? w[1] : w[3];
+        if (a < 5) *reinterpret_cast<uint2*>(h + 4) = make_uint2(w[2], w[3]);
+    } else if (a == 0) {                         // up to b: 8, 4 and 2
+        if (b & 4) *reinterpret_cast<uint2*>(h) = make_uint2(w[0], w[1]);
+        if (b & 2) *reinterpret_cast<uint32_t*>(h + (b & 4)) = b & 4 ? w[2] : w[0];
+        if (b & 1) h[b & 6] = (uint16_t)(b & 4 ? (b & 2 ? w[3] : w[2]) : (b & 2 ? w[1] : w[0]));
+    } else {
+#pragma unroll
+        for (int j = 1; j < 7; ++j)
+            if (j >= a && j < b) h[j] = (uint16_t)(j & 1 ? w[j / 2] >> 16 : w[j / 2]);
+    }
+}
+
 template <bool PAIR, bool SPLIT, bool FUSED, bool YF32>
 __global__ void __launch_bounds__(kMmThreads, 1)
     fp8_mm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
@@ -126,7 +163,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                   const __grid_constant__ MmPlan p) {
     constexpr int CG = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    // (An offset, not a cast of the rounded address: from that the compiler made generic accesses.)
+    uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     const int w_rows = p.bn / CG;                               // rows of W this CTA loads
     const int stage_bytes = kXStage + w_rows * kFp8Block;       // both parts multiples of 1024
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
@@ -140,10 +178,10 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     uint64_t* drain = dempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* sbias = reinterpret_cast<float*>(bars + 64);         // [256]
-    float* sgate = sbias + 256;                                 // [256]
+    float* sbias = reinterpret_cast<float*>(bars + 64);         // [2][256], a tile's in turn
+    float* sgate = sbias + 512;                                 // [2][256]
     // [slots][3 column quads][32 lanes][4 columns][4 steps], X's quad first
-    uint8_t* sscale = reinterpret_cast<uint8_t*>(sgate + 256);
+    uint8_t* sscale = reinterpret_cast<uint8_t*>(sgate + 512);
     float* stage32 = reinterpret_cast<float*>(sscale + kSlots * kCells);    // the transposing buffers, if any
     unsigned int* status = &g_fp8_status;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -190,24 +228,29 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     // first.  So the CTAs at work share W's rows, and the group's X stays in L2 while W streams
     // past it once per group.
     auto place = [&](int tile, int& ft, int& tt) {
-        const int per = p.group * nft, g = tile / per, r = tile - g * per;
+        const int g = p.by_tiles.of(tile), r = tile - g * p.group * nft;
         const int h = ntt - g * p.group < p.group ? ntt - g * p.group : p.group;
-        ft = r / h;
+        ft = h == p.group ? p.by_group.of(r) : p.by_rest.of(r);
         tt = g * p.group + (r - ft * h);
     };
 
-    auto place_of = [&](int tile) {
+    // The bias and gate of a tile, a feature for each of the output stage's 256 threads: fetched a tile
+    // ahead, then put into shared memory as f32 (half b of sbias and sgate).  (Fetched when the tile
+    // began, they took 900 cycles of a tile whose output is 3500.)
+    uint32_t bias_bits = 0, gate_bits = 0x3F80;  // as loaded: a conversion would wait for the load
+    auto fetch_bias = [&](int tile) {
         int ft, tt;
         place(tile, ft, tt);
-        return ft;
+        const int i = threadIdx.x - 256, f = ft * p.bn + i;
+        if (i < p.bn && f < p.n) {
+            if (epi.bias != nullptr) bias_bits = YF32 ? reinterpret_cast<const uint32_t*>(epi.bias)[f] : epi.bias[f];
+            if (FUSED && epi.gate != nullptr) gate_bits = epi.gate[f];
+        }
     };
-    // The bias and gate of the tile of features f0, f0 + 1, ..., as f32, by the output stage's 256 threads.
-    auto load_bias = [&](int f0) {
-        const int i = threadIdx.x - 256, f = f0 + i;
-        const bool in = i < p.bn && f < p.n;
-        sbias[i] = !in || epi.bias == nullptr ? 0.f
-                   : YF32 ? reinterpret_cast<const float*>(epi.bias)[f] : bf16_bits_to_f32(epi.bias[f]);
-        if (FUSED) sgate[i] = !in || epi.gate == nullptr ? 1.f : bf16_bits_to_f32(epi.gate[f]);
+    auto put_bias = [&](int b) {
+        const int i = 256 * b + threadIdx.x - 256;
+        sbias[i] = YF32 ? __uint_as_float(bias_bits) : bf16_bits_to_f32(bias_bits);
+        if (FUSED) sgate[i] = bf16_bits_to_f32(gate_bits);
     };
     bool complete = false;                       // SPLIT: this warp has seen the accumulator complete
     if (warp == 0) {
@@ -373,68 +416,117 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             if (g + kSlots < groups) fetch(g + kSlots);
         }
     } else if (SPLIT && warp >= 8) {
-        load_bias(place_of(first) * p.bn);
+        fetch_bias(first);
+        put_bias(0);
         complete = __all_sync(0xffffffffu, mbar_wait_sleep(dfull, 0, abort_flag, status, 8u, 32));
     } else if (warp >= 8) {
         // ------------------------------------------------------------ output stage
-        // Thread = token (its quarter of the lanes); group e of four warps takes pieces e, e + 2, ...
-        // of 32 features.
+        // Thread = token (its quarter of the lanes); group e of four warps takes one half of the tile's
+        // features, 32 at a time.
         const int e = (warp - 8) >> 2;
         const uint32_t quarter = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t dempty0 = PAIR ? cluster_addr(dempty, 0) : 0;
-        float* mine = stage32 + (warp - 8) * 32 * kPitch;
+        const bool resid = FUSED && epi.resid != nullptr;
+        // Rows that do not start on 32 bytes: the warp turns 32 tokens x 32 features around in shared
+        // memory, and a lane stores a chunk, the CHUNK values of an aligned 16 bytes of y; LANES lanes
+        // take a token's piece.  What is over of a piece (row t's chunks start `over` values before
+        // feature c) waits for the next one in front of it.  Chunks that the half's ends cut are stored
+        // in parts.  (Two bytes a lane, 64 bytes of a token a warp, took twice the time: 3907 x 320 x
+        // 8597 with gate and residual 112 us.)
+        constexpr int CHUNK = YF32 ? 4 : 8, LANES = 32 / CHUNK, TOKENS = 32 / LANES;
+        float* mine = stage32 + (warp - 8) * 32 * kMaxPitch;
+        const uint32_t y_off = (uint32_t)(reinterpret_cast<uintptr_t>(y) / (YF32 ? 4 : 2));
+        const int64_t total = (int64_t)p.m * p.n;
+        // The residual tile on its way to L2, a tile ahead: group e, sixteen of the warp's rows, four
+        // lanes a row, 64 features (128 bytes) each.
+        auto prefetch_resid = [&](int tile) {
+            int ft, tt;
+            place(tile, ft, tt);
+            const int left = p.n - ft * p.bn < p.bn ? p.n - ft * p.bn : p.bn;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = (tt * CG + (int)rank) * kTokens + 32 * (warp & 3) + 16 * e + 8 * i + (lane >> 2), c = 64 * (lane & 3);
+                if (c < left && t < p.m) prefetch_l2(epi.resid + (int64_t)t * p.n + ft * p.bn + c);
+            }
+        };
+        if (first < ntiles) {
+            fetch_bias(first);
+            if (resid) prefetch_resid(first);
+        }
         int tc = 0;
         for (int tile = first; tile < ntiles; tile += stride, ++tc) {
             int ft, tt;
             place(tile, ft, tt);
             const int buf = tc & 1, f0 = ft * p.bn;
             const int width = p.n - f0 < p.bn ? p.n - f0 : p.bn;
+            const int half = (width + 63) / 64 * 32, h0 = e * half, h1 = e == 0 && half < width ? half : width;
             const int row0 = (tt * CG + (int)rank) * kTokens + 32 * (warp & 3);      // the warp's first token
-            const int row = row0 + lane;
-            named_barrier_sync(1, 256);
-            load_bias(f0);
-            const bool resid = FUSED && epi.resid != nullptr;
-            if (resid) {
-                // The residual tile on its way to L2 while the accumulator fills: group e, sixteen of
-                // the warp's rows, four lanes a row, 64 features (128 bytes) each.
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int t = row0 + 16 * e + 8 * i + (lane >> 2), c = 64 * (lane & 3);
-                    if (c < width && t < p.m) prefetch_l2(epi.resid + (int64_t)t * p.n + f0 + c);
-                }
+            const int row = row0 + lane, rows = p.m - row0 < 32 ? p.m - row0 : 32;
+            put_bias(buf);                                          // read by all after the barrier below
+            if (tile + stride < ntiles) {
+                fetch_bias(tile + stride);
+                if (resid) prefetch_resid(tile + stride);
             }
-            // The residual of a piece: 32 features of this thread's token or, with any other pitch, this
-            // lane's feature of the warp's 32 tokens, two a word.  The first piece's is fetched while
-            // the accumulator fills.
-            const int rows = p.m - row0 < 32 ? p.m - row0 : 32;
+            // How many values before a piece's first feature token t's first chunk of it starts.
+            auto over = [&](int t) { return (int)((y_off + (uint32_t)(row0 + t) * (uint32_t)p.n) & (CHUNK - 1)); };
+            // The residual of a piece: 32 features of this thread's token, or those of its chunks.  The
+            // first piece's is fetched while the accumulator fills.
             uint32_t r[16];
             auto fetch_resid = [&](int c) {
                 if (p.aligned) {
                     if (row < p.m) {
                         const uint16_t* from = epi.resid + (int64_t)row * p.n + f0 + c;
                         ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[0]), from);
-                        if (width - c > 16) ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[8]), from + 16);
+                        if (h1 - c > 16) ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[8]), from + 16);
                     }
-                } else if (lane < width - c) {
-                    const uint16_t* from = epi.resid + (int64_t)row0 * p.n + f0 + c + lane;
-                    uint32_t one[32];                               // no branch between the loads: all under way at once
+                } else if (p.resid_like_y) {
 #pragma unroll
-                    for (int t = 0; t < 32; ++t) one[t] = from[(int64_t)(t < rows ? t : 0) * p.n];
-#pragma unroll
-                    for (int t = 0; t < 16; ++t) r[t] = one[2 * t] | (one[2 * t + 1] << 16);
+                    for (int u = 0; u < 4; ++u) {
+                        const int t = TOKENS * u + lane / LANES, cs = c - over(t) + CHUNK * (lane % LANES);
+                        const int64_t at = (int64_t)(row0 + t) * p.n + f0 + cs;
+                        // Whole chunks, the neighbours' values in them too, except past the tensor's ends.
+                        if (t < rows && cs + CHUNK > h0 && cs < h1 && at >= 0 && at + CHUNK <= total) {
+                            const uint4 z = *reinterpret_cast<const uint4*>(epi.resid + at);
+                            r[4 * u] = z.x; r[4 * u + 1] = z.y; r[4 * u + 2] = z.z; r[4 * u + 3] = z.w;
+                        }
+                    }
                 }
             };
-            if (resid && row0 < p.m && 32 * e < width) fetch_resid(32 * e);
+            // The chunk of token t that starts at feature cs: from the transposing buffer, plus the
+            // residual (`r4`: as fetched), to memory.
+            auto put = [&](int t, int cs, const float* from, const uint32_t* r4) {
+                if (t >= rows || cs + CHUNK <= h0 || cs >= h1) return;
+                const int64_t at = (int64_t)(row0 + t) * p.n + f0 + cs;
+                const int a = cs < h0 ? h0 - cs : 0, b = h1 - cs < CHUNK ? h1 - cs : CHUNK;     // values [a, b) of it
+                float z[CHUNK];
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < CHUNK; ++j) z[j] = from[j];
+                if (resid) {
+                    if (r4 != nullptr && p.resid_like_y && at >= 0 && at + CHUNK <= total) {
+#pragma unroll
+                        for (int j = 0; j < CHUNK; ++j) z[j] += bf16_bits_to_f32(j & 1 ? r4[j / 2] >> 16 : r4[j / 2] & 0xFFFFu);
+                    } else {
+                        uint32_t one[CHUNK];
+#pragma unroll
+                        for (int j = 0; j < CHUNK; ++j) one[j] = epi.resid[at + (j < a ? a : j < b ? j : b - 1)];
+#pragma unroll
+                        for (int j = 0; j < CHUNK; ++j) z[j] += bf16_bits_to_f32(one[j]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = YF32 ? __float_as_uint(z[j]) : pack_bf16x2(z[(2 * j) % CHUNK], z[(2 * j + 1) % CHUNK]);
+                store_chunk(static_cast<uint8_t*>(y) + at * (16 / CHUNK), w, a * (8 / CHUNK), b * (8 / CHUNK));
+            };
+            if (resid && row0 < p.m && h0 < h1) fetch_resid(h0);
             const bool ok = __all_sync(0xffffffffu, mbar_wait_sleep(dfull + buf, (tc >> 1) & 1, abort_flag, status, 8u, 32));
             // All eight warps go on or none does: none is left at a barrier.
             if (!named_barrier_and(1, 256, ok)) break;
             tc_fence_after();
             if (row0 < p.m) {                                       // warps of tokens that are not there rest
                 const uint32_t acc = tmem + quarter + buf * d_cols;
-                for (int c = 32 * e; c < width; c += 64) {
-                    const int64_t at = (int64_t)row * p.n + f0 + c;
-                    const bool wide = width - c > 16;               // 32 features of this piece, or 16
-                    if (resid && c != 32 * e) fetch_resid(c);
+                for (int c = h0; c < h1; c += 32) {
+                    if (resid && c != h0) fetch_resid(c);
                     uint32_t v[32];
                     __syncwarp();
                     tmem_ld32(acc + c, v);
@@ -442,7 +534,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                     float2 o[16];
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        const float4 b = *reinterpret_cast<const float4*>(sbias + c + 2 * j);
+                        const float4 b = *reinterpret_cast<const float4*>(sbias + 256 * buf + c + 2 * j);
                         o[j] = add2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), make_float2(b.x, b.y));
                         o[j + 1] = add2(make_float2(__uint_as_float(v[2 * j + 2]), __uint_as_float(v[2 * j + 3])), make_float2(b.z, b.w));
                     }
@@ -456,14 +548,15 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                         }
                         if (epi.gate != nullptr) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = mul2(o[j], *reinterpret_cast<const float2*>(sgate + c + 2 * j));
+                            for (int j = 0; j < 16; ++j) o[j] = mul2(o[j], *reinterpret_cast<const float2*>(sgate + 256 * buf + c + 2 * j));
                         }
                     }
                     if (p.aligned) {
+                        const int64_t at = (int64_t)row * p.n + f0 + c;
                         if (row < p.m) {
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                if (h == 1 && !wide) break;
+                                if (h == 1 && h1 - c <= 16) break;  // 32 features of this piece, or 16
                                 uint32_t w[8];
                                 if (YF32) {
 #pragma unroll
@@ -489,26 +582,26 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                             }
                         }
                     } else {
-                        // Any other pitch: the warp turns its 32 tokens x 32 features around in shared
-                        // memory and stores a token's features side by side.
+                        float* to = mine + lane * p.pitch;          // [CHUNK of the last piece, 32]
                         __syncwarp();
+                        if (c != h0) {
+#pragma unroll
+                            for (int j = 0; j < CHUNK; ++j) to[j] = to[32 + j];
+                        }
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            mine[lane * kPitch + 2 * j] = o[j].x;
-                            mine[lane * kPitch + 2 * j + 1] = o[j].y;
+                            to[CHUNK + 2 * j] = o[j].x;
+                            to[CHUNK + 2 * j + 1] = o[j].y;
                         }
                         __syncwarp();
-                        if (lane < width - c) {
-                            const int64_t to = (int64_t)row0 * p.n + f0 + c + lane;
 #pragma unroll
-                            for (int t = 0; t < 32; ++t) {
-                                if (t < rows) {
-                                    float z = mine[t * kPitch + lane];
-                                    if (resid) z += bf16_bits_to_f32(t & 1 ? r[t / 2] >> 16 : r[t / 2] & 0xFFFFu);
-                                    if (YF32) static_cast<float*>(y)[to + (int64_t)t * p.n] = z;
-                                    else static_cast<uint16_t*>(y)[to + (int64_t)t * p.n] = (uint16_t)(pack_bf16x2(z, 0.f) & 0xFFFFu);
-                                }
-                            }
+                        for (int u = 0; u < LANES; ++u) {
+                            const int t = TOKENS * u + lane / LANES, before = over(t), i = CHUNK * (lane % LANES);
+                            put(t, c - before + i, mine + t * p.pitch + CHUNK - before + i, &r[(4 * u) & 15]);
+                        }
+                        if (c + 32 >= h1 && over(lane) != 0) {      // what is over of the last piece
+                            const int before = over(lane);
+                            put(lane, c + 32 - before, to + CHUNK + 32 - before, nullptr);
                         }
                     }
                 }
@@ -698,12 +791,15 @@ int clusters_at_once(int ctas) {
 
 // The tile: a CTA, a pair or a cluster that shares it, and the width, by the cycles of the longest SM:
 // whole waves of tiles, each KT steps of the longest of the MMAs (2 cycles a feature, 300 at least) and
-// the copies (64 bytes a cycle from L2), not less than the weight's way from DRAM (3500 bytes a cycle),
-// the last wave's output stage, and a pair's later start or the exchange on top.  Measured, us: 512 x
-// 4096 x 10240 pairs by 144 20.7 (by 224 23.4, CTAs by 144 23.5); 1 x 9728 x 2560 fours by 80 9.6
-// (CTAs by 48 15.3, twos by 48 11.7, eights by 176 10.7); 16 x 8192 x 128 eights by 16 5.7 (CTAs by 32
-// 12.5).  Over some 30 shapes from 1 to 4608 tokens its choice was within 8 % of the best, mostly 4 %.
-void choose(int64_t m, int64_t n, int64_t k, bool fused, bool& pair, int& bn, int& split) {
+// the copies (64 bytes a cycle from L2), not less than the weight's way from DRAM (3500 bytes a cycle);
+// beside them, a tile behind, the output stage (750 cycles for 64 features, as much again for an
+// activation, gate or residual, 1000 more for rows of any pitch), which of many short tiles sets the
+// pace; the last tile's, and a pair's later start or the exchange, on top.  Measured, us: 512 x 4096 x
+// 10240 pairs by 144 20.3 (CTAs by 144 21.8); 1 x 9728 x 2560 fours by 80 9.1 (CTAs by 48 15.0, twos by
+// 64 11.2, eights by 176 10.2); 16 x 8192 x 128 eights by 16 5.2 (CTAs by 64 12.2); 3116 x 48 x 4181
+// with SiLU CTAs by 224 27.6 (by 80 39.6).  Over some 45 shapes from 1 to 4608 tokens its choice was
+// within 9 % of the best, mostly 4 %.
+void choose(int64_t m, int64_t n, int64_t k, bool fused, bool aligned, bool& pair, int& bn, int& split) {
     const int64_t kt = (k + kFp8Block - 1) / kFp8Block, sms = num_sms();
     const int64_t dram = n * k / 3500;
     int64_t best = -1;
@@ -715,8 +811,8 @@ void choose(int64_t m, int64_t n, int64_t k, bool fused, bool& pair, int& bn, in
             const int64_t copy = (x_rows + w / cg) * kFp8Block / 64;
             int64_t step = 2 * w > copy ? 2 * w : copy;
             step = step < 300 ? 300 : step;
-            const int64_t out = 600 + w * (fused ? 24 : 12), tile = kt * step > out ? kt * step : out;
-            const int64_t cost = (waves * tile > dram ? waves * tile : dram) + out + (cg == 2 ? 700 : 0);
+            const int64_t out = 900 + (w + 63) / 64 * (750 + (fused ? 750 : 0) + (aligned ? 0 : 1000)), tile = kt * step > out ? kt * step : out;
+            const int64_t all = kt * step + (waves - 1) * tile, cost = (all > dram ? all : dram) + out + (cg == 2 ? 700 : 0);
             if (best < 0 || cost < best) {
                 best = cost;
                 pair = cg == 2;
@@ -746,15 +842,19 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
                           const char** msg) {
     MmPlan p{};
     bool pair = false;
-    choose(m, n, k, epi.fused(), pair, p.bn, p.split);
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(y) | (epi.resid ? reinterpret_cast<uintptr_t>(epi.resid) : 0);
+    p.aligned = n % 16 == 0 && bases % 32 == 0;
+    choose(m, n, k, epi.fused(), p.aligned, pair, p.bn, p.split);
     const int cg = pair ? 2 : 1;
     p.m = (int)m;
     p.n = (int)n;
     p.k = (int)k;
     p.kt = (int)((k + kFp8Block - 1) / kFp8Block);
     p.x_rows = m < kTokens ? (int)((m + 7) / 8 * 8) : kTokens;
-    const uintptr_t bases = reinterpret_cast<uintptr_t>(y) | (epi.resid ? reinterpret_cast<uintptr_t>(epi.resid) : 0);
-    p.aligned = n % 16 == 0 && bases % 32 == 0;
+    p.resid_like_y = (reinterpret_cast<uintptr_t>(y) - reinterpret_cast<uintptr_t>(epi.resid)) % 16 == 0;
+    // Odd, so that a lane a token writes without bank conflicts; lanes that read a chunk each, of rows
+    // whose chunks start n values further back each time, then meet in pairs at most.
+    p.pitch = n % 4 == 1 ? kMaxPitch : kMaxPitch - 2;
     const size_t fixed = kFixedSmem + (p.aligned ? 0 : kTransposeSmem), stage = kXStage + (size_t)(p.bn / cg) * kFp8Block;
     const int fit = (int)((kQmvMaxSmem - fixed) / stage);
     p.stages = fit < kMaxStages ? fit : kMaxStages;
@@ -763,6 +863,9 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
     p.ntt = (int)ntt;
     const int64_t fit_tt = (32ll << 20) / ((int64_t)cg * kTokens * k);     // token tiles whose X is 32 MB
     p.group = (int)(fit_tt < 1 ? 1 : (fit_tt < ntt ? fit_tt : ntt));
+    p.by_tiles = Divisor((uint32_t)(p.group * p.nft));
+    p.by_group = Divisor((uint32_t)p.group);
+    p.by_rest = Divisor((uint32_t)(ntt % p.group ? ntt % p.group : p.group));
     const int64_t places = num_sms() / cg;
     const int grid = p.split > 1 ? (int)tiles * p.split : (int)(tiles < places ? tiles : places) * cg;
     CUtensorMap tmX, tmW;

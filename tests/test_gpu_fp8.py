@@ -234,6 +234,35 @@ def test_nothing_beside_the_result_is_written(m):
     check(y, want, want.abs() * 2.0 ** -8 + sums_tol(s, k))
 
 
+@pytest.mark.parametrize("oy,orr", [(0, 0), (1, 1), (3, 8), (6, 1), (8, 0), (16, 16)])
+@pytest.mark.parametrize("m,n", [(1, 5), (34, 1), (70, 8), (97, 13), (33, 24), (300, 77), (130, 256), (40, 233), (2300, 500)])
+def test_result_and_residual_at_any_offset(m, n, oy, orr):
+    """y and the residual ``oy`` and ``orr`` values past 512 bytes, at the same place within 16 bytes and
+    not, rows of every length: the tensors' ends, chunks that a tile cuts, in place; and y in f32.
+    Sentinels around y stay."""
+    k = 272
+    ops = operands(m + n, m, k, n)
+    want, s = product(*ops)
+    gate = normals(7, n).to(torch.bfloat16)
+    place = lambda o, dt: torch.full((m * n + 128,), -7.0, device="cuda", dtype=dt)[o: o + m * n + 64]  # noqa: E731
+    ry, rr, rf = place(oy, torch.bfloat16), place(orr, torch.bfloat16), place(oy, torch.float32)
+    res, y, yf = (t[: m * n].view(m, n) for t in (rr, ry, rf))
+    res.copy_(normals(8, m, n) * want.abs().mean())
+    z = res.double() + gate.double() * want
+    tol = gate.double().abs() * (sums_tol(s, k) + want.abs() * 2.0 ** -23) + (z.abs() + (gate.double() * want).abs() * 2.0 ** -14) * 2.0 ** -8
+    sdq.fp8_matmul(*ops, gate=gate, residual=res, out=y)
+    check(y, z, tol)
+    sdq.fp8_matmul(*ops, gate=gate, residual=res, out=res)
+    check(res, z, tol)
+    sdq.fp8_matmul(*ops, out=yf)
+    check(yf, want, want.abs() * 2.0 ** -24 + sums_tol(s, k))
+    for room in (ry, rr, rf):
+        assert (room[m * n:] == -7).all()
+    for t in (y, yf, res):
+        before = t._base[: t.storage_offset()]
+        assert (before == -7).all()
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 1040, 700), (40, 1040, 700), (300, 1040, 700), (9, 9728, 512), (70, 8192, 72)])
 def test_same_call_same_bits(m, k, n):
     ops = operands(9, m, k, n)
