@@ -210,7 +210,8 @@ int sdq_fp8_dequantize(const uint8_t* q, const uint8_t* scales, int64_t rows, in
  * bias, gate, residual may be NULL (0, 1, 0); act is one of SDQ_ACT_*.  With y bf16, bias and gate
  * are [n] bf16 and residual [m,n] bf16 (residual may be y itself, but not otherwise overlap it).
  * With y f32 only a bias ([n] f32) may be given.  y overlaps no other input.  m may be 0.  xq and wq
- * are 16-byte aligned.  All sizes run one kernel (block-scaled tcgen05 MMAs, alone or in CTA pairs).
+ * are 16-byte aligned.  All sizes run one kernel (block-scaled tcgen05 MMAs; a CTA, a pair or a cluster
+ * a tile).
  */
 int sdq_fp8_matmul(const uint8_t* xq, const uint8_t* x_scales, int64_t m, int64_t k, const uint8_t* wq,
                    const uint8_t* w_scales, int64_t n, const void* bias, int act, const void* gate,
@@ -233,14 +234,14 @@ typedef struct sdq_heads {
  * [batch, heads, tokens, head_dim], or a part of a longer sequence.  Computed in f32, rounded once.
  *
  * cos and sin are [table_rows, rope_dim/2] f32; a token's row is its index, or positions[b, t]
- * (int32 or int64, rows pos_batch_stride elements apart).  A position outside the tables makes that
- * token's queries and keys NaN.  interleaved non-zero: pairs (x[2i], x[2i+1]), otherwise
+ * (int32 or int64, rows pos_batch_stride elements apart).  A position outside the tables makes the
+ * rotated values of that token's queries and keys NaN.  interleaved non-zero: pairs (x[2i], x[2i+1]), otherwise
  * (x[i], x[i + rope_dim/2]).  v may be NULL, and q or k have 0 heads, to leave them out.
  *
  * dtype (bf16 or f32) is that of the vectors and of the norm's weights.  head_dim is a multiple of 8
  * up to 256; rope_dim (0: no rotation) a multiple of 16, at most head_dim.  Bases and strides keep
  * every vector, and the tables their rows, 16-byte aligned.  An output may be its own input (same
- * address, same strides); otherwise outputs overlap neither inputs nor each other.
+ * address, same strides); otherwise outputs overlap neither inputs nor each other nor themselves.
  *
  * Replaces the reference's split_qkv, qk_norm, concatenation and rotate between the qkv linear and
  * attention (crates/sd-models/src/mlx/flux.rs:302-329, 165-212).

@@ -54,6 +54,15 @@ PyObject* pair(at::Tensor a, at::Tensor b) {
     return t;
 }
 
+// The library's call without the interpreter's lock: a launch may wait for room in the stream's queue.
+template <class F, class... A>
+int unlocked(F f, A... a) {
+    PyThreadState* t = PyEval_SaveThread();
+    const int rc = f(a...);
+    PyEval_RestoreThread(t);
+    return rc;
+}
+
 // quantize(x) and quantize_weight(w) -> (codes, scales)
 template <bool WEIGHT>
 PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -68,7 +77,7 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
     at::Tensor q = empty(x->sizes(), kE4M3, dev);
     at::Tensor s = WEIGHT ? empty({(rows + kBlock - 1) / kBlock, kb}, kE8M0, dev) : empty({kb, rows}, kE8M0, dev);
     const auto f = WEIGHT ? g_quantize_weight : g_quantize;
-    if (f(x->data_ptr(), (sdq_dtype)dt, rows, k, (uint8_t*)q.data_ptr(), (uint8_t*)s.data_ptr(), stream(dev)) != SDQ_OK)
+    if (unlocked(f, x->data_ptr(), (sdq_dtype)dt, rows, k, (uint8_t*)q.data_ptr(), (uint8_t*)s.data_ptr(), stream(dev)) != SDQ_OK)
         Py_RETURN_NONE;
     return pair(std::move(q), std::move(s));
     END_HANDLE_TH_ERRORS
@@ -116,7 +125,7 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
     size.back() = f;
     if (out && !(flat(out, dev, dt) && out->sizes() == at::IntArrayRef(size))) Py_RETURN_NONE;
     at::Tensor y = out ? *out : empty(size, dt, dev);
-    if (g_matmul((const uint8_t*)xq->data_ptr(), (const uint8_t*)xs->data_ptr(), m, k, (const uint8_t*)wq->data_ptr(),
+    if (unlocked(g_matmul, (const uint8_t*)xq->data_ptr(), (const uint8_t*)xs->data_ptr(), m, k, (const uint8_t*)wq->data_ptr(),
                  (const uint8_t*)ws->data_ptr(), f, bias ? bias->data_ptr() : nullptr, act, gate ? gate->data_ptr() : nullptr,
                  residual ? residual->data_ptr() : nullptr, y.data_ptr(), (sdq_dtype)code(dt), stream(dev)) != SDQ_OK)
         Py_RETURN_NONE;
@@ -141,7 +150,7 @@ PyObject* heads(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::ScalarType type = x[0]->scalar_type();
     const int64_t b = x[0]->size(0), t = x[0]->size(1), d = x[0]->size(3);
     PyObject* const given = args[10];
-    if (given != Py_None && !((PyTuple_Check(given) || PyList_Check(given)) && PySequence_Fast_GET_SIZE(given) == count)) Py_RETURN_NONE;
+    if (given != Py_None && !(PyTuple_Check(given) && PyTuple_GET_SIZE(given) == count)) Py_RETURN_NONE;
     at::Tensor made[3];
     const at::Tensor* y[3] = {};
     sdq_heads in[3] = {}, to[3] = {};
@@ -155,7 +164,7 @@ PyObject* heads(PyObject*, PyObject* const* args, Py_ssize_t n) {
             made[i] = empty({b, h, t, d}, type, dev);
             y[i] = &made[i];
         } else {
-            y[i] = tensor(PySequence_Fast_GET_ITEM(given, i));
+            y[i] = tensor(PyTuple_GET_ITEM(given, i));
             if (!y[i] || !here(*y[i], dev) || y[i]->scalar_type() != type || y[i]->dim() != 4 || y[i]->size(0) != b ||
                 y[i]->size(1) != h || y[i]->size(2) != t || y[i]->size(3) != d || y[i]->stride(3) != 1)
                 Py_RETURN_NONE;
@@ -179,7 +188,7 @@ PyObject* heads(PyObject*, PyObject* const* args, Py_ssize_t n) {
             Py_RETURN_NONE;
         stride = pos->stride(0);
     }
-    if (d > 256 || g_heads(&in[0], &in[1], x[2] ? &in[2] : nullptr, &to[0], &to[1], x[2] ? &to[2] : nullptr, (sdq_dtype)dt, b, t,
+    if (d > 256 || unlocked(g_heads, &in[0], &in[1], x[2] ? &in[2] : nullptr, &to[0], &to[1], x[2] ? &to[2] : nullptr, (sdq_dtype)dt, b, t,
                            (int)d, w[0] ? w[0]->data_ptr() : nullptr, w[1] ? w[1]->data_ptr() : nullptr,
                            (float)PyFloat_AS_DOUBLE(args[7]), cos ? cos->data_ptr<float>() : nullptr,
                            sin ? sin->data_ptr<float>() : nullptr, rows, (int)rope, inter, pos ? pos->data_ptr() : nullptr, wide,
@@ -190,7 +199,7 @@ PyObject* heads(PyObject*, PyObject* const* args, Py_ssize_t n) {
     for (int i = 0; i < 3; ++i)
         PyTuple_SET_ITEM(r, i, i >= count ? Py_NewRef(Py_None)
                                           : given == Py_None ? THPVariable_Wrap(std::move(made[i]))
-                                                             : Py_NewRef(PySequence_Fast_GET_ITEM(given, i)));
+                                                             : Py_NewRef(PyTuple_GET_ITEM(given, i)));
     return r;
     END_HANDLE_TH_ERRORS
 }

@@ -591,6 +591,9 @@ int sdq_qk_norm_rope(const sdq_heads* q, const sdq_heads* k, const sdq_heads* v,
             if (!aligned(h->data, 16) || (used * (int64_t)es) % 16 != 0)
                 return fail(SDQ_ERR_INVALID, "%s: %s and its output need 16-byte aligned bases and strides", fn, name);
         }
+        const sdq_heads& o = *out[i];
+        if ((batch > 1 && o.batch_stride == 0) || (tokens > 1 && o.token_stride == 0) || (a.heads[i] > 1 && o.head_stride == 0))
+            return fail(SDQ_ERR_INVALID, "%s: %s's output has a stride of 0", fn, name);
         a.in[i] = {in[i]->data, in[i]->batch_stride, in[i]->token_stride, in[i]->head_stride};
         a.out[i] = {out[i]->data, out[i]->batch_stride, out[i]->token_stride, out[i]->head_stride};
     }

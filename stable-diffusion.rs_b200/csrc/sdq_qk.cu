@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
         }
     }
     // What each value, and its partner's, is multiplied by.  A position outside the tables reads
-    // nothing and makes the token's queries and keys NaN.
+    // nothing and makes what it turns of the token's queries and keys NaN.
     float own[8], other[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) { own[i] = w[i]; other[i] = 0.f; }

@@ -182,9 +182,10 @@ class Fp8Array:
         return fp8_dequantize(self.weight, self.scales, True, out_dtype, stream)
 
     def matmul(self, x: torch.Tensor, bias=None, stream=None, out=None) -> torch.Tensor:
-        """``x @ weight.T`` (+ bias) in x's type, x [..., k] bf16 or f32."""
+        """``x @ weight.T`` (+ bias) in x's type or ``out``'s, x [..., k] bf16 or f32."""
         xq, xs = fp8_quantize(x, stream)
-        return fp8_matmul(xq, xs, self.weight, self.scales, bias=bias, out=out, out_dtype=x.dtype, stream=stream)
+        return fp8_matmul(xq, xs, self.weight, self.scales, bias=bias, out=out, out_dtype=x.dtype if out is None else None,
+                          stream=stream)
 
     def matmul_fused(self, x: torch.Tensor, bias=None, act=None, gate=None, residual=None, out=None,
                      stream=None) -> torch.Tensor:

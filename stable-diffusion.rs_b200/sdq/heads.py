@@ -30,8 +30,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None
     The inputs are bf16 or f32 views of any strides whose last axis is contiguous, such as slices of a
     fused projection.  ``q_weight`` / ``k_weight`` [d] scale the normed vectors (None: no norm).  ``cos``
     and ``sin`` are f32 tables [positions, rope / 2] (None: no rotation), read at the token's index or at
-    ``positions`` [b, n] (int32 or int64); a position outside the tables makes its token's queries and
-    keys NaN.  ``pairs`` says which values turn together: ``"interleaved"`` (2i, 2i + 1) or ``"halves"``
+    ``positions`` [b, n] (int32 or int64); a position outside the tables makes the rotated values of its
+    token's queries and keys NaN.  ``pairs`` says which values turn together: ``"interleaved"`` (2i, 2i + 1) or ``"halves"``
     (i, i + rope / 2); values from rope on stay.  ``out`` gives the three results' places, views
     [b, heads, n, d] of any strides with a contiguous last axis, for instance parts of a joint sequence.
     An output may be its input's own memory (with the same strides), and must not overlap otherwise."""

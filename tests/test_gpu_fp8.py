@@ -9,6 +9,10 @@ every partial sum:  |error| <= (K/32 + 32) 2^-23 S, and 2^-8 of the value for th
 """
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -329,6 +333,8 @@ def test_leading_axes_and_the_array_class():
     check(y.view(14, 300), want, want.abs() * 2.0 ** -8 + sums_tol(s, 256))
     f = a.matmul(x.float())
     assert f.dtype is torch.float32
+    half = torch.empty(*x.shape[:-1], 300, device="cuda", dtype=torch.bfloat16)
+    assert torch.equal(a.matmul(x.float(), out=half), f.to(torch.bfloat16))
     check(f.view(14, 300), want, want.abs() * 2.0 ** -24 + sums_tol(s, 256))
     # each value is within half an e4m3 step (2^-4 of it; 2^-10 of the scale below the normals)
     d = a.dequantize(torch.float32).double()
@@ -361,6 +367,30 @@ def test_another_stream_and_a_captured_graph():
         graphs[i % 2].replay()
         assert torch.equal(out, want)
     sdq.device_status()
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    """Kernels' attributes and the tile choice's device queries are made by the first call: in a capture."""
+    code = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+import sdq
+x, w = torch.randn(2, 8192, device="cuda"), torch.randn(128, 8192, device="cuda")
+qkv = torch.randn(1, 4, 6, 64, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    xq, xs = sdq.fp8_quantize(x)
+    wq, ws = sdq.fp8_quantize_weight(w)
+    y = sdq.fp8_matmul(xq, xs, wq, ws, out_dtype=torch.float32)
+    z = sdq.qk_norm_rope(*qkv.split(2, 2))[0]
+g.replay()
+assert torch.equal(y, sdq.fp8_matmul(xq, xs, wq, ws, out_dtype=torch.float32)) and y.abs().min() > 0
+assert torch.equal(z, sdq.qk_norm_rope(*qkv.split(2, 2))[0])
+sdq.device_status()
+"""
+    done = subprocess.run([sys.executable, "-c", code, os.path.dirname(os.path.dirname(sdq.__file__))], capture_output=True,
+                          text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 @pytest.mark.parametrize("m", [3, 200])

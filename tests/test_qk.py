@@ -12,13 +12,15 @@ from sdq import _abi
 
 
 def _call(dtype=1, b=2, n=3, d=64, qh=4, kh=2, vh=2, ohq=None, q=0x1000, qo=0x2000, st=None, rope=64, rows=3, cos=0x7000,
-          pos=0, pos64=0, w=0x8000, eps=1e-6, no_v=False, no_vout=False):
+          pos=0, pos64=0, w=0x8000, eps=1e-6, no_v=False, no_vout=False, zero=None):
     def h(ptr, heads, token_stride=None):
         return _abi.SdqHeads(ptr, heads, n * heads * d, heads * d if token_stride is None else token_stride, d)
 
     qi, ki, vi = h(q, qh, st), h(0x3000, kh), h(0x4000, vh)
     qo, ko, vo = h(qo, qh if ohq is None else ohq), h(0x5000, kh), h(0x6000, vh)
     r = ctypes.byref
+    if zero:
+        setattr(qo, zero, 0)
     return _abi.lib().sdq_qk_norm_rope(r(qi), r(ki), None if no_v else r(vi), r(qo), r(ko), None if no_vout else r(vo), dtype,
                                        b, n, d, w, w, eps, cos, cos, rows, rope, 1, pos or None, pos64, n, None)
 
@@ -40,6 +42,9 @@ def _call(dtype=1, b=2, n=3, d=64, qh=4, kh=2, vh=2, ohq=None, q=0x1000, qo=0x20
     (dict(q=0), _abi.SDQ_ERR_INVALID, "have data"),
     (dict(q=0x1008), _abi.SDQ_ERR_INVALID, "aligned"),
     (dict(st=4 * 64 + 4), _abi.SDQ_ERR_INVALID, "aligned"),
+    (dict(zero="batch_stride"), _abi.SDQ_ERR_INVALID, "q's output has a stride of 0"),
+    (dict(zero="token_stride"), _abi.SDQ_ERR_INVALID, "q's output has a stride of 0"),
+    (dict(zero="head_stride"), _abi.SDQ_ERR_INVALID, "q's output has a stride of 0"),
     (dict(w=0x8008), _abi.SDQ_ERR_INVALID, "norm weight"),
     (dict(cos=0), _abi.SDQ_ERR_INVALID, "cos and sin"),
     (dict(cos=0x7004), _abi.SDQ_ERR_INVALID, "cos or sin"),
