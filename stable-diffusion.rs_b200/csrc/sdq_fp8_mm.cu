@@ -16,12 +16,12 @@
 //
 // Where the tiles leave SMs idle and K is long, a cluster of 2, 4 or 8 CTAs shares one tile's K (SPLIT):
 // each accumulates its steps, then they exchange pieces of 16 features through one another's shared
-// memory, each adding up (in the order of K) and storing its own.  1 x 9728 x 2560: 15.3 -> 9.6 us.
+// memory, each adding up (in the order of K) and storing its own.  1 x 9728 x 2560: 15.0 -> 9.1 us.
 //
 // One kernel for every number of tokens.  For a few of them a stream of the weight through mma.sync
 // was measured beside it and is not kept: its e4m3 form is emulated on sm_100a (170 cycles each), and
 // with the codes turned into f16 the conversion sets the pace (1 x 2560 x 9728: 14.3 us by the
-// conversion instruction, 18.7 by shifts, 7.5 here, where nothing is unpacked).
+// conversion instruction, 18.7 by shifts, 7.3 here, where nothing is unpacked).
 //
 // Warp roles (512 threads, one CTA per SM, persistent over tiles):
 //   warp 0       TMA producer of the operand ring (one thread)
