@@ -58,7 +58,7 @@ static_assert(2 * kMaxBn + kSlots * 12 <= 512, "tensor memory");
 constexpr int kMaxPitch = 43;                      // words per token of a warp's transposing buffer
 constexpr int kFixedSmem = 1024 /* alignment */ + 512 /* barriers */ + 4 * 256 * 4 /* two tiles' bias and gate */ +
                            kSlots * kCells;
-constexpr int kTransposeSmem = 8 * 32 * kMaxPitch * 4 + 32 /* a cut chunk is read whole */;
+constexpr int kTransposeSmem = 8 * 32 * kMaxPitch * 4;
 
 // Quotients of numbers below 2^31 by a settled divisor d, 2^(l-1) < d <= 2^l: n / d is the upper half of
 // n * ceil(2^(31+l) / d), l - 1 places down.  (A tile's place took 400 cycles by division.)
@@ -135,28 +135,9 @@ __device__ __forceinline__ float2 silu2(float2 a) {
     return mul2(a, r);
 }
 
-// The 2-byte values [a, b) of the 16-byte aligned chunk w, 0 <= a < b <= 8.
-__device__ __forceinline__ void store_chunk(uint8_t* to, const uint32_t (&w)[4], int a, int b) {
-    uint16_t* h = reinterpret_cast<uint16_t*>(to);
-    if (b - a == 8) {
-        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else if (b == 8) {                         // from a on: 2, 4 and 8 bytes, as far as they are due
-        if (a & 1) h[a] = (uint16_t)((a < 4 ? (a < 2 ? w[0] : w[1]) : (a < 6 ? w[2] : w[3])) >> 16);
-        const int a4 = (a + 1) & 6;
-        if (a < 7 && a4 & 2) *reinterpret_cast<uint32_t*>(h + a4) = a4 < 4 ? w[1] : w[3];
-        if (a < 5) *reinterpret_cast<uint2*>(h + 4) = make_uint2(w[2], w[3]);
-    } else if (a == 0) {                         // up to b: 8, 4 and 2
-        if (b & 4) *reinterpret_cast<uint2*>(h) = make_uint2(w[0], w[1]);
-        if (b & 2) *reinterpret_cast<uint32_t*>(h + (b & 4)) = b & 4 ? w[2] : w[0];
-        if (b & 1) h[b & 6] = (uint16_t)(b & 4 ? (b & 2 ? w[3] : w[2]) : (b & 2 ? w[1] : w[0]));
-    } else {
-#pragma unroll
-        for (int j = 1; j < 7; ++j)
-            if (j >= a && j < b) h[j] = (uint16_t)(j & 1 ? w[j / 2] >> 16 : w[j / 2]);
-    }
-}
-
-template <bool PAIR, bool SPLIT, bool FUSED, bool YF32>
+// ANY: rows of y that do not start on 32 bytes (a kernel of its own: the two output stages in one cost
+// the aligned one 3 %).
+template <bool PAIR, bool SPLIT, bool FUSED, bool YF32, bool ANY>
 __global__ void __launch_bounds__(kMmThreads, 1)
     fp8_mm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                   const uint8_t* __restrict__ xs, const uint8_t* __restrict__ ws, const EpiArgs epi, void* y,
@@ -430,13 +411,12 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         // Rows that do not start on 32 bytes: the warp turns 32 tokens x 32 features around in shared
         // memory, and a lane stores a chunk, the CHUNK values of an aligned 16 bytes of y; LANES lanes
         // take a token's piece.  What is over of a piece (row t's chunks start `over` values before
-        // feature c) waits for the next one in front of it.  Chunks that the half's ends cut are stored
-        // in parts.  (Two bytes a lane, 64 bytes of a token a warp, took twice the time: 3907 x 320 x
-        // 8597 with gate and residual 112 us.)
+        // feature c) waits for the next one in front of it.  Values of chunks that the half's ends cut are
+        // stored one by one, a lane a token.  (All of it by 2 bytes a lane, 64 bytes of a token a warp,
+        // took much longer: 3907 x 320 x 8597 with gate and residual 112 us, 66 this way.)
         constexpr int CHUNK = YF32 ? 4 : 8, LANES = 32 / CHUNK, TOKENS = 32 / LANES;
         float* mine = stage32 + (warp - 8) * 32 * kMaxPitch;
         const uint32_t y_off = (uint32_t)(reinterpret_cast<uintptr_t>(y) / (YF32 ? 4 : 2));
-        const int64_t total = (int64_t)p.m * p.n;
         // The residual tile on its way to L2, a tile ahead: group e, sixteen of the warp's rows, four
         // lanes a row, 64 features (128 bytes) each.
         auto prefetch_resid = [&](int tile) {
@@ -473,7 +453,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             // first piece's is fetched while the accumulator fills.
             uint32_t r[16];
             auto fetch_resid = [&](int c) {
-                if (p.aligned) {
+                if (!ANY) {
                     if (row < p.m) {
                         const uint16_t* from = epi.resid + (int64_t)row * p.n + f0 + c;
                         ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[0]), from);
@@ -483,40 +463,46 @@ __global__ void __launch_bounds__(kMmThreads, 1)
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         const int t = TOKENS * u + lane / LANES, cs = c - over(t) + CHUNK * (lane % LANES);
-                        const int64_t at = (int64_t)(row0 + t) * p.n + f0 + cs;
-                        // Whole chunks, the neighbours' values in them too, except past the tensor's ends.
-                        if (t < rows && cs + CHUNK > h0 && cs < h1 && at >= 0 && at + CHUNK <= total) {
-                            const uint4 z = *reinterpret_cast<const uint4*>(epi.resid + at);
+                        if (t < rows && cs >= h0 && cs + CHUNK <= h1) {
+                            const uint4 z = *reinterpret_cast<const uint4*>(epi.resid + (int64_t)(row0 + t) * p.n + f0 + cs);
                             r[4 * u] = z.x; r[4 * u + 1] = z.y; r[4 * u + 2] = z.z; r[4 * u + 3] = z.w;
                         }
                     }
                 }
             };
-            // The chunk of token t that starts at feature cs: from the transposing buffer, plus the
-            // residual (`r4`: as fetched), to memory.
-            auto put = [&](int t, int cs, const float* from, const uint32_t* r4) {
-                if (t >= rows || cs + CHUNK <= h0 || cs >= h1) return;
-                const int64_t at = (int64_t)(row0 + t) * p.n + f0 + cs;
-                const int a = cs < h0 ? h0 - cs : 0, b = h1 - cs < CHUNK ? h1 - cs : CHUNK;     // values [a, b) of it
-                float z[CHUNK];
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < CHUNK; ++j) z[j] = from[j];
-                if (resid) {
-                    if (r4 != nullptr && p.resid_like_y && at >= 0 && at + CHUNK <= total) {
-#pragma unroll
-                        for (int j = 0; j < CHUNK; ++j) z[j] += bf16_bits_to_f32(j & 1 ? r4[j / 2] >> 16 : r4[j / 2] & 0xFFFFu);
-                    } else {
-                        uint32_t one[CHUNK];
-#pragma unroll
-                        for (int j = 0; j < CHUNK; ++j) one[j] = epi.resid[at + (j < a ? a : j < b ? j : b - 1)];
-#pragma unroll
-                        for (int j = 0; j < CHUNK; ++j) z[j] += bf16_bits_to_f32(one[j]);
+            // `count` < CHUNK values of this thread's token from feature c on, up to a chunk's start (`head`) or
+            // from one on: as 2, 4 and 8 bytes, each as far as it is due.
+            auto put_cut = [&](int c, int count, float* from, bool head) {
+                const int64_t at = (int64_t)row * p.n + f0 + c;
+                if (YF32) {
+                    float* to = static_cast<float*>(y) + at;
+                    const int e4 = head ? 0 : count & 2, e8 = head ? count & 1 : 0;
+                    if (count & 1) to[e4] = from[e4];
+                    if (count & 2) *reinterpret_cast<float2*>(to + e8) = make_float2(from[e8], from[e8 + 1]);
+                } else {
+                    uint16_t* to = static_cast<uint16_t*>(y) + at;
+                    const uint16_t* add = epi.resid + at;
+                    const int e2 = head ? 0 : count & 6, e4 = head ? count & 1 : count & 4, e8 = head ? count & 3 : 0;
+                    const bool wide = resid && p.resid_like_y;
+                    uint32_t r2 = 0, r4 = 0;
+                    uint2 r8 = make_uint2(0, 0);
+                    if (wide) {
+                        if (count & 1) r2 = add[e2];
+                        if (count & 2) r4 = *reinterpret_cast<const uint32_t*>(add + e4);
+                        if (count & 4) r8 = *reinterpret_cast<const uint2*>(add + e8);
+                    } else if (resid) {
+#pragma unroll 1
+                        for (int j = 0; j < count; ++j) from[j] += bf16_bits_to_f32(add[j]);
                     }
+                    auto two = [&](int e, uint32_t r) {
+                        float2 z = make_float2(from[e], from[e + 1]);
+                        if (wide) z = add2(z, make_float2(bf16_bits_to_f32(r & 0xFFFFu), bf16_bits_to_f32(r >> 16)));
+                        return pack_bf16x2(z.x, z.y);
+                    };
+                    if (count & 1) to[e2] = (uint16_t)(pack_bf16x2(wide ? from[e2] + bf16_bits_to_f32(r2) : from[e2], 0.f) & 0xFFFFu);
+                    if (count & 2) *reinterpret_cast<uint32_t*>(to + e4) = two(e4, r4);
+                    if (count & 4) *reinterpret_cast<uint2*>(to + e8) = make_uint2(two(e8, r8.x), two(e8 + 2, r8.y));
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = YF32 ? __float_as_uint(z[j]) : pack_bf16x2(z[(2 * j) % CHUNK], z[(2 * j + 1) % CHUNK]);
-                store_chunk(static_cast<uint8_t*>(y) + at * (16 / CHUNK), w, a * (8 / CHUNK), b * (8 / CHUNK));
             };
             if (resid && row0 < p.m && h0 < h1) fetch_resid(h0);
             const bool ok = __all_sync(0xffffffffu, mbar_wait_sleep(dfull + buf, (tc >> 1) & 1, abort_flag, status, 8u, 32));
@@ -551,7 +537,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                             for (int j = 0; j < 16; ++j) o[j] = mul2(o[j], *reinterpret_cast<const float2*>(sgate + 256 * buf + c + 2 * j));
                         }
                     }
-                    if (p.aligned) {
+                    if constexpr (!ANY) {
                         const int64_t at = (int64_t)row * p.n + f0 + c;
                         if (row < p.m) {
 #pragma unroll
@@ -597,11 +583,34 @@ __global__ void __launch_bounds__(kMmThreads, 1)
 #pragma unroll
                         for (int u = 0; u < LANES; ++u) {
                             const int t = TOKENS * u + lane / LANES, before = over(t), i = CHUNK * (lane % LANES);
-                            put(t, c - before + i, mine + t * p.pitch + CHUNK - before + i, &r[(4 * u) & 15]);
+                            const int cs = c - before + i;
+                            if (t < rows && cs >= h0 && cs + CHUNK <= h1) {
+                                const float* from = mine + t * p.pitch + CHUNK - before + i;
+                                const int64_t at = (int64_t)(row0 + t) * p.n + f0 + cs;
+                                float z[CHUNK];
+                                uint32_t w[4];
+#pragma unroll
+                                for (int j = 0; j < CHUNK; ++j) z[j] = from[j];
+                                if (resid) {
+#pragma unroll
+                                    for (int j = 0; j < CHUNK; ++j)
+                                        z[j] += !p.resid_like_y ? bf16_bits_to_f32(epi.resid[at + j])
+                                                : bf16_bits_to_f32(j & 1 ? r[(4 * u + j / 2) & 15] >> 16 : r[(4 * u + j / 2) & 15] & 0xFFFFu);
+                                }
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    w[j] = YF32 ? __float_as_uint(z[j]) : pack_bf16x2(z[(2 * j) % CHUNK], z[(2 * j + 1) % CHUNK]);
+                                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(y) + at * (16 / CHUNK)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
                         }
-                        if (c + 32 >= h1 && over(lane) != 0) {      // what is over of the last piece
-                            const int before = over(lane);
-                            put(lane, c + 32 - before, to + CHUNK + 32 - before, nullptr);
+                        // Of this thread's token, values before the half's first chunk, and where the last one ends.
+                        const int mine_over = over(lane), lead = -mine_over & (CHUNK - 1), end = h1 - ((h1 - h0 + mine_over) & (CHUNK - 1));
+                        if (lane < rows && lead <= h1 - h0) {
+                            if (c == h0) put_cut(h0, lead, to + CHUNK, true);
+                            if (c + 32 >= h1) put_cut(end, h1 - end, to + CHUNK + end - c, false);
+                        } else if (lane < rows) {                   // no chunk starts here
+#pragma unroll 1
+                            for (int f = h0; f < h1; ++f) put_cut(f, 1, to + CHUNK + f - h0, true);
                         }
                     }
                 }
@@ -730,14 +739,14 @@ bool byte_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int b
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool PAIR, bool SPLIT, bool FUSED, bool YF32>
+template <bool PAIR, bool SPLIT, bool FUSED, bool YF32, bool ANY>
 cudaError_t launch_mm_t(const CUtensorMap& tmX, const CUtensorMap& tmW, const uint8_t* xs, const uint8_t* ws,
                         const EpiArgs& epi, void* y, const MmPlan& p, int grid, size_t smem, cudaStream_t st) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     static bool configured[64] = {};
-    auto kernel = fp8_mm_kernel<PAIR, SPLIT, FUSED, YF32>;
+    auto kernel = fp8_mm_kernel<PAIR, SPLIT, FUSED, YF32, ANY>;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQmvMaxSmem);
         if (e != cudaSuccess) return e;
@@ -767,7 +776,7 @@ int clusters_at_once(int ctas) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
     int& n = known[dev][ctas];
     if (n == 0) {
-        auto kernel = fp8_mm_kernel<false, true, false, false>;
+        auto kernel = fp8_mm_kernel<false, true, false, false, false>;
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)(ctas * num_sms()));
         cfg.blockDim = dim3(kMmThreads);
@@ -797,7 +806,7 @@ int clusters_at_once(int ctas) {
 // pace; the last tile's, and a pair's later start or the exchange, on top.  Measured, us: 512 x 4096 x
 // 10240 pairs by 144 20.3 (CTAs by 144 21.8); 1 x 9728 x 2560 fours by 80 9.1 (CTAs by 48 15.0, twos by
 // 64 11.2, eights by 176 10.2); 16 x 8192 x 128 eights by 16 5.2 (CTAs by 64 12.2); 3116 x 48 x 4181
-// with SiLU CTAs by 224 27.6 (by 80 39.6).  Over some 45 shapes from 1 to 4608 tokens its choice was
+// with SiLU CTAs by 224 26.6 (by 80 39.6).  Over some 45 shapes from 1 to 4608 tokens its choice was
 // within 9 % of the best, mostly 4 %.
 void choose(int64_t m, int64_t n, int64_t k, bool fused, bool aligned, bool& pair, int& bn, int& split) {
     const int64_t kt = (k + kFp8Block - 1) / kFp8Block, sms = num_sms();
@@ -876,14 +885,17 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
     // More than half of an SM's shared memory, so that no second CTA waits there for tensor memory.
     size_t smem = fixed + p.stages * stage;
     if (smem < 120 * 1024) smem = 120 * 1024;
-    auto go = [&](auto pr, auto sp) {
-        constexpr bool P = decltype(pr)::value, S = decltype(sp)::value;
-        if (epi.fused()) return launch_mm_t<P, S, true, false>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
-        if (epi.f32) return launch_mm_t<P, S, false, true>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
-        return launch_mm_t<P, S, false, false>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
+    auto go = [&](auto pr, auto sp, auto any) {
+        constexpr bool P = decltype(pr)::value, S = decltype(sp)::value, A = decltype(any)::value;
+        if (epi.fused()) return launch_mm_t<P, S, true, false, A>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
+        if (epi.f32) return launch_mm_t<P, S, false, true, A>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
+        return launch_mm_t<P, S, false, false, A>(tmX, tmW, xs, ws, epi, y, p, grid, smem, st);
     };
-    if (pair) return go(std::true_type{}, std::false_type{});
-    return p.split > 1 ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (p.split > 1) return go(No{}, Yes{}, No{});
+    if (pair) return p.aligned ? go(Yes{}, No{}, No{}) : go(Yes{}, No{}, Yes{});
+    return p.aligned ? go(No{}, No{}, No{}) : go(No{}, No{}, Yes{});
 }
 
 cudaError_t read_and_clear_fp8_status(unsigned int* out, cudaStream_t st) {
