@@ -411,8 +411,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         // Rows that do not start on 32 bytes: the warp turns 32 tokens x 32 features around in shared
         // memory, and a lane stores a chunk, the CHUNK values of an aligned 16 bytes of y; LANES lanes
         // take a token's piece.  What is over of a piece (row t's chunks start `over` values before
-        // feature c) waits for the next one in front of it.  Values of chunks that the half's ends cut are
-        // stored one by one, a lane a token.  (All of it by 2 bytes a lane, 64 bytes of a token a warp,
+        // feature c) waits for the next one in front of it.  What the half's ends leave of a chunk is
+        // stored by a lane a token.  (All of it by 2 bytes a lane, 64 bytes of a token a warp,
         // took much longer: 3907 x 320 x 8597 with gate and residual 112 us, 66 this way.)
         constexpr int CHUNK = YF32 ? 4 : 8, LANES = 32 / CHUNK, TOKENS = 32 / LANES;
         float* mine = stage32 + (warp - 8) * 32 * kMaxPitch;

@@ -86,9 +86,16 @@ def indexed(name: str) -> bool:
             or name == "lm_head.weight")
 
 
+def _known(bits: Bits) -> None:
+    if isinstance(bits, str) and bits != FP8:
+        raise SdqError(SDQ_ERR_INVALID, f"weights are held at a bit width or as {FP8!r}, not as {bits!r}")
+
+
 def mixed(bits: Bits) -> Callable[[str], Bits]:
     """Default policy: indexed dense (0), sensitive 8, the rest ``bits`` (quantized.rs:156-166),
     which may be :data:`FP8`."""
+    _known(bits)
+
     def f(name: str) -> Bits:
         if indexed(name):
             return 0
@@ -111,6 +118,7 @@ def fp8_quantizable(shape) -> bool:
 def quantize_to(w: torch.Tensor, bits: Bits, stream=None) -> Union[QuantizedArray, Fp8Array, None]:
     """``w`` as a policy's ``bits`` say: affine at 4 or 8 bits, :data:`FP8`, or None for a tensor that
     stays dense (0, or a shape that the form does not take)."""
+    _known(bits)
     if bits == FP8:
         return Fp8Array.quantize(w.contiguous(), stream) if fp8_quantizable(tuple(w.shape)) else None
     if bits >= 2 and quantizable(tuple(w.shape)):

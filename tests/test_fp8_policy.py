@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import pytest
 
+import sdq
 from sdq import quantized as Q
 
 
@@ -17,6 +18,14 @@ def test_mixed_gives_fp8_to_the_ordinary_layers_only():
                                         ((2, 4, 16), False), ((0, 16), False), ((4, 0), False)])
 def test_shapes_that_fp8_takes(shape, fits):
     assert Q.fp8_quantizable(shape) is fits
+
+
+def test_another_name_is_refused():
+    import torch
+    with pytest.raises(sdq.SdqError, match="'int8'"):
+        Q.mixed("int8")
+    with pytest.raises(sdq.SdqError, match="'FP8'"):
+        Q.from_dense_with({"a.weight": torch.zeros(2, 64)}, lambda name: "FP8")
 
 
 def test_a_policy_keeps_unfit_tensors_dense():

@@ -312,6 +312,23 @@ def test_two_streams_at_once():
         assert all(torch.equal(y, w) for y in g)
 
 
+def test_beside_the_affine_kernels_on_another_stream():
+    """Both take an SM's tensor memory: whichever comes second waits for it."""
+    w, x = normals(40, 2048, 1024), normals(41, 700, 1024).to(torch.bfloat16)
+    affine, fp8 = sdq.QuantizedArray.quantize(w), sdq.Fp8Array.quantize(w)
+    want = affine.matmul(x), fp8.matmul(x), affine.matmul(x[:4]), fp8.matmul(x[:4])
+    streams = [torch.cuda.Stream() for _ in want]
+    torch.cuda.synchronize()
+    got = [[] for _ in want]
+    for _ in range(10):
+        for g, a, v, st in zip(got, (affine, fp8) * 2, (x, x, x[:4], x[:4]), streams):
+            g.append(a.matmul(v, stream=st))
+    torch.cuda.synchronize()
+    sdq.device_status()
+    for g, y in zip(got, want):
+        assert all(torch.equal(v, y) for v in g)
+
+
 def test_empty_batch():
     wq, ws = sdq.fp8_quantize_weight(normals(1, 64, 128))
     x = torch.empty(0, 128, device="cuda", dtype=torch.bfloat16)
