@@ -16,7 +16,7 @@
 //
 // Where the tiles leave SMs idle and K is long, a cluster of 2, 4 or 8 CTAs shares one tile's K (SPLIT):
 // each accumulates its steps, then they exchange pieces of 16 features through one another's shared
-// memory, each adding up (in the order of K) and storing its own.  1 x 9728 x 2560: 15.0 -> 9.1 us.
+// memory, each adding up (in the order of K) and storing its own.  1 x 9728 x 2560: 15.0 -> 9.0 us.
 //
 // One kernel for every number of tokens.  For a few of them a stream of the weight through mma.sync
 // was measured beside it and is not kept: its e4m3 form is emulated on sm_100a (170 cycles each), and
@@ -658,18 +658,39 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                 }
             }
         }
+        // Its own pieces; the residual of the first is on its way while the others' sums arrive.  Where rows
+        // do not start on 32 bytes, a warp turns its 32 tokens x 16 features around, so that 16 lanes
+        // load and store a token's features side by side (a lane a token: 2 to 4 us more).
+        const bool resid = FUSED && epi.resid != nullptr;
+        uint32_t r[16];
+        auto fetch_resid = [&](int piece) {
+            const int f = f0 + 16 * piece;
+            if (p.aligned) {
+                if (row < p.m) ld_global_32(reinterpret_cast<uint32_t(&)[8]>(r[0]), epi.resid + (int64_t)row * p.n + f);
+            } else {
+                const uint16_t* from = epi.resid + (f + (lane & 15) < p.n ? f + (lane & 15) : p.n - 1);
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    const int t = row0 + 2 * u + (lane >> 4);
+                    r[u] = from[(int64_t)(t < p.m ? t : p.m - 1) * p.n];
+                }
+            }
+        };
+        const int mine = (share & 1) == e ? share : width;              // S is even: one group has them all
+        const bool there = warp >= 8 && complete && row0 < p.m;
+        float* turned = stage32 + (warp - 8) * 32 * kMaxPitch;          // pitch 17
+        if (resid && there && 16 * mine < width) fetch_resid(mine);
         cluster_sync();
-        if (warp >= 8 && complete && row0 < p.m) {
-            for (int piece = e; 16 * piece < width; piece += 2) {
-                if (piece % S != share) continue;
+        if (there) {
+            for (int piece = mine; 16 * piece < width; piece += S) {
                 uint32_t v[16];
                 __syncwarp();
                 tmem_ld16(acc + 16 * piece, v);
                 tc_wait_ld();
-                if (row >= p.m) continue;
-                float a[16];
+                if (resid && piece != mine) fetch_resid(piece);
+                float2 o[8];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) a[j] = 0.f;
+                for (int j = 0; j < 8; ++j) o[j] = make_float2(0.f, 0.f);
                 for (int from = 0; from < S; ++from) {
                     const float4* at = reinterpret_cast<const float4*>(smem + slot_of(from, piece)) + token;
 #pragma unroll
@@ -677,39 +698,61 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                         const float4 z = from == share ? make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]),
                                                                      __uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3]))
                                                        : at[q * kTokens];
-                        a[4 * q] += z.x; a[4 * q + 1] += z.y; a[4 * q + 2] += z.z; a[4 * q + 3] += z.w;
+                        o[2 * q] = add2(o[2 * q], make_float2(z.x, z.y));
+                        o[2 * q + 1] = add2(o[2 * q + 1], make_float2(z.z, z.w));
                     }
                 }
-                const int64_t to = (int64_t)row * p.n + f0 + 16 * piece;
-                uint32_t o[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int i = 16 * piece + j;
-                    float z = a[j] + sbias[i];
-                    if (YF32) {
-                        o[j] = __float_as_uint(z);
-                    } else {
-                        if (FUSED) {
-                            z = epi_activation(z, epi.act) * sgate[i];
-                            if (epi.resid != nullptr && f0 + i < p.n) z += bf16_bits_to_f32(epi.resid[to + j]);
-                        }
-                        if (j & 1) o[j / 2] = pack_bf16x2(__uint_as_float(o[j / 2]), z);
-                        else o[j / 2] = __float_as_uint(z);
+                for (int j = 0; j < 8; ++j) o[j] = add2(o[j], *reinterpret_cast<const float2*>(sbias + 16 * piece + 2 * j));
+                if (FUSED) {
+                    if (epi.act == SDQ_ACT_GELU_TANH) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) o[j] = gelu2(o[j]);
+                    } else if (epi.act == SDQ_ACT_SILU) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) o[j] = silu2(o[j]);
+                    }
+                    if (epi.gate != nullptr) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) o[j] = mul2(o[j], *reinterpret_cast<const float2*>(sgate + 16 * piece + 2 * j));
                     }
                 }
                 if (p.aligned) {
+                    if (row >= p.m) continue;
+                    const int64_t to = (int64_t)row * p.n + f0 + 16 * piece;
+                    uint32_t w[16];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (resid) o[j] = add2(o[j], make_float2(bf16_bits_to_f32(r[j] & 0xFFFFu), bf16_bits_to_f32(r[j] >> 16)));
+                        if (YF32) { w[2 * j] = __float_as_uint(o[j].x); w[2 * j + 1] = __float_as_uint(o[j].y); }
+                        else w[j] = pack_bf16x2(o[j].x, o[j].y);
+                    }
                     if (YF32) {
-                        st_global_32(static_cast<float*>(y) + to, reinterpret_cast<uint32_t(&)[8]>(o[0]));
-                        st_global_32(static_cast<float*>(y) + to + 8, reinterpret_cast<uint32_t(&)[8]>(o[8]));
+                        st_global_32(static_cast<float*>(y) + to, reinterpret_cast<uint32_t(&)[8]>(w[0]));
+                        st_global_32(static_cast<float*>(y) + to + 8, reinterpret_cast<uint32_t(&)[8]>(w[8]));
                     } else {
-                        st_global_32(static_cast<uint16_t*>(y) + to, reinterpret_cast<uint32_t(&)[8]>(o[0]));
+                        st_global_32(static_cast<uint16_t*>(y) + to, reinterpret_cast<uint32_t(&)[8]>(w[0]));
                     }
                 } else {
+                    __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if (f0 + 16 * piece + j >= p.n) break;
-                        if (YF32) static_cast<uint32_t*>(y)[to + j] = o[j];
-                        else static_cast<uint16_t*>(y)[to + j] = (uint16_t)(j & 1 ? o[j / 2] >> 16 : o[j / 2] & 0xFFFFu);
+                    for (int j = 0; j < 8; ++j) {
+                        turned[17 * lane + 2 * j] = o[j].x;
+                        turned[17 * lane + 2 * j + 1] = o[j].y;
+                    }
+                    __syncwarp();
+                    if ((lane & 15) < width - 16 * piece) {
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            const int t = 2 * u + (lane >> 4);
+                            const int64_t to = (int64_t)(row0 + t) * p.n + f0 + 16 * piece + (lane & 15);
+                            if (row0 + t < p.m) {
+                                float z = turned[17 * t + (lane & 15)];
+                                if (resid) z += bf16_bits_to_f32(r[u]);
+                                if (YF32) static_cast<float*>(y)[to] = z;
+                                else static_cast<uint16_t*>(y)[to] = (uint16_t)(pack_bf16x2(z, 0.f) & 0xFFFFu);
+                            }
+                        }
                     }
                 }
             }
@@ -804,10 +847,10 @@ int clusters_at_once(int ctas) {
 // beside them, a tile behind, the output stage (750 cycles for 64 features, as much again for an
 // activation, gate or residual, 1000 more for rows of any pitch), which of many short tiles sets the
 // pace; the last tile's, and a pair's later start or the exchange, on top.  Measured, us: 512 x 4096 x
-// 10240 pairs by 144 20.3 (CTAs by 144 21.8); 1 x 9728 x 2560 fours by 80 9.1 (CTAs by 48 15.0, twos by
-// 64 11.2, eights by 176 10.2); 16 x 8192 x 128 eights by 16 5.2 (CTAs by 64 12.2); 3116 x 48 x 4181
-// with SiLU CTAs by 224 26.6 (by 80 39.6).  Over some 45 shapes from 1 to 4608 tokens its choice was
-// within 9 % of the best, mostly 4 %.
+// 10240 pairs by 144 20.3 (CTAs by 144 21.8); 1 x 9728 x 2560 fours by 80 9.0 (CTAs by 32 15.0, twos by
+// 48 11.3, eights by 176 9.8); 16 x 8192 x 128 eights by 16 5.2 (CTAs by 64 12.2); 3116 x 48 x 4181
+// with SiLU CTAs by 224 26.6 (by 80 39.6).  Over some 60 shapes from 1 to 4608 tokens its choice was
+// within 5 % of the best, mostly 2 %.
 void choose(int64_t m, int64_t n, int64_t k, bool fused, bool aligned, bool& pair, int& bn, int& split) {
     const int64_t kt = (k + kFp8Block - 1) / kFp8Block, sms = num_sms();
     const int64_t dram = n * k / 3500;
@@ -828,11 +871,13 @@ void choose(int64_t m, int64_t n, int64_t k, bool fused, bool aligned, bool& pai
                 bn = w;
                 split = 1;
             }
-            // Shared tiles: all clusters at once, a step at least for every CTA, and the exchange.
+            // Shared tiles: all clusters at once, a step at least for every CTA, its own pieces of 16
+            // features and the exchange.
             for (int s = 2; cg == 1 && s <= 8 && s <= kt; s *= 2) {
                 if (tiles > clusters_at_once(s)) break;
                 const int64_t steps = (kt + s - 1) / s * step, exchange = 3000 + 150 * s + w * (15 + x_rows / 12);
-                const int64_t shared = (steps > dram ? steps : dram) + out + exchange;
+                const int64_t own = 900 + (w / 16 + s - 1) / s * (500 + (fused ? 250 : 0) + (aligned ? 0 : 300));
+                const int64_t shared = (steps > dram ? steps : dram) + own + exchange;
                 if (shared < best) {
                     best = shared;
                     pair = false;
