@@ -224,6 +224,27 @@ def test_nan_stays_in_its_row_and_its_features(m):
     assert nan[:, 128:256].all() and nan.sum() == m * 128
 
 
+@pytest.mark.parametrize("act", [None, "silu", "gelu_approx"])
+@pytest.mark.parametrize("m,k,n", [(40, 144, 320), (40, 144, 77), (8, 8192, 64), (8, 8192, 51)])
+def test_one_feature_out_of_range(m, k, n, act):
+    """A NaN, an infinity and numbers near f32's end in the bias: each in its own feature.  SiLU of
+    numbers far below 0 is 0 (to 2^-50), of numbers far above themselves."""
+    ops = operands(m + k, m, k, n)
+    bias = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    free = sdq.fp8_matmul(*ops, bias=bias, act=act)
+    odd = {3: float("nan"), 6: float("inf"), 9: -3e38, 12: 3e38, 16: -100.0, 21: float("nan")}
+    big = float(product(*ops)[0].abs().max())
+    for f, v in odd.items():
+        bias[f] = v if v != -100.0 else -100.0 - 2 * big
+    y = sdq.fp8_matmul(*ops, bias=bias, act=act)
+    rest = [f for f in range(n) if f not in odd]
+    assert torch.equal(y[:, rest], free[:, rest])
+    assert y[:, [3, 21]].isnan().all() and (y[:, 6] == float("inf")).all() and (y[:, 12] > 2.9e38).all()
+    if act:
+        assert (y[:, [9, 16]].abs() <= 2.0 ** -50).all()
+    sdq.device_status()
+
+
 @pytest.mark.parametrize("m", [1, 5, 20, 300])
 def test_nothing_beside_the_result_is_written(m):
     """Sentinels around y, odd n (an unaligned pitch) and a y that starts off 16 bytes."""
