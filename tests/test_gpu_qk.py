@@ -60,6 +60,8 @@ CASES = [  # b, n, heads, kv heads, d, rope
     (1, 2, 100, 100, 128, 64),
     # fewer heads than fit a warp: several tokens side by side, the last of them not there
     (3, 37, 1, 1, 32, 32), (2, 5, 3, 1, 16, 16), (1, 9, 9, 1, 64, 64), (5, 3, 2, 2, 8, 0), (1, 41, 33, 1, 32, 16),
+    # two and three rounds of a warp's heads
+    (3, 37, 4, 2, 96, 48), (1, 21, 7, 1, 64, 64), (2, 9, 2, 1, 256, 256), (1, 17, 6, 3, 128, 64),
 ]
 
 
