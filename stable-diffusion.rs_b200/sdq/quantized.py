@@ -8,6 +8,7 @@ the same errors, with `QuantizedArray` backed by libsdq instead of MLX.  Dense
 """
 from __future__ import annotations
 
+import contextlib
 from typing import Callable, Dict, Mapping, Optional, Protocol, Union
 
 import torch
@@ -115,14 +116,36 @@ def fp8_quantizable(shape) -> bool:
     return len(shape) == 2 and shape[0] > 0 and shape[1] > 0 and shape[1] % 16 == 0
 
 
+@contextlib.contextmanager
+def _on(stream, device: torch.device):
+    """``device`` current and, where it is not None, ``stream`` (a torch stream or a raw handle).  What a
+    loader copies, allocates and drops between its kernels then belongs to the stream that these run on:
+    the allocator hands a dropped block on at once, in the order of that stream."""
+    if device.type != "cuda":
+        yield
+        return
+    with torch.cuda.device(device):
+        if stream is None:
+            yield
+            return
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(int(stream))
+        if stream.device_index != torch.cuda.current_device():
+            raise SdqError(SDQ_ERR_INVALID, f"a stream of {stream.device} cannot run work on {device}")
+        with torch.cuda.stream(stream):
+            yield
+
+
 def quantize_to(w: torch.Tensor, bits: Bits, stream=None) -> Union[QuantizedArray, Fp8Array, None]:
     """``w`` as a policy's ``bits`` say: affine at 4 or 8 bits, :data:`FP8`, or None for a tensor that
-    stays dense (0, or a shape that the form does not take)."""
+    stays dense (0, or a shape that the form does not take).  With a ``stream`` all of it, a copy of a
+    ``w`` that is not contiguous among it, runs and allocates there."""
     _known(bits)
-    if bits == FP8:
-        return Fp8Array.quantize(w.contiguous(), stream) if fp8_quantizable(tuple(w.shape)) else None
-    if bits >= 2 and quantizable(tuple(w.shape)):
-        return QuantizedArray.quantize(w.contiguous(), GROUP_SIZE, bits, stream)
+    with _on(stream, w.device):
+        if bits == FP8:
+            return Fp8Array.quantize(w.contiguous()) if fp8_quantizable(tuple(w.shape)) else None
+        if bits >= 2 and quantizable(tuple(w.shape)):
+            return QuantizedArray.quantize(w.contiguous(), GROUP_SIZE, bits)
     return None
 
 
@@ -143,7 +166,8 @@ def from_dense_with(w: Mapping[str, torch.Tensor], bits_for: Callable[[str], Bit
         if q is not None:
             quantized[name] = q
         else:
-            dense[name] = array.contiguous()
+            with _on(stream, array.device):
+                dense[name] = array.contiguous()
     return QuantizedWeights(quantized, dense)
 
 
@@ -152,7 +176,8 @@ def from_gguf(path: str, bits: Bits, device=None, stream=None) -> QuantizedWeigh
     (quantized.rs:180-211).  One tensor at a time: its raw block bytes are copied to the
     device and either quantised there straight from the block format (``sdq.gguf_quantize``)
     or dequantised to a dense f32 tensor, which for :data:`FP8` is then quantised; nothing else of
-    the file is held meanwhile."""
+    the file is held meanwhile.  With a ``stream`` the uploads and kernels run, and every tensor is
+    allocated, there."""
     return _load_gguf(path, bits, None, device, stream)
 
 
@@ -172,27 +197,28 @@ def _load_gguf(path, bits, rename, device, stream) -> QuantizedWeights:
     quantized: Dict[str, Union[QuantizedArray, Fp8Array]] = {}
     dense: Weights = {}
     policy = mixed(bits)
-    for info in g.tensors:
-        name = info.name if rename is None else rename(info.name)
-        if name is None:
-            continue
-        raw = torch.from_numpy(g.raw(info)).to(dev)         # the peak: one tensor's blocks
-        want = policy(name)
-        if want == FP8:
-            array = gguf_dequantize(raw, info.kind, info.shape, torch.float32, stream)
-            q = quantize_to(array, FP8, stream)
-            if q is not None:
-                quantized[name] = q
+    with _on(stream, dev):
+        for info in g.tensors:
+            name = info.name if rename is None else rename(info.name)
+            if name is None:
+                continue
+            raw = torch.from_numpy(g.raw(info)).to(dev)     # the peak: one tensor's blocks
+            want = policy(name)
+            if want == FP8:
+                array = gguf_dequantize(raw, info.kind, info.shape, torch.float32)
+                q = quantize_to(array, FP8)
+                if q is not None:
+                    quantized[name] = q
+                else:
+                    dense[name] = array
+                del array
+            elif want >= 2 and quantizable(info.shape):
+                n, k = info.shape
+                wq, s, b = gguf_quantize(raw, info.kind, n, k, want, GROUP_SIZE)
+                quantized[name] = QuantizedArray(wq, s, b, GROUP_SIZE, want)
             else:
-                dense[name] = array
-            del array
-        elif want >= 2 and quantizable(info.shape):
-            n, k = info.shape
-            wq, s, b = gguf_quantize(raw, info.kind, n, k, want, GROUP_SIZE, stream)
-            quantized[name] = QuantizedArray(wq, s, b, GROUP_SIZE, want)
-        else:
-            dense[name] = gguf_dequantize(raw, info.kind, info.shape, torch.float32, stream)
-        del raw
+                dense[name] = gguf_dequantize(raw, info.kind, info.shape, torch.float32)
+            del raw
     if not quantized and not dense:
         raise SdqError(SDQ_ERR_INVALID, f"gguf: {path} carries no tensors"
                        + ("" if rename is None else " this model recognises"))
