@@ -329,6 +329,14 @@ int sdq_device_status(void* stream);
 int sdq_debug_wait_hook(uint64_t wait_limit_ns, int withhold_first_copy, void* stream);
 
 /*
+ * How sdq_fp8_matmul would run a product on the current device, for tests that have to reach each of its
+ * forms; runs nothing.  fused: an activation, a gate or a residual; aligned: n is a multiple of 16, and y
+ * and the residual start on 32 bytes.  plan[0] CTAs a tile's pair (1 or 2), [1] CTAs that share a tile's
+ * k, [2] features a tile, [3] tiles, [4] tiles at work at once, [5] token tiles walked together.
+ */
+int sdq_debug_fp8_plan(int64_t m, int64_t k, int64_t n, int fused, int aligned, int32_t* plan);
+
+/*
  * Communicators for the column-sharded linear.  The library owns its NCCL
  * communicator, so no NCCL type crosses the ABI: rank 0 calls
  * sdq_comm_unique_id, shares the 128 bytes with the other ranks by any means

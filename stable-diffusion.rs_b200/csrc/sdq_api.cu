@@ -714,6 +714,20 @@ int sdq_debug_wait_hook(uint64_t wait_limit_ns, int withhold_first_copy, void* s
     return ok();
 }
 
+int sdq_debug_fp8_plan(int64_t m, int64_t k, int64_t n, int fused, int aligned_rows, int32_t* plan) {
+    const char* fn = "sdq_debug_fp8_plan";
+    int rc;
+    if ((rc = check_fp8_shape(m, k, "m (rows of x)", 1, fn)) || (rc = check_fp8_shape(n, k, "n (rows, out features)", 1, fn)))
+        return rc;
+    if (!plan) return fail(SDQ_ERR_INVALID, "%s: plan must be non-null", fn);
+    if (aligned_rows && n % 16 != 0) return fail(SDQ_ERR_INVALID, "%s: rows of %lld values are not aligned", fn, (long long)n);
+    if ((rc = check_device())) return rc;
+    int32_t out[6];
+    fp8_mm_plan(m, k, n, fused != 0, aligned_rows != 0, out);
+    for (int i = 0; i < 6; ++i) plan[i] = out[i];
+    return ok();
+}
+
 int sdq_device_status(void* stream) {
     int rc;
     if ((rc = check_device())) return rc;

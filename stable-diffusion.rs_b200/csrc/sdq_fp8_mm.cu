@@ -59,6 +59,7 @@ constexpr int kMaxPitch = 43;                      // words per token of a warp'
 constexpr int kFixedSmem = 1024 /* alignment */ + 512 /* barriers */ + 4 * 256 * 4 /* two tiles' bias and gate */ +
                            kSlots * kCells;
 constexpr int kTransposeSmem = 8 * 32 * kMaxPitch * 4;
+constexpr size_t fixed_smem(bool aligned) { return kFixedSmem + (aligned ? 0 : kTransposeSmem); }
 
 // Quotients of numbers below 2^31 by a settled divisor d, 2^(l-1) < d <= 2^l: n / d is the upper half of
 // n * ceil(2^(31+l) / d), l - 1 places down.  (A tile's place took 400 cycles by division.)
@@ -893,28 +894,22 @@ void choose(int64_t m, int64_t n, int64_t k, bool fused, bool aligned, bool& pai
     }
 }
 
-}  // namespace
-
-cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t k, const uint8_t* wq,
-                          const uint8_t* ws, int64_t n, const EpiArgs& epi, void* y, cudaStream_t st,
-                          const char** msg) {
+// All that a launch depends on but its pointers; `aligned` as in MmPlan.  grid: CTAs.
+MmPlan plan_for(int64_t m, int64_t n, int64_t k, bool fused, bool aligned, bool& pair, int& grid) {
     MmPlan p{};
-    bool pair = false;
-    const uintptr_t bases = reinterpret_cast<uintptr_t>(y) | (epi.resid ? reinterpret_cast<uintptr_t>(epi.resid) : 0);
-    p.aligned = n % 16 == 0 && bases % 32 == 0;
-    choose(m, n, k, epi.fused(), p.aligned, pair, p.bn, p.split);
+    p.aligned = aligned;
+    choose(m, n, k, fused, aligned, pair, p.bn, p.split);
     const int cg = pair ? 2 : 1;
     p.m = (int)m;
     p.n = (int)n;
     p.k = (int)k;
     p.kt = (int)((k + kFp8Block - 1) / kFp8Block);
     p.x_rows = m < kTokens ? (int)((m + 7) / 8 * 8) : kTokens;
-    p.resid_like_y = (reinterpret_cast<uintptr_t>(y) - reinterpret_cast<uintptr_t>(epi.resid)) % 16 == 0;
     // Odd, so that a lane a token writes without bank conflicts; lanes that read a chunk each, of rows
     // whose chunks start n values further back each time, then meet in pairs at most.
     p.pitch = n % 4 == 1 ? kMaxPitch : kMaxPitch - 2;
-    const size_t fixed = kFixedSmem + (p.aligned ? 0 : kTransposeSmem), stage = kXStage + (size_t)(p.bn / cg) * kFp8Block;
-    const int fit = (int)((kQmvMaxSmem - fixed) / stage);
+    const size_t stage = kXStage + (size_t)(p.bn / cg) * kFp8Block;
+    const int fit = (int)((kQmvMaxSmem - fixed_smem(aligned)) / stage);
     p.stages = fit < kMaxStages ? fit : kMaxStages;
     const int64_t nft = (n + p.bn - 1) / p.bn, ntt = (m + cg * kTokens - 1) / (cg * kTokens), tiles = nft * ntt;
     p.nft = (int)nft;
@@ -925,14 +920,28 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
     p.by_group = Divisor((uint32_t)p.group);
     p.by_rest = Divisor((uint32_t)(ntt % p.group ? ntt % p.group : p.group));
     const int64_t places = num_sms() / cg;
-    const int grid = p.split > 1 ? (int)tiles * p.split : (int)(tiles < places ? tiles : places) * cg;
+    grid = p.split > 1 ? (int)tiles * p.split : (int)(tiles < places ? tiles : places) * cg;
+    return p;
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t k, const uint8_t* wq,
+                          const uint8_t* ws, int64_t n, const EpiArgs& epi, void* y, cudaStream_t st,
+                          const char** msg) {
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(y) | (epi.resid ? reinterpret_cast<uintptr_t>(epi.resid) : 0);
+    bool pair = false;
+    int grid = 0;
+    MmPlan p = plan_for(m, n, k, epi.fused(), n % 16 == 0 && bases % 32 == 0, pair, grid);
+    p.resid_like_y = (reinterpret_cast<uintptr_t>(y) - reinterpret_cast<uintptr_t>(epi.resid)) % 16 == 0;
     CUtensorMap tmX, tmW;
-    if (!byte_map(&tmX, xq, m, k, p.x_rows) || !byte_map(&tmW, wq, n, k, p.bn / cg)) {
+    const int w_rows = p.bn / (pair ? 2 : 1);
+    if (!byte_map(&tmX, xq, m, k, p.x_rows) || !byte_map(&tmW, wq, n, k, w_rows)) {
         *msg = "cuTensorMapEncodeTiled rejected an fp8 operand's tensor map";
         return cudaErrorInvalidValue;
     }
     // More than half of an SM's shared memory, so that no second CTA waits there for tensor memory.
-    size_t smem = fixed + p.stages * stage;
+    size_t smem = fixed_smem(p.aligned) + (size_t)p.stages * (kXStage + w_rows * kFp8Block);
     if (smem < 120 * 1024) smem = 120 * 1024;
     auto go = [&](auto pr, auto sp, auto any) {
         constexpr bool P = decltype(pr)::value, S = decltype(sp)::value, A = decltype(any)::value;
@@ -945,6 +954,15 @@ cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64
     if (p.split > 1) return go(No{}, Yes{}, No{});
     if (pair) return p.aligned ? go(Yes{}, No{}, No{}) : go(Yes{}, No{}, Yes{});
     return p.aligned ? go(No{}, No{}, No{}) : go(No{}, No{}, Yes{});
+}
+
+void fp8_mm_plan(int64_t m, int64_t k, int64_t n, bool fused, bool aligned, int32_t (&out)[6]) {
+    bool pair = false;
+    int grid = 0;
+    const MmPlan p = plan_for(m, n, k, fused, aligned, pair, grid);
+    const int ctas = pair ? 2 : p.split;
+    const int32_t v[6] = {pair ? 2 : 1, p.split, p.bn, p.nft * p.ntt, grid / ctas, p.group};
+    for (int i = 0; i < 6; ++i) out[i] = v[i];
 }
 
 cudaError_t read_and_clear_fp8_status(unsigned int* out, cudaStream_t st) {

@@ -119,6 +119,9 @@ cudaError_t launch_fp8_dequantize(const uint8_t* q, const uint8_t* scales, int64
 cudaError_t launch_fp8_mm(const uint8_t* xq, const uint8_t* xs, int64_t m, int64_t k, const uint8_t* wq,
                           const uint8_t* ws, int64_t n, const EpiArgs& epi, void* y, cudaStream_t st,
                           const char** msg);
+// How it would be run: CTAs a tile's pair, CTAs that share its K, features a tile, tiles, tiles at work at
+// once, token tiles walked together.
+void fp8_mm_plan(int64_t m, int64_t k, int64_t n, bool fused, bool aligned, int32_t (&out)[6]);
 // Queries, keys and values made ready for attention (sdq_qk.cu).  Strides in elements; the last
 // axis is contiguous.  heads[i] == 0 leaves tensor i out; weight == nullptr skips the norm,
 // rope == 0 the rotation.

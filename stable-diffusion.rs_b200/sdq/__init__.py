@@ -391,5 +391,5 @@ def quantized_matmul_sharded(x, wq, scales, biases, comm: Comm, group_size: int 
     return (out if permute else None), y_shards
 
 
-from .fp8 import Fp8Array, fp8_dequantize, fp8_matmul, fp8_quantize, fp8_quantize_weight  # noqa: E402
+from .fp8 import Fp8Array, debug_fp8_plan, fp8_dequantize, fp8_matmul, fp8_quantize, fp8_quantize_weight  # noqa: E402
 from .heads import qk_norm_rope  # noqa: E402

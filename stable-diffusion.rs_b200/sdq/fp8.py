@@ -13,6 +13,7 @@ results are allocated on it.
 """
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -165,6 +166,13 @@ def fp8_matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.T
                                None if gate is None else gate.data_ptr(),
                                None if residual is None else residual.data_ptr(), out.data_ptr(), _SOURCE[dtype], _raw_stream(dev)))
     return out
+
+
+def debug_fp8_plan(m: int, k: int, n: int, fused: bool = False, aligned: bool = True) -> dict:
+    """How :func:`fp8_matmul` would run on the current device (``sdq_debug_fp8_plan``), for tests."""
+    plan = (ctypes.c_int32 * 6)()
+    check(lib().sdq_debug_fp8_plan(m, k, n, int(bool(fused)), int(bool(aligned)), plan))
+    return dict(zip(("pair", "split", "features", "tiles", "at_once", "group"), plan))
 
 
 @dataclass

@@ -97,3 +97,11 @@ def test_no_cpu_fallback():
     for call in (lambda: sdq.fp8_quantize(x), lambda: sdq.fp8_quantize_weight(x), lambda: sdq.Fp8Array.quantize(x)):
         with pytest.raises(sdq.SdqError, match="no CPU fallback"):
             call()
+
+
+def test_plan_refusals():
+    for args, needle in (((0, 128, 64), "m (rows of x)"), ((4, 0, 64), "k must be"), ((4, 120, 64), "multiple of 16"), ((4, 128, 0), "n (rows"),
+                         ((4, 128, 60), "not aligned")):
+        with pytest.raises(sdq.SdqError) as e:
+            sdq.debug_fp8_plan(*args)
+        assert e.value.code == _abi.SDQ_ERR_INVALID and needle in str(e.value)
