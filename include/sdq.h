@@ -323,7 +323,10 @@ int sdq_device_status(void* stream);
  * first copy and the arrival that goes with it, so the consumers' wait on that
  * stage runs out: the kernel then records its status bit, lets the copies it
  * did start land, frees its tensor memory and returns, and sdq_device_status
- * reports SDQ_ERR_TIMEOUT.  Settings hold for the current device until changed.
+ * reports SDQ_ERR_TIMEOUT.  The fp8 kernel does the same; with 2 or 3, where it
+ * runs a tile on a pair of CTAs, the second's or the first's producer starts
+ * nothing at all, so that the two stop at different steps (elsewhere as 1).
+ * Settings hold for the current device until changed.
  * Synchronises `stream`.  No counterpart in the reference.
  */
 int sdq_debug_wait_hook(uint64_t wait_limit_ns, int withhold_first_copy, void* stream);

@@ -706,7 +706,7 @@ int sdq_debug_wait_hook(uint64_t wait_limit_ns, int withhold_first_copy, void* s
     int rc;
     if ((rc = check_device())) return rc;
     const unsigned long long lim = wait_limit_ns == 0 ? 2000000000ull : wait_limit_ns;
-    const int wh = withhold_first_copy != 0;
+    const int wh = withhold_first_copy == 2 || withhold_first_copy == 3 ? withhold_first_copy : withhold_first_copy != 0;
     cudaError_t e = set_wait_hook_tc(lim, wh, static_cast<cudaStream_t>(stream));
     if (e == cudaSuccess) e = set_wait_hook_qmv(lim, wh, static_cast<cudaStream_t>(stream));
     if (e == cudaSuccess) e = set_wait_hook_fp8(lim, wh, static_cast<cudaStream_t>(stream));

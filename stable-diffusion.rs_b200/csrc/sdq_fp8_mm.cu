@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     uint64_t* drain = dempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* started = reinterpret_cast<int*>(tmem_slot + 2);       // steps whose copies this CTA has issued
     float* sbias = reinterpret_cast<float*>(bars + 64);         // [2][256], a tile's in turn
     float* sgate = sbias + 512;                                 // [2][256]
     // [slots][3 column quads][32 lanes][4 columns][4 steps], X's quad first
@@ -172,6 +173,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     unsigned int* status = &g_fp8_status;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_rank() : 0;
+    const int hook = g_withhold_first_copy;      // testing hook, normally 0; read here, where nothing waits for it yet
+    const bool withhold = PAIR ? hook == 1 : hook != 0;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) { mbar_init(full + i, 1); mbar_init(done + i, 1); }
@@ -246,8 +249,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             const uint32_t full0 = PAIR ? cluster_addr(full, 0) : 0;
             int it = 0, s = 0;
             uint32_t phase = 1;
-            bool ok = true;
-            const bool withhold = g_withhold_first_copy != 0;      // testing hook, normally false
+            bool ok = !(PAIR && hook == (rank == 0 ? 3 : 2));
             for (int tile = first; ok && tile < ntiles; tile += stride) {
                 int ft, tt;
                 place(tile, ft, tt);
@@ -269,18 +271,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                     if (++s == p.stages) { s = 0; phase ^= 1; }
                 }
             }
-            // After an abort no copy may outlive shared memory: the last steps started are waited
-            // for, by rank 0 for both CTAs of a pair (its peer waits at the end of the kernel), and
-            // so is the one that the peer alone may have started.
-            if (!ok && rank == 0) {
-                bool landed = true;
-                for (int j = it < p.stages ? 0 : it - p.stages; j < it; ++j)
-                    landed = !(withhold && j == 0) && mbar_wait_drain(full + j % p.stages, (uint32_t)((j / p.stages) & 1)) && landed;
-                if (PAIR && landed) {
-                    mbar_arrive_expect_tx(full + s, my_bytes);
-                    mbar_wait_drain(full + s, (uint32_t)((it / p.stages) & 1));
-                }
-            }
+            *started = it;
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
@@ -629,8 +620,28 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         }
     }
 
+    // After an abort, whichever role's, no copy may outlive shared memory: each stage's last step started is
+    // waited for.  (The steps before it have landed: their MMAs are what freed the stage.)  The CTAs of a
+    // pair may have stopped at different steps, up to a ring apart: rank 0, whose barriers count both,
+    // expects the peer's bytes of a step that only the peer has started, and counts off those of one that
+    // only itself has.
+    auto drain_copies = [&](int mine, int peers) {
+        const uint32_t bytes = (uint32_t)((p.x_rows + w_rows) * kFp8Block);
+        const int last = mine > peers ? mine : peers;
+        for (int j = last < p.stages ? 0 : last - p.stages; j < last; ++j) {
+            if (j == 0 && withhold) continue;
+            uint64_t* bar = full + j % p.stages;
+            if (j >= peers) mbar_complete_tx(bar, bytes);
+            else if (j >= mine) mbar_arrive_expect_tx(bar, bytes);
+            mbar_wait_drain(bar, (uint32_t)((j / p.stages) & 1));
+        }
+    };
     tc_fence_before();
     __syncthreads();
+    if (!PAIR && *abort_flag) {
+        if (threadIdx.x == 0) drain_copies(*started, *started);
+        __syncthreads();
+    }
     if constexpr (SPLIT) {
         // ------------------------------------------------------------ output of a shared tile
         // Every CTA's copies and MMAs are done: the operand rings are free for the exchange.  Piece
@@ -765,7 +776,15 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         tc_fence_before();
         __syncthreads();
     }
-    if (PAIR) cluster_sync();                    // no MMA, copy or arrival still needs the peer
+    if constexpr (PAIR) {
+        // An abort of one CTA is the pair's; both end when its copies have landed.
+        if (threadIdx.x == 0 && *abort_flag) st_cluster_4(cluster_addr(const_cast<int*>(abort_flag), rank ^ 1), 1);
+        cluster_sync();                          // no MMA or arrival still needs the peer
+        if (*abort_flag) {
+            if (rank == 0 && threadIdx.x == 0) drain_copies(*started, ld_cluster_4(cluster_addr(started, 1)));
+            cluster_sync();
+        }
+    }
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();

@@ -21,7 +21,8 @@ constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s
 // its own copy, and the hook sets each): the limit the waits use (kWaitLimitNs unless a test
 // shortened it), and a switch that makes the weight producer of every CTA skip its first copy
 // together with the arrival that goes with it, so that the consumers' wait on that stage runs
-// out and the abort path (status bit, drain, TMEM release, early return) is taken.
+// out and the abort path (status bit, drain, TMEM release, early return) is taken.  (2 or 3: the second
+// or the first CTA of a pair starts nothing at all.)
 static __device__ unsigned long long g_wait_limit_ns = kWaitLimitNs;
 static __device__ int g_withhold_first_copy = 0;
 
@@ -350,6 +351,19 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
 __device__ __forceinline__ void st_cluster_16(uint32_t addr, float4 v) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                  : "memory");
+}
+// A word of any CTA's shared memory.
+__device__ __forceinline__ void st_cluster_4(uint32_t addr, int v) {
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ int ld_cluster_4(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+// Take `bytes` off what this CTA's barrier still expects, as their copy would have.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 // One arrival on a barrier of either CTA of the cluster, by its shared::cluster address.  It
 // releases at CTA scope: what it orders are accesses to this CTA's own shared and tensor memory

@@ -249,11 +249,11 @@ def device_status(stream=None) -> None:
     check(lib().sdq_device_status(_stream(stream)))
 
 
-def debug_wait_hook(wait_limit_ns: int = 0, withhold_first_copy: bool = False, stream=None) -> None:
+def debug_wait_hook(wait_limit_ns: int = 0, withhold_first_copy: bool | int = False, stream=None) -> None:
     """Testing hook (``sdq_debug_wait_hook``): shorten the kernels' bounded waits to
     ``wait_limit_ns`` (0 restores 2 s) and, with ``withhold_first_copy``, make every CTA's
-    weight producer skip its first copy so that the abort path runs."""
-    check(lib().sdq_debug_wait_hook(ctypes.c_uint64(wait_limit_ns), int(bool(withhold_first_copy)),
+    weight producer skip its first copy so that the abort path runs (2 or 3: see the header)."""
+    check(lib().sdq_debug_wait_hook(ctypes.c_uint64(wait_limit_ns), int(withhold_first_copy),
                                     _stream(stream)))
 
 

@@ -4,6 +4,8 @@ is smaller than the others -- each against 64 bits on every row, with the plan a
 tile choice cannot leave a form without a test.  Tolerances as derived in test_gpu_fp8.py."""
 from __future__ import annotations
 
+import time
+
 import pytest
 import torch
 
@@ -100,3 +102,31 @@ def test_activations_of_each_plan(shape, wanted, several, ragged, act):
     y = sdq.fp8_matmul(*ops, bias=bias, act=act)
     check(y, a, 1.13 * (sums_tol(s, k) + v.abs() * 2.0 ** -23) + 2.0 ** -10 * (1 + v.abs()) + a.abs() * 2.0 ** -8)
     sdq.device_status()
+
+
+@pytest.mark.parametrize("withhold", [1, 2, 3])
+@pytest.mark.parametrize("shape,wanted,several,ragged", [
+    ((300, 4096, 4096), PAIRS, False, False), ((300, 2640, 4099), PAIRS, False, False), ((9000, 4112, 1024), PAIRS, True, True),
+    ((2100, 272, 3008), SINGLE, True, False), ((7, 9728, 2560), SHARED, False, False)])
+def test_waits_that_run_out_in_each_plan(shape, wanted, several, ragged, withhold):
+    """As test_gpu_abort.py, without a fault: each CTA withholds its first copy, or one CTA of a pair all of
+    its copies; the waits give up, what was started lands, and the next call is right."""
+    m, k, n = shape
+    expect(shape, wanted, several, ragged)
+    ops = operands(m, m, k, n)
+    want = sdq.fp8_matmul(*ops)
+    sdq.device_status()
+    for _ in range(2):
+        sdq.debug_wait_hook(20_000_000, withhold)
+        try:
+            t0 = time.monotonic()
+            sdq.fp8_matmul(*ops)
+            torch.cuda.synchronize()
+            elapsed = time.monotonic() - t0
+            with pytest.raises(sdq.SdqError, match="gave up"):
+                sdq.device_status()
+        finally:
+            sdq.debug_wait_hook(0, False)
+        assert elapsed < 1.0, elapsed                      # one 20 ms limit; the copies land at once
+        assert torch.equal(sdq.fp8_matmul(*ops), want)
+        sdq.device_status()
