@@ -64,6 +64,18 @@ def _need_cuda(*ts):
             raise SdqError(SDQ_ERR_INVALID, "libsdq takes contiguous row-major tensors")
 
 
+def _like_result(dtype: torch.dtype, n: int | None, **ts):
+    """The kernels read these as the result's type, whatever the tensors hold: ``n`` values each (None:
+    counted by the caller)."""
+    for name, t in ts.items():
+        if t is None:
+            continue
+        if t.dtype != dtype:
+            raise SdqError(SDQ_ERR_INVALID, f"{name} must be {dtype} like the result, not {t.dtype}")
+        if n is not None and t.numel() != n:
+            raise SdqError(SDQ_ERR_INVALID, f"{name} holds {t.numel()} values, the layer has {n} outputs")
+
+
 def quantize(w: torch.Tensor, group_size: int = GROUP_SIZE, bits: int = 4, stream=None,
              sb_dtype=torch.bfloat16):
     """``mlx_quantize`` replacement: w [n, k] f32/bf16 -> (wq u32 [n, k*bits/32] as int32,
@@ -112,7 +124,10 @@ def quantized_matmul(x: torch.Tensor, wq, scales, biases, group_size: int = GROU
 
     A 3-D ``x`` ([b, s, k]) is flattened to M = b*s rows, as MLX does.  ``x``, the scales and
     the result may each be bf16 or f32; the result defaults to ``x``'s dtype.  f32 inputs are
-    rounded to bf16 for the tensor cores; an f32 result is the f32 accumulator, unrounded."""
+    rounded to bf16 for the tensor cores; an f32 result is the f32 accumulator, unrounded.
+    ``bias`` holds n values of the result's dtype."""
+    ydt = out.dtype if out is not None else torch.float32 if x.dtype == torch.float32 else torch.bfloat16
+    _like_result(ydt, wq.shape[0], bias=bias)
     _need_cuda(x, wq, scales, biases, bias, out)
     lead = x.shape[:-1]
     k = x.shape[-1]
@@ -121,8 +136,7 @@ def quantized_matmul(x: torch.Tensor, wq, scales, biases, group_size: int = GROU
         m *= d
     n = wq.shape[0]
     if out is None:
-        out = torch.empty((*lead, n), device=x.device,
-                          dtype=torch.float32 if x.dtype == torch.float32 else torch.bfloat16)
+        out = torch.empty((*lead, n), device=x.device, dtype=ydt)
     check(lib().sdq_quantized_matmul(_ptr(x), _dt(x), m, k, _ptr(wq), _ptr(scales), _ptr(biases),
                                      _dt(scales), n, 1, group_size, bits, MODE.encode(), _ptr(bias),
                                      _ptr(out), _dt(out), _stream(stream)))
@@ -137,6 +151,8 @@ def quantized_matmul_host(x_host: torch.Tensor, wq, scales, biases, group_size: 
     the rows go up, through the product and back down in overlapped chunks.  ``x_host`` and
     ``out`` are CPU tensors (pinned for the copies to overlap); ``x_dev`` / ``y_dev`` are the
     device workspaces (allocated here when not given).  Asynchronous on ``stream``."""
+    ydt = torch.float32 if x_host.dtype == torch.float32 else torch.bfloat16
+    _like_result(ydt if out is None else out.dtype, wq.shape[0], bias=bias)
     _need_cuda(wq, scales, biases, bias, x_dev, y_dev)
     if x_host.is_cuda or not x_host.is_contiguous():
         raise SdqError(SDQ_ERR_INVALID, "x_host must be a contiguous CPU tensor")
@@ -146,7 +162,6 @@ def quantized_matmul_host(x_host: torch.Tensor, wq, scales, biases, group_size: 
     for d in lead:
         m *= d
     n = wq.shape[0]
-    ydt = torch.float32 if x_host.dtype == torch.float32 else torch.bfloat16
     if out is None:
         out = torch.empty((*lead, n), dtype=ydt, pin_memory=True)
     if out.is_cuda or not out.is_contiguous():
@@ -177,6 +192,7 @@ def quantized_matmul_epilogue(x: torch.Tensor, wq, scales, biases, group_size: i
     output's shape.  ``out`` may be ``residual`` itself (an in-place residual update)."""
     if act not in _ACTS:
         raise SdqError(SDQ_ERR_INVALID, f"unknown activation {act!r}")
+    _like_result(torch.bfloat16, None, bias=bias, gate=gate, residual=residual)
     _need_cuda(x, wq, scales, biases, bias, gate, residual, out)
     lead = x.shape[:-1]
     k = x.shape[-1]
@@ -377,6 +393,7 @@ def quantized_matmul_sharded(x, wq, scales, biases, comm: Comm, group_size: int 
 
     Returns ``(out, y_shards)``; ``out`` is None when ``permute`` is False (the caller then
     reads the blocked [world, m, n_local] layout from ``y_shards``)."""
+    _like_result(torch.bfloat16, wq.shape[0], bias=bias)
     _need_cuda(x, wq, scales, biases, bias)
     m, k = x.reshape(-1, x.shape[-1]).shape
     nl = wq.shape[0]

@@ -44,3 +44,32 @@ def test_quantizable_rule():
     assert not Q.quantizable((32, 100))     # 100 does not divide by 64
     assert not Q.quantizable((2, 3, 64))
     assert Q.GROUP_SIZE == 64 and Q.DEFAULT_BITS == 4
+
+
+def test_a_bias_of_another_type_than_the_result_is_refused():
+    """The kernels read a bias, a gate and a residual as the result's type."""
+    import torch
+
+    import sdq
+
+    x, wq = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(8, 8, dtype=torch.int32)
+    sb, wide, narrow = torch.zeros(8, 1, dtype=torch.bfloat16), torch.zeros(8), torch.zeros(8, dtype=torch.bfloat16)
+    out = torch.zeros(4, 8)
+    calls = [
+        lambda: sdq.quantized_matmul(x, wq, sb, sb, bias=wide),
+        lambda: sdq.quantized_matmul(x.float(), wq, sb, sb, bias=narrow),
+        lambda: sdq.quantized_matmul(x, wq, sb, sb, bias=narrow, out=out),
+        lambda: sdq.quantized_matmul_host(x, wq, sb, sb, bias=wide),
+        lambda: sdq.quantized_matmul_host(x, wq, sb, sb, bias=narrow, out=out),
+        lambda: sdq.quantized_matmul_epilogue(x, wq, sb, sb, bias=wide),
+        lambda: sdq.quantized_matmul_epilogue(x, wq, sb, sb, gate=wide),
+        lambda: sdq.quantized_matmul_epilogue(x, wq, sb, sb, residual=out),
+        lambda: sdq.quantized_matmul_sharded(x, wq, sb, sb, None, bias=wide),
+    ]
+    for call in calls:
+        with pytest.raises(sdq.SdqError, match="like the result"):
+            call()
+    for call in (lambda: sdq.quantized_matmul(x, wq, sb, sb, bias=narrow[:7]),
+                 lambda: sdq.quantized_matmul_host(x, wq, sb, sb, bias=narrow[:7])):
+        with pytest.raises(sdq.SdqError, match="7 values"):
+            call()
