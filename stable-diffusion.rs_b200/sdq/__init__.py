@@ -16,7 +16,8 @@ from dataclasses import dataclass
 import torch
 
 from ._abi import (SDQ_BF16, SDQ_ERR_CUDA, SDQ_ERR_INVALID, SDQ_ERR_NCCL, SDQ_ERR_TIMEOUT,
-                   SDQ_ERR_UNSUPPORTED, SDQ_F16, SDQ_F32, SDQ_OK, SdqError, check, last_error, lib)
+                   SDQ_ERR_UNSUPPORTED, SDQ_F16, SDQ_F32, SDQ_OK, SdqError, as_result, check, last_error,
+                   lib)
 
 __all__ = [
     "SdqError", "QuantizedArray", "quantize", "dequantize", "quantized_matmul", "quantized_matmul_epilogue",
@@ -301,14 +302,19 @@ class QuantizedArray:
     def matmul(self, x: torch.Tensor, bias: torch.Tensor | None = None, stream=None,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """``x @ weight.T``, dequantising inside the kernel (mlx.rs:1947-1975); ``out``, if
-        given, receives the result."""
+        given, receives the result.  A bias of another float type than the result's (a checkpoint's
+        f32 beside bf16 activations) is converted for the call."""
+        ydt = out.dtype if out is not None else torch.float32 if x.dtype == torch.float32 else torch.bfloat16
+        bias = as_result(bias, ydt, stream)
         return quantized_matmul(x, self.weight, self.scales, self.biases, self.group_size, self.bits,
                                 bias=bias, out=out, stream=stream)
 
     def matmul_fused(self, x: torch.Tensor, bias=None, act=None, gate=None, residual=None,
                      out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
         """``residual + gate * act(x @ weight.T + bias)`` in one kernel (see
-        :func:`quantized_matmul_epilogue`)."""
+        :func:`quantized_matmul_epilogue`).  A bias or gate of another float type is converted for
+        the call."""
+        bias, gate = (as_result(t, torch.bfloat16, stream) for t in (bias, gate))
         return quantized_matmul_epilogue(x, self.weight, self.scales, self.biases, self.group_size,
                                          self.bits, bias=bias, act=act, gate=gate, residual=residual,
                                          out=out, stream=stream)

@@ -7,10 +7,11 @@ every call raises :class:`SdqError`.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
-import torch  # noqa: F401  (the shortcut below links against its libraries)
+import torch  # (the shortcut below links against its libraries)
 
 try:
     from . import _native
@@ -119,3 +120,31 @@ def last_error() -> str:
 def check(rc: int) -> None:
     if rc != SDQ_OK:
         raise SdqError(rc, last_error())
+
+
+@contextlib.contextmanager
+def on(stream, device: torch.device):
+    """``device`` current and, where it is not None, ``stream`` (a torch stream or a raw handle).  What is
+    copied, allocated and dropped between kernels then belongs to the stream that these run on: the
+    allocator hands a dropped block on at once, in the order of that stream."""
+    if device.type != "cuda":
+        yield
+        return
+    with torch.cuda.device(device):
+        if stream is None:
+            yield
+            return
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(int(stream))
+        if stream.device_index != torch.cuda.current_device():
+            raise SdqError(SDQ_ERR_INVALID, f"a stream of {stream.device} cannot run work on {device}")
+        with torch.cuda.stream(stream):
+            yield
+
+
+def as_result(t, dtype: torch.dtype, stream=None):
+    """A bias or gate (or None) in the result's type, which is what the kernels read."""
+    if t is None or t.dtype == dtype or not t.is_floating_point():
+        return t
+    with on(stream, t.device):
+        return t.to(dtype)

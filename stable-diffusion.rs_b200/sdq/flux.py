@@ -230,10 +230,11 @@ def attention(q, k, v):
 
 def prepare_heads(w, qkv, heads, hd, norm, cos, sin, out=None):
     """Queries, keys and values [b, heads, n, hd] of a fused projection [b, n, 3 * heads * hd] (a view
-    of a wider one will do), normed with ``norm``'s scales and rotated; into ``out`` if given."""
+    of a wider one will do), normed with ``norm``'s scales (in qkv's type: a checkpoint's f32 ones are
+    rounded) and rotated; into ``out`` if given."""
     q, k, v = qkv.unflatten(-1, (3, heads, hd)).unbind(2)
-    return qk_norm_rope(q, k, v, w.dense_tensor(f"{norm}.query_norm.scale"), w.dense_tensor(f"{norm}.key_norm.scale"),
-                        cos, sin, EPS, out=out)
+    scales = (w.dense_tensor(f"{norm}.{which}_norm.scale").to(qkv.dtype) for which in ("query", "key"))
+    return qk_norm_rope(q, k, v, *scales, cos, sin, EPS, out=out)
 
 
 def double_block(w, img, txt, vec, cos, sin, i, cfg: FluxShape, fused_heads=False):

@@ -19,7 +19,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _ACTS
-from ._abi import SDQ_BF16, SDQ_ERR_INVALID, SDQ_ERR_UNSUPPORTED, SDQ_F32, SdqError, check, lib, native
+from ._abi import SDQ_BF16, SDQ_ERR_INVALID, SDQ_ERR_UNSUPPORTED, SDQ_F32, SdqError, as_result, check, lib, native, on
 
 #: Values that share a scale, along a row (activations) or both ways (weights).
 BLOCK = 128
@@ -38,14 +38,7 @@ def _elsewhere(fn, device, stream, *args, **kw):
     """``fn`` again with ``stream`` current (allocations included), or on another device."""
     if device.type != "cuda":
         raise SdqError(SDQ_ERR_INVALID, "libsdq takes device tensors (no CPU fallback)")
-    if stream is not None:
-        if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream), device=device)
-        if stream.device != device:
-            raise SdqError(SDQ_ERR_INVALID, f"a stream of {stream.device} cannot run work on {device}")
-        with torch.cuda.device(device), torch.cuda.stream(stream):
-            return fn(*args, **kw)
-    with torch.cuda.device(device):
+    with on(stream, device):
         return fn(*args, **kw)
 
 
@@ -190,15 +183,19 @@ class Fp8Array:
         return fp8_dequantize(self.weight, self.scales, True, out_dtype, stream)
 
     def matmul(self, x: torch.Tensor, bias=None, stream=None, out=None) -> torch.Tensor:
-        """``x @ weight.T`` (+ bias) in x's type or ``out``'s, x [..., k] bf16 or f32."""
+        """``x @ weight.T`` (+ bias) in x's type or ``out``'s, x [..., k] bf16 or f32.  A bias of another
+        float type is converted for the call."""
         xq, xs = fp8_quantize(x, stream)
+        bias = as_result(bias, x.dtype if out is None else out.dtype, stream)
         return fp8_matmul(xq, xs, self.weight, self.scales, bias=bias, out=out, out_dtype=x.dtype if out is None else None,
                           stream=stream)
 
     def matmul_fused(self, x: torch.Tensor, bias=None, act=None, gate=None, residual=None, out=None,
                      stream=None) -> torch.Tensor:
-        """``residual + gate * act(x @ weight.T + bias)``, rounded to bf16 once."""
+        """``residual + gate * act(x @ weight.T + bias)``, rounded to bf16 once.  A bias or gate of another
+        float type is converted for the call."""
         xq, xs = fp8_quantize(x, stream)
+        bias, gate = (as_result(t, torch.bfloat16 if out is None else out.dtype, stream) for t in (bias, gate))
         return fp8_matmul(xq, xs, self.weight, self.scales, bias=bias, act=act, gate=gate, residual=residual, out=out,
                           stream=stream)
 

@@ -8,7 +8,6 @@ the same errors, with `QuantizedArray` backed by libsdq instead of MLX.  Dense
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Callable, Dict, Mapping, Optional, Protocol, Union
 
 import torch
@@ -16,6 +15,7 @@ import torch.nn.functional as F
 
 from . import ACT_GELU_TANH, ACT_NONE, ACT_SILU, Fp8Array, QuantizedArray, SdqError
 from ._abi import SDQ_ERR_INVALID
+from ._abi import on as _on
 
 #: MLX's default group size; must divide the weight's input width (quantized.rs:45-46).
 GROUP_SIZE = 64
@@ -114,26 +114,6 @@ def quantizable(shape) -> bool:
 def fp8_quantizable(shape) -> bool:
     """2-D with rows of whole 16-byte pieces, the block-scaled form's only condition."""
     return len(shape) == 2 and shape[0] > 0 and shape[1] > 0 and shape[1] % 16 == 0
-
-
-@contextlib.contextmanager
-def _on(stream, device: torch.device):
-    """``device`` current and, where it is not None, ``stream`` (a torch stream or a raw handle).  What a
-    loader copies, allocates and drops between its kernels then belongs to the stream that these run on:
-    the allocator hands a dropped block on at once, in the order of that stream."""
-    if device.type != "cuda":
-        yield
-        return
-    with torch.cuda.device(device):
-        if stream is None:
-            yield
-            return
-        if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream))
-        if stream.device_index != torch.cuda.current_device():
-            raise SdqError(SDQ_ERR_INVALID, f"a stream of {stream.device} cannot run work on {device}")
-        with torch.cuda.stream(stream):
-            yield
 
 
 def quantize_to(w: torch.Tensor, bits: Bits, stream=None) -> Union[QuantizedArray, Fp8Array, None]:
