@@ -161,7 +161,9 @@ int sdq_quantized_matmul_host(const void* x_host, sdq_dtype x_dtype, int64_t m, 
  * with the linear being quantized::linear (quantized.rs:298-318).
  * gate and bias are [n] bf16, residual [m, n] bf16 (row-major, contiguous).
  * residual may be y itself (in-place update of a residual stream) but must
- * not otherwise overlap y.  The other arguments and the dispatch (small-M
+ * not otherwise overlap y.  GELU goes by the hardware's tanh, which may be off by 2^-11,
+ * so that the value is by up to |a| 2^-12: more than bf16's rounding below about a = -3.
+ * The other arguments and the dispatch (small-M
  * weight stream for m <= 8, tensor cores otherwise) are those of
  * sdq_quantized_matmul with transpose = 1 and mode "affine".
  */
@@ -206,7 +208,9 @@ int sdq_fp8_dequantize(const uint8_t* q, const uint8_t* scales, int64_t rows, in
 
 /*
  * y[t,f] = residual[t,f] + gate[f] * act( sum_k X[t,k] W[f,k] + bias[f] ), X and W the values that
- * xq / x_scales and wq / w_scales stand for; products and sums in f32, one rounding to y_dtype.
+ * xq / x_scales and wq / w_scales stand for; products and sums in f32, one rounding to y_dtype.  The
+ * activations are as exact as that rounding needs; arguments below -43 (SiLU) or -7.6 (GELU) have the value
+ * there, under 10^-17.
  * bias, gate, residual may be NULL (0, 1, 0); act is one of SDQ_ACT_*.  With y bf16, bias and gate
  * are [n] bf16 and residual [m,n] bf16 (residual may be y itself, but not otherwise overlap it).
  * With y f32 only a bias ([n] f32) may be given.  y overlaps no other input.  m may be 0.  xq and wq

@@ -8,8 +8,9 @@
 //   silu         a * sigmoid(a) = a / (1 + e^-a)   (mlx.rs:697-705)
 // The epilogue runs while the tile's accumulator is held, so its per-element cost delays
 // the next tile's MMAs: tanh is the hardware approximation (PTX tanh.approx.f32, maximum
-// relative error about 2^-11, below bf16's 2^-9 rounding step) and the sigmoid uses
-// __expf and a fast divide.  The reference itself evaluates both chains op by op in bf16.
+// relative error about 2^-11, below bf16's 2^-9 rounding step; of negative arguments 1 + tanh
+// cancels, and below about -3 the error, up to |a| 2^-12, exceeds that step) and the sigmoid
+// uses __expf and a fast divide.  The reference itself evaluates both chains op by op in bf16.
 #pragma once
 
 #include <cstdint>

@@ -115,29 +115,45 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)), "l"(pack2(c)));
     return unpack2(r);
 }
-// epi_activation's GELU of two values: a (1 + tanh(a (c + 0.044715 c a^2))) / 2, c = sqrt(2/pi),
-// with the same hardware tanh, in packed arithmetic.
-__device__ __forceinline__ float2 gelu2(float2 a) {
-    const float c = 0.7978845608028654f, k = 0.044715f * c;
-    const float2 arg = mul2(a, fma2(mul2(a, a), make_float2(k, k), make_float2(c, c)));
-    const float2 h = mul2(a, make_float2(0.5f, 0.5f));
-    return fma2(h, make_float2(tanh_approx(arg.x), tanh_approx(arg.y)), h);
-}
-
-// Its SiLU of two values, a / (1 + 2^(-a log2 e)), with the hardware exponential and one reciprocal for
-// both: 1 / d0 = d1 (1 / (d0 d1)).  Below -43 a stands for -43, so that the product stays finite; the
-// value there is under 10^-17 either way.  (The special function unit sets the output stage's pace:
-// 3 of its operations for two values instead of 4.)
-__device__ __forceinline__ float2 silu2(float2 a) {
-    float2 d = mul2(make_float2(fmaxf(a.x, -43.f), fmaxf(a.y, -43.f)), make_float2(-1.4426950408889634f, -1.4426950408889634f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a.x) : "f"(-43.f));         // a NaN stays, but out of d, which the two share
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a.y) : "f"(-43.f));
+// Both activations are a / (1 + 2^x): SiLU with x = -a log2 e, GELU (tanh form), a (1 + tanh u) / 2 with
+// u = sqrt(2/pi) (a + 0.044715 a^3), with x = -2u log2 e.  Nothing cancels, so a value keeps its relative
+// accuracy.  (1 + tanh u by the hardware's tanh does: at a = -4 its 2^-11 is fourteen times 1 + tanh u.
+// It takes two special functions for two values, this three: GELU of 3116 x 48 x 4176 15.4 us, 16.9 here, and
+// 18.2 with a reciprocal for each value, which needs no LEAST.)
+// For two values, with the hardware's exponential and one reciprocal for both, 1 / d0 = d1 (1 / (d0 d1)):
+// the special function unit sets the output stage's pace.  So that the product stays finite an a below LEAST,
+// where 2^x is 2^62, stands for LEAST; the value there is under 10^-17 either way.
+template <class F>
+__device__ __forceinline__ float2 over_one_plus_exp2(float2 a, float least, F exponent) {
+    float2 d = exponent(make_float2(fmaxf(a.x, least), fmaxf(a.y, least)));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a.x) : "f"(least));         // a NaN stays, but out of d, which the two share
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a.y) : "f"(least));
     float r;
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d.x));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d.y));
     d = add2(d, make_float2(1.f, 1.f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d.x * d.y));
     return mul2(a, mul2(make_float2(d.y, d.x), make_float2(r, r)));
+}
+__device__ __forceinline__ float2 gelu2(float2 a) {
+    return over_one_plus_exp2(a, -7.6f, [](float2 v) {
+        const float c = -2.f * 0.7978845608028654f * 1.4426950408889634f, k = 0.044715f * c;
+        return mul2(v, fma2(mul2(v, v), make_float2(k, k), make_float2(c, c)));
+    });
+}
+__device__ __forceinline__ float2 silu2(float2 a) {
+    return over_one_plus_exp2(a, -43.f, [](float2 v) { return mul2(v, make_float2(-1.4426950408889634f, -1.4426950408889634f)); });
+}
+// The activation of N pairs of values; one decision a piece, not one a value.
+template <int N>
+__device__ __forceinline__ void activate(float2 (&o)[N], int act) {
+    if (act == SDQ_ACT_GELU_TANH) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = gelu2(o[j]);
+    } else if (act == SDQ_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = silu2(o[j]);
+    }
 }
 
 // ANY: rows of y that do not start on 32 bytes (a kernel of its own: the two output stages in one cost
@@ -520,14 +536,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                         o[j] = add2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), make_float2(b.x, b.y));
                         o[j + 1] = add2(make_float2(__uint_as_float(v[2 * j + 2]), __uint_as_float(v[2 * j + 3])), make_float2(b.z, b.w));
                     }
-                    if (FUSED) {                                    // one decision a piece, not one a value
-                        if (epi.act == SDQ_ACT_GELU_TANH) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = gelu2(o[j]);
-                        } else if (epi.act == SDQ_ACT_SILU) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = silu2(o[j]);
-                        }
+                    if (FUSED) {
+                        activate(o, epi.act);
                         if (epi.gate != nullptr) {
 #pragma unroll
                             for (int j = 0; j < 16; ++j) o[j] = mul2(o[j], *reinterpret_cast<const float2*>(sgate + 256 * buf + c + 2 * j));
@@ -721,13 +731,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = add2(o[j], *reinterpret_cast<const float2*>(sbias + 16 * piece + 2 * j));
                 if (FUSED) {
-                    if (epi.act == SDQ_ACT_GELU_TANH) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) o[j] = gelu2(o[j]);
-                    } else if (epi.act == SDQ_ACT_SILU) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) o[j] = silu2(o[j]);
-                    }
+                    activate(o, epi.act);
                     if (epi.gate != nullptr) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) o[j] = mul2(o[j], *reinterpret_cast<const float2*>(sgate + 16 * piece + 2 * j));

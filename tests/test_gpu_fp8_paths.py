@@ -130,3 +130,28 @@ def test_waits_that_run_out_in_each_plan(shape, wanted, several, ragged, withhol
         assert elapsed < 1.0, elapsed                      # one 20 ms limit; the copies land at once
         assert torch.equal(sdq.fp8_matmul(*ops), want)
         sdq.device_status()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_approx"])
+@pytest.mark.parametrize("shape,wanted", [((1, 16, 65280), SINGLE), ((3, 16, 65279), SINGLE), ((300, 4096, 65280), PAIRS), ((300, 4096, 65277), PAIRS),
+                                          ((16, 8192, 1020), SHARED), ((16, 8192, 1008), SHARED)])
+def test_activations_of_every_bf16_number(shape, wanted, act):
+    """A product of zeros, so that the bias is the activation's exact argument: every finite bf16 number (of
+    shared tiles, every 64th).  The exponential's argument, at most 64 where it matters, is rounded four times and
+    its constants once each, 5 x 2^-24 of it, which gives 64 x 5 x 2^-24 ln 2 < 2^-16 of the value; exponential,
+    reciprocal and products some 2^-21.  Rounding to bf16 is off by 2^-8 of a result at most, and by 2^-134 of one
+    below 2^-126, where its numbers are 2^-133 apart.  Arguments below -43 and -7.6 have the value there,
+    43 e^-43 < 2^-56 and 7.6 e^-43 < 2^-59."""
+    m, k, n = shape
+    expect(shape, wanted, wanted == PAIRS or n > 60000 and sdq.debug_fp8_plan(m, k, n, True, n % 16 == 0)["tiles"] > 148, False, True)
+    every = torch.arange(65536, device="cuda", dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    every = every[every.isfinite()]
+    bias = every[:n] if n > 60000 else every[5::64][:n].contiguous()
+    ops = (*sdq.fp8_quantize(torch.zeros(m, k, device="cuda")), *sdq.fp8_quantize_weight(normals(1, n, k)))
+    v = bias.double()
+    a = v * torch.sigmoid(v if act == "silu" else 2 * (2 / torch.pi) ** 0.5 * (v + 0.044715 * v ** 3))
+    low, most = (-43, 2.0 ** -56) if act == "silu" else (-7.6, 2.0 ** -59)
+    tol = a.abs() * (2.0 ** -8 + 2.0 ** -14) + 2.0 ** -134 + torch.where(v < low, most, 0.0)
+    y = sdq.fp8_matmul(*ops, bias=bias, act=act)
+    check(y, a.expand(m, n), tol.expand(m, n))
+    sdq.device_status()
