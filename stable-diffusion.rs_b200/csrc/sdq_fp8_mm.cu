@@ -16,12 +16,12 @@
 //
 // Where the tiles leave SMs idle and K is long, a cluster of 2, 4 or 8 CTAs shares one tile's K (SPLIT):
 // each accumulates its steps, then they exchange pieces of 16 features through one another's shared
-// memory, each adding up (in the order of K) and storing its own.  1 x 9728 x 2560: 15.0 -> 9.0 us.
+// memory, each adding up (in the order of K) and storing its own.  1 x 9728 x 2560: 14.8 -> 9.2 us.
 //
 // One kernel for every number of tokens.  For a few of them a stream of the weight through mma.sync
 // was measured beside it and is not kept: its e4m3 form is emulated on sm_100a (170 cycles each), and
 // with the codes turned into f16 the conversion sets the pace (1 x 2560 x 9728: 14.3 us by the
-// conversion instruction, 18.7 by shifts, 7.3 here, where nothing is unpacked).
+// conversion instruction, 18.7 by shifts, 7.1 here, where nothing is unpacked).
 //
 // Warp roles (512 threads, one CTA per SM, persistent over tiles):
 //   warp 0       TMA producer of the operand ring (one thread)
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         // take a token's piece.  What is over of a piece (row t's chunks start `over` values before
         // feature c) waits for the next one in front of it.  What the half's ends leave of a chunk is
         // stored by a lane a token.  (All of it by 2 bytes a lane, 64 bytes of a token a warp,
-        // took much longer: 3907 x 320 x 8597 with gate and residual 112 us, 66 this way.)
+        // took much longer: 3907 x 320 x 8597 with gate and residual 112 us, 65 this way.)
         constexpr int CHUNK = YF32 ? 4 : 8, LANES = 32 / CHUNK, TOKENS = 32 / LANES;
         float* mine = stage32 + (warp - 8) * 32 * kMaxPitch;
         const uint32_t y_off = (uint32_t)(reinterpret_cast<uintptr_t>(y) / (YF32 ? 4 : 2));
@@ -874,11 +874,12 @@ int clusters_at_once(int ctas) {
 // the copies (64 bytes a cycle from L2), not less than the weight's way from DRAM (3500 bytes a cycle);
 // beside them, a tile behind, the output stage (750 cycles for 64 features, as much again for an
 // activation, gate or residual, 1000 more for rows of any pitch), which of many short tiles sets the
-// pace; the last tile's, and a pair's later start or the exchange, on top.  Measured, us: 512 x 4096 x
-// 10240 pairs by 144 20.3 (CTAs by 144 21.8); 1 x 9728 x 2560 fours by 80 9.0 (CTAs by 32 15.0, twos by
-// 48 11.3, eights by 176 9.8); 16 x 8192 x 128 eights by 16 5.2 (CTAs by 64 12.2); 3116 x 48 x 4181
-// with SiLU CTAs by 224 26.0 (by 80 39.6).  Over some 60 shapes from 1 to 4608 tokens its choice was
-// within 5 % of the best, mostly 2 %.
+// pace; the last tile's, and a pair's later start or the exchange, on top.  Measured in a graph, us: 512 x
+// 4096 x 10240 with GELU pairs by 144 20.6 (CTAs by 144 22.3); 1 x 9728 x 2560 fours by 80 9.2 (CTAs by 48
+// 14.7, twos by 48 11.8, eights by 176 9.7); 16 x 8192 x 128 eights by 16 5.4 (fours 6.5, CTAs 12.3); 3116 x
+// 48 x 4181 with SiLU CTAs by 192 25.7 (by 80 35.2, pairs by 192 24.5).  Over 54 shapes from 1 to 4608
+// tokens, timed at every width and kind (profiles/fp8_tiles.md), its choice is at the best's time for half
+// of them, within 5 % for all but five and within 9 % for all.
 void choose(int64_t m, int64_t n, int64_t k, bool fused, bool aligned, bool& pair, int& bn, int& split) {
     const int64_t kt = (k + kFp8Block - 1) / kFp8Block, sms = num_sms();
     const int64_t dram = n * k / 3500;

@@ -81,8 +81,9 @@ __device__ __forceinline__ uint4 encode(const V& v, float inv) {
 
 // Activations: eight lanes take the 128 values of one group, a warp the same group of four
 // consecutive rows, so that the four scale bytes, which lie [group, row], share a sector; of bf16
-// it takes eight rows, for as many bytes under way as of f32.  4608 x 12288 bf16: 27.2 us (6.3 TB/s),
-// four rows 28.6, sixteen 29.5; f32 42.3 us (6.7 TB/s).
+// it takes eight rows, for as many bytes under way as of f32.  A dozen calls in a graph, at full clocks:
+// 4608 x 12288 bf16 27 us (6.3 TB/s), four rows 28.6, sixteen 29.5; f32 42 us (6.7 TB/s).  Call after call
+// the bf16 case takes 28.5 us (6.0 TB/s).
 template <bool BF16>
 __global__ void __launch_bounds__(256) fp8_quantize_rows(const void* __restrict__ x, int64_t m, int64_t k,
                                                          uint8_t* __restrict__ q, uint8_t* __restrict__ scales) {
@@ -113,8 +114,8 @@ __global__ void __launch_bounds__(256) fp8_quantize_rows(const void* __restrict_
     }
 }
 
-// Weights: one CTA per 128 x 128 block, four rows of 16 values per thread.  32768 x 5120 bf16: 74 us
-// (6.8 TB/s).
+// Weights: one CTA per 128 x 128 block, four rows of 16 values per thread.  32768 x 5120 bf16: 80 us call
+// after call (6.3 TB/s), 75 in a few calls at full clocks.
 template <bool BF16>
 __global__ void __launch_bounds__(256) fp8_quantize_blocks(const void* __restrict__ w, int64_t n, int64_t k,
                                                            uint8_t* __restrict__ q, uint8_t* __restrict__ scales) {

@@ -367,8 +367,11 @@ __device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) 
 }
 // One arrival on a barrier of either CTA of the cluster, by its shared::cluster address.  It
 // releases at CTA scope: what it orders are accesses to this CTA's own shared and tensor memory
-// before the ones that the observer then has made here.  (At cluster scope it waits for the SM's
-// memory operations in flight, and took some 3500 cycles.)
+// before the ones that the observer then has made here.  The memory model promises that order to
+// observers of this CTA only; that it holds for the other CTA's thread too, which touches this memory by
+// tensor-core instructions alone, is relied upon (with the proxy fence or the tcgen05 fence before the
+// arrival).  (At cluster scope it waits for the SM's memory operations in flight, and took some 3500
+// cycles.)
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }

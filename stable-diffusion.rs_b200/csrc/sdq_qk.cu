@@ -22,7 +22,8 @@
 // in the output.  The norm's weights are multiplied into the cosines and sines once for all the heads:
 // a c - b s becomes r (x0 (w0 c) - x1 (w1 s)), three operations a value.
 // 4608 tokens, 72 heads of 128: a block a token, looping over its heads, took 63 us (49 KB a SM
-// under way); this layout 40 with the norm and the rotation one after the other, now 30.8 (5.5 TB/s).
+// under way); this layout 40 with the norm and the rotation one after the other, now 30.9 in a graph and
+// 31.8 call after call (5.4 TB/s).
 // 4 x 8192 tokens with one query and one key head of 64: 35 us with a token a warp, 7.9 with four.
 #include <cstdint>
 #include <cuda_bf16.h>
