@@ -878,7 +878,7 @@ int clusters_at_once(int ctas) {
 // 4096 x 10240 with GELU pairs by 144 20.6 (CTAs by 144 22.3); 1 x 9728 x 2560 fours by 80 9.2 (CTAs by 48
 // 14.7, twos by 48 11.8, eights by 176 9.7); 16 x 8192 x 128 eights by 16 5.4 (fours 6.5, CTAs 12.3); 3116 x
 // 48 x 4181 with SiLU CTAs by 192 25.7 (by 80 35.2, pairs by 192 24.5).  Over 54 shapes from 1 to 4608
-// tokens, timed at every width and kind (profiles/fp8_tiles.md), its choice is at the best's time for half
+// tokens, timed at every width and kind, its choice is at the best's time for half
 // of them, within 5 % for all but five and within 9 % for all.
 void choose(int64_t m, int64_t n, int64_t k, bool fused, bool aligned, bool& pair, int& bn, int& split) {
     const int64_t kt = (k + kFp8Block - 1) / kFp8Block, sms = num_sms();
