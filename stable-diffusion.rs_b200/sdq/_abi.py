@@ -135,7 +135,9 @@ def on(stream, device: torch.device):
             yield
             return
         if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream))
+            handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+            # (torch takes a handle of 0, the default stream's, for none and hands out a stream of its own.)
+            stream = torch.cuda.ExternalStream(handle) if handle else torch.cuda.default_stream()
         if stream.device_index != torch.cuda.current_device():
             raise SdqError(SDQ_ERR_INVALID, f"a stream of {stream.device} cannot run work on {device}")
         with torch.cuda.stream(stream):

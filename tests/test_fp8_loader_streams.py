@@ -107,3 +107,46 @@ def test_transposed_weights_quantised_on_a_busy_stream(bits):
         assert torch.equal(held.quantized[name].weight.view(torch.uint8), q.weight.view(torch.uint8))
         assert torch.equal(held.quantized[name].scales.view(torch.uint8), q.scales.view(torch.uint8))
     assert len(other) == len(w)
+
+
+def test_which_stream_a_raw_handle_is(monkeypatch):
+    """0 is the default stream's handle, which torch's ExternalStream does not take for it."""
+    from sdq import _abi
+
+    here, used = contextlib.nullcontext(), []
+    monkeypatch.setattr(torch.cuda, "device", lambda d: here)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+
+    class Some:
+        device_index, device = 0, "cuda:0"
+
+        def __init__(self, name):
+            self.name = name
+
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle: Some(handle))
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda: Some("default"))
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: (used.append(s.name), here)[1])
+
+    class Foreign:
+        cuda_stream = 78
+
+    for given in (0, 77, Foreign()):
+        with _abi.on(given, torch.device("cuda", 0)):
+            pass
+    assert used == ["default", 77, 78]
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not gpu_available(), reason="needs an sm_100 device")
+def test_work_on_the_default_streams_handle_is_in_its_order():
+    x, w = torch.randn(300, 512, device="cuda"), sdq.Fp8Array.quantize(torch.randn(130, 512, device="cuda"))
+    q = torch.randn(2, 30, 4, 64, device="cuda")
+    new_x, new_q = torch.randn_like(x), torch.randn_like(q)
+    want = w.matmul(new_x), sdq.qk_norm_rope(new_q, new_q, eps=1e-6)[0]
+    assert torch.cuda.current_stream().cuda_stream == 0
+    busy(torch.cuda.current_stream())
+    x.copy_(new_x)
+    q.copy_(new_q)
+    got = w.matmul(x, stream=0), sdq.qk_norm_rope(q, q, eps=1e-6, stream=0)[0]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
