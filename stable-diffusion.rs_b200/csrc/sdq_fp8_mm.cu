@@ -161,7 +161,7 @@ __device__ __forceinline__ void activate(float2 (&o)[N], int act) {
 template <bool PAIR, bool SPLIT, bool FUSED, bool YF32, bool ANY>
 __global__ void __launch_bounds__(kMmThreads, 1)
     fp8_mm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
-                  const uint8_t* __restrict__ xs, const uint8_t* __restrict__ ws, const EpiArgs epi, void* y,
+                  const uint8_t* xs, const uint8_t* ws, const EpiArgs epi, void* y,
                   const __grid_constant__ MmPlan p) {
     constexpr int CG = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             for (int c = 0; c < 4; ++c) {
                 const uint8_t* x = xs + (int64_t)(kbase + kt0) * p.m + (t + 32 * c < p.m ? t + 32 * c : p.m - 1);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) raw[4 * c + q] = __ldg(x + (int64_t)step[q] * p.m);
+                for (int q = 0; q < 4; ++q) raw[4 * c + q] = x[(int64_t)step[q] * p.m];
             }
 #pragma unroll
             for (int c = 4; c < 12; ++c) {
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                 const int fc = f + 32 * (c - 4) < p.n ? f + 32 * (c - 4) : p.n - 1;
                 const uint8_t* row = ws + (int64_t)(fc / kFp8Block) * p.kt + kbase + kt0;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) raw[4 * c + q] = __ldg(row + step[q]);
+                for (int q = 0; q < 4; ++q) raw[4 * c + q] = row[step[q]];
             }
         };
 #pragma unroll

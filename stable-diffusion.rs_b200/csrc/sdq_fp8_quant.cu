@@ -85,8 +85,8 @@ __device__ __forceinline__ uint4 encode(const V& v, float inv) {
 // 4608 x 12288 bf16 27 us (6.3 TB/s), four rows 28.6, sixteen 29.5; f32 42 us (6.7 TB/s).  Call after call
 // the bf16 case takes 28.5 us (6.0 TB/s).
 template <bool BF16>
-__global__ void __launch_bounds__(256) fp8_quantize_rows(const void* __restrict__ x, int64_t m, int64_t k,
-                                                         uint8_t* __restrict__ q, uint8_t* __restrict__ scales) {
+__global__ void __launch_bounds__(256) fp8_quantize_rows(const void* x, int64_t m, int64_t k, uint8_t* q,
+                                                         uint8_t* scales) {
     constexpr int NQ = row_quads<BF16>();
     const int lane = threadIdx.x & 31;
     const uint32_t kb = (uint32_t)((k + kFp8Block - 1) / kFp8Block);

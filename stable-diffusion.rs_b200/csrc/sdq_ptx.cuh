@@ -177,7 +177,9 @@ __device__ __forceinline__ bool mbar_wait_drain(uint64_t* bar, uint32_t parity) 
 // kernel has completed and its memory operations are visible; nothing the earlier kernels
 // write may be read (or overwritten) before it.  griddep_launch_dependents() lets the next
 // kernel of the stream launch early (it still waits in its own griddep_wait()).  Without
-// the attribute both are no-ops.
+// the attribute both are no-ops.  What an earlier kernel may write is read by plain loads: the
+// non-coherent ones (__ldg, const __restrict__ parameters) are for data that nothing writes during
+// the kernel's life, and this life begins before the earlier kernel's end.
 __device__ __forceinline__ void griddep_wait() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }

@@ -183,8 +183,8 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
             const int64_t at = row * half + (INTER ? e / 2 : (low ? e : e - half));
 #pragma unroll
             for (int i = 0; i < NC / 4; ++i) {
-                const float4 cc = __ldg(reinterpret_cast<const float4*>(a.cos + at) + i);
-                const float4 ss = __ldg(reinterpret_cast<const float4*>(a.sin + at) + i);
+                const float4 cc = reinterpret_cast<const float4*>(a.cos + at)[i];
+                const float4 ss = reinterpret_cast<const float4*>(a.sin + at)[i];
                 c[4 * i] = cc.x; c[4 * i + 1] = cc.y; c[4 * i + 2] = cc.z; c[4 * i + 3] = cc.w;
                 s[4 * i] = ss.x; s[4 * i + 1] = ss.y; s[4 * i + 2] = ss.z; s[4 * i + 3] = ss.w;
             }
