@@ -597,6 +597,7 @@ int sdq_qk_norm_rope(const sdq_heads* q, const sdq_heads* k, const sdq_heads* v,
         a.in[i] = {in[i]->data, in[i]->batch_stride, in[i]->token_stride, in[i]->head_stride};
         a.out[i] = {out[i]->data, out[i]->batch_stride, out[i]->token_stride, out[i]->head_stride};
     }
+    if (all == 0 || batch == 0 || tokens == 0) return ok();              // tables of no rows may have no data
     if ((q_weight && !aligned(q_weight, 16)) || (k_weight && !aligned(k_weight, 16)))
         return fail(SDQ_ERR_INVALID, "%s: misaligned norm weight (16 bytes)", fn);
     if (rope_dim > 0) {
@@ -608,7 +609,6 @@ int sdq_qk_norm_rope(const sdq_heads* q, const sdq_heads* k, const sdq_heads* v,
             return fail(SDQ_ERR_INVALID, "%s: the tables have %lld rows for %lld tokens", fn, (long long)table_rows,
                         (long long)tokens);
     }
-    if (all == 0 || batch == 0 || tokens == 0) return ok();
     int rc;
     if ((rc = check_device())) return rc;
     a.weight[0] = q_weight;

@@ -67,3 +67,19 @@ def test_no_cpu_fallback():
     x = torch.zeros(1, 2, 4, 64)
     with pytest.raises(sdq.SdqError, match="no CPU fallback"):
         sdq.qk_norm_rope(x, x, x)
+
+
+@pytest.mark.parametrize("kwargs", [dict(n=0, cos=0, rows=0), dict(b=0, cos=0, rows=0), dict(qh=0, kh=0, no_v=True, cos=0, rows=0)])
+def test_nothing_to_do_needs_no_tables(kwargs):
+    assert _call(**kwargs) == _abi.SDQ_OK
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not gpu_available(), reason="needs an sm_100 device")
+def test_no_tokens_with_an_empty_part_of_the_tables():
+    """As a joint sequence's stream that holds nothing gives them: cos[0:0] has no address."""
+    q = torch.zeros(1, 0, 2, 64, device="cuda", dtype=torch.bfloat16)
+    w, table = torch.ones(64, device="cuda", dtype=torch.bfloat16), torch.zeros(5, 32, device="cuda")
+    joint = torch.full((3, 1, 2, 5, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+    got = sdq.qk_norm_rope(q, q, q, w, w, table[0:0], table[0:0], out=tuple(joint[:, :, :, 0:0]))
+    assert all(t.shape == (1, 2, 0, 64) for t in got) and (joint == 7).all()
