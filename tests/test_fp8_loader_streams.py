@@ -150,3 +150,18 @@ def test_work_on_the_default_streams_handle_is_in_its_order():
     got = w.matmul(x, stream=0), sdq.qk_norm_rope(q, q, eps=1e-6, stream=0)[0]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_stream_of_another_device_is_refused(monkeypatch):
+    from sdq import _abi
+
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle: handle)
+
+    class Handle:
+        cuda_stream = type("S", (), {"device_index": 1, "device": "cuda:1"})()
+
+    with pytest.raises(sdq.SdqError, match="cannot run work"):
+        with _abi.on(Handle(), torch.device("cuda", 0)):
+            pass

@@ -95,3 +95,26 @@ def test_chains_that_reuse_their_buffers():
     sdq.device_status()
     for g, w in zip(got, want):
         assert all(same(a, b) for again in g for a, b in zip(again, w))
+
+
+def test_calls_of_several_threads_at_once():
+    """The library's calls run without the interpreter's lock; each thread has a stream of its own."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    x = normals(21, 130, 528).to(torch.bfloat16)
+    ws = [sdq.Fp8Array.quantize(normals(22 + i, 3 * 4 * 64 + 16 * i, 528)) for i in range(4)]
+    heads = heads_case(torch.bfloat16, 1, 130, 4, 4, 64, "halves")
+    run = lambda w: (w.matmul(x), w.matmul_fused(x, act="silu"), *heads(), *sdq.fp8_quantize(x))  # noqa: E731
+    want = [run(w) for w in ws]
+    torch.cuda.synchronize()
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got = [run(ws[i]) for _ in range(25)]
+        s.synchronize()
+        return all(same(g, want[i]) for g in got)
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
+    sdq.device_status()
